@@ -46,6 +46,10 @@ extern "C" {
 /* GEMM output type additionally allows the raw accumulators */
 #define SAMQ_I32   3
 
+/* microscaled 4-bit floating point (e2m1 elements) */
+#define SAMQ_FP4_MX  0        /* blocks of 32 columns, scale a power of two (e8m0)    */
+#define SAMQ_FP4_NV  1        /* blocks of 16 columns, scale e4m3, times a global one */
+
 /* quantization granularity.  For activations these are the reference strings
  * "per_token" | "per_tensor" | "per_group_token"
  * (RTN_quantization/per_tensor_channel_group.py:130-140); for weights
@@ -270,6 +274,52 @@ int samq_matmul_i4(const uint8_t* A, const uint8_t* B, int64_t M, int64_t N, int
                    int32_t* C, int32_t* status, void* stream);
 int samq_sym_dequant_i32(const int32_t* q, const void* scale_row, const void* scale_col, int64_t rows, int64_t cols,
                          void* out, void* stream);
+
+/* ---- RMS norm with an 8-bit output -------------------------------------------------------------
+ *
+ * The norm in front of a quantized linear layer of a residual block, in one pass over the rows (the RMS-norm
+ * sibling of the LayerNorm prologue of samq_act_quant_i8_ex):
+ *     h = T(x + residual)                         rounded as it is stored; h = x without a residual
+ *     y = h * rsqrt(mean(h^2) + eps) * weight     fp32, not rounded to the tensor type
+ *     s = max(max|y|, 1e-5) / q_max,  q = round_half_even(y / s)     q_max = 2^(n_bits-1) - 1, n_bits 2..8
+ * x, residual, residual_out : [M, K] of `dtype`, row strides ldx, ldr, ldo elements; residual and residual_out
+ *     are given together or both NULL; residual_out may be residual or x itself (same stride), not overlap otherwise
+ * weight    : [K] of `dtype`
+ * q_out     : [M, K] int8 codes or NULL;  scale_out : [M] fp32 or NULL (what samq_gemm_i8 takes as ROW scales)
+ * fq_out    : [M, K] of `dtype`, the values q * s, or NULL
+ * A row with a NaN or an infinity gets a NaN scale and zero codes.  K <= 32768. */
+int samq_rms_norm_quant_i8(const void* x, const void* residual, const void* weight, int dtype, int64_t M, int64_t K,
+                           int64_t ldx, int64_t ldr, float eps, int n_bits, void* residual_out, int64_t ldo,
+                           int8_t* q_out, float* scale_out, void* fq_out, void* stream);
+
+/* ---- microscaled 4-bit floating point ------------------------------------------------------------
+ *
+ * The 4-bit type that the tensor cores multiply (the packed int4 format above is widened to int8): e2m1
+ * elements (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) in blocks along K that share a scale.
+ *     MX : 32 columns, s = 2^(floor(log2 max|x|) - 2), at least 2^-127, code = e2m1(x / s)
+ *     NV : 16 columns, s = b * global_scale, b = e4m3(max|x| / (6 global_scale)) in [2^-9, 448], code = e2m1(x / s)
+ * both roundings to nearest, ties to even, e2m1 saturating at 6.  A block with a NaN or an infinity gets the NaN
+ * scale byte (0xFF, 0x7F) and zero codes.  global_scale is a power of two in [2^-64, 2^64] (1 for MX), so that no
+ * border between codes depends on a rounding.
+ *
+ * Storage of [rows, K]:
+ *   codes  : uint8 [rows, ldq], column 2j in the low nibble of byte j; ldq a multiple of 16 for the product
+ *   scales : samq_fp4_scale_bytes() bytes, 16-byte aligned: [ceil(rows/128)][G][32][4][4], the byte of (row, block) at
+ *            [row / 128][block / 4][row % 32][row % 128 / 32][block % 4]; G = ceil(K / 256) * (2 for MX, 4 for NV).
+ *            Scales of blocks behind K are zero (the product multiplies them with zero codes).
+ *
+ * samq_quant_fp4 : x [M, K] of `dtype`, row stride ldx -> codes, scales and, unless NULL, fq_out [M, K] of `dtype` (the
+ *            values).  All of `scales` is written, and the codes up to ldq (at most the columns that G covers). */
+size_t samq_fp4_scale_bytes(int format, int64_t rows, int64_t K);
+int samq_quant_fp4(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, int format, float global_scale,
+                   uint8_t* codes, int64_t ldq, uint8_t* scales, void* fq_out, void* stream);
+
+/* y[m,n] = act(alpha * sum_k a[m,k] * w[n,k] + bias[n]) + residual[m,n]   on the tensor cores' block-scaled 4-bit kinds,
+ * accumulated in fp32.  A [M, K] and W [N, K] are operands in the storage above, of one format; alpha is the product of
+ * their global scales.  bias, residual, activation, out, ldo and status as in samq_gemm_i8 (out F16, BF16 or F32). */
+int samq_gemm_fp4(const uint8_t* A, int64_t lda, const uint8_t* a_scales, const uint8_t* W, int64_t ldw, const uint8_t* w_scales,
+                  int64_t M, int64_t N, int64_t K, int format, float alpha, const void* bias, const void* residual, int64_t ldr,
+                  int activation, void* out, int out_dtype, int64_t ldo, int32_t* status, void* stream);
 
 /* Process-wide choice between the two implementations of samq_gemm_i8 for row / tensor scales
  * (no reference counterpart: the reference has a single cuBLAS-style path):

@@ -17,6 +17,7 @@ F16, BF16, F32, I32 = 0, 1, 2, 3
 GRAN_ROW, GRAN_TENSOR, GRAN_GROUP = 0, 1, 2
 ACT_NONE, ACT_GELU = 0, 1
 HAD_NONE, HAD_FULL, HAD_PARTIAL = 0, 1, 2
+FP4_MX, FP4_NV = 0, 1
 
 EXPORTED_SYMBOLS = (
     "samq_version",
@@ -34,6 +35,10 @@ EXPORTED_SYMBOLS = (
     "samq_unpack_i4",
     "samq_matmul_i4",
     "samq_sym_dequant_i32",
+    "samq_rms_norm_quant_i8",
+    "samq_fp4_scale_bytes",
+    "samq_quant_fp4",
+    "samq_gemm_fp4",
     "samq_attn_window_prep",
     "samq_attn_rel_bias",
     "samq_attn_windowed",
@@ -148,6 +153,27 @@ def load() -> ctypes.CDLL:
     lib.samq_matmul_i4.argtypes = [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_size_t, c_void_p, c_void_p, c_void_p]
     lib.samq_sym_dequant_i32.restype = c_int
     lib.samq_sym_dequant_i32.argtypes = [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p]
+    lib.samq_rms_norm_quant_i8.restype = c_int
+    lib.samq_rms_norm_quant_i8.argtypes = [
+        c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64,   # x, residual, weight, dtype, M, K
+        c_int64, c_int64, c_float, c_int, c_void_p, c_int64,     # ldx, ldr, eps, n_bits, residual_out, ldo
+        c_void_p, c_void_p, c_void_p, c_void_p,                  # q, scale, fq, stream
+    ]
+    lib.samq_fp4_scale_bytes.restype = c_size_t
+    lib.samq_fp4_scale_bytes.argtypes = [c_int, c_int64, c_int64]
+    lib.samq_quant_fp4.restype = c_int
+    lib.samq_quant_fp4.argtypes = [
+        c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_float,   # x, dtype, M, K, ldx, format, global_scale
+        c_void_p, c_int64, c_void_p, c_void_p, c_void_p,              # codes, ldq, scales, fq, stream
+    ]
+    lib.samq_gemm_fp4.restype = c_int
+    lib.samq_gemm_fp4.argtypes = [
+        c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p,     # A, lda, a_scales, W, ldw, w_scales
+        c_int64, c_int64, c_int64, c_int, c_float,                    # M, N, K, format, alpha
+        c_void_p, c_void_p, c_int64,                                  # bias, residual, ldr
+        c_int, c_void_p, c_int, c_int64,                              # activation, out, out_dtype, ldo
+        c_void_p, c_void_p,                                           # status, stream
+    ]
     lib.samq_gemm_set_pair_mode.restype = c_int
     lib.samq_gemm_set_pair_mode.argtypes = [c_int]
     lib.samq_attn_transpose_v.restype = c_int

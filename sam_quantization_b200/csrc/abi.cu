@@ -1,6 +1,7 @@
 // extern "C" surface of libsamq: argument checks, thread-local error text and dispatch
 // into the kernels.  Declarations and the reference interfaces they replace: include/samq.h.
 #include "common.cuh"
+#include "fp4.cuh"
 #include <string.h>
 #include <atomic>
 
@@ -63,6 +64,14 @@ int sym_quant_i4_dispatch(const void* x, const void* scale, int64_t rows, int64_
 int unpack_i4_dispatch(const uint8_t* q, int64_t rows, int64_t cols, int64_t ldq, int8_t* out, int64_t ldo, void* stream);
 int pack_i4_dispatch(const int8_t* codes, int64_t rows, int64_t cols, int64_t ldc, uint8_t* q, int64_t ldq, void* stream);
 int sym_dequant_i32_dispatch(const int32_t* q, const void* scale_row, const void* scale_col, int64_t rows, int64_t cols, void* out, void* stream);
+int rms_norm_quant_dispatch(const void* x, const void* residual, const void* weight, int dtype, int64_t M, int64_t K,
+                            int64_t ldx, int64_t ldr, float eps, int n_bits, void* residual_out, int64_t ldo,
+                            int8_t* q, float* scale, void* fq, void* stream);
+int quant_fp4_dispatch(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, int fmt, float global_scale,
+                       uint8_t* codes, int64_t ldq, uint8_t* scales, void* fq, void* stream);
+int gemm_fp4_dispatch(const uint8_t* A, int64_t lda, const uint8_t* a_scales, const uint8_t* W, int64_t ldw, const uint8_t* w_scales,
+                      int64_t M, int64_t N, int64_t K, int fmt, float alpha, const void* bias, const void* residual, int64_t ldr,
+                      int activation, void* out, int out_dtype, int64_t ldo, int32_t* status, void* stream);
 int attn_window14_dispatch(const void* qkv, const void* table, int table_rows, int dtype, int64_t windows, int heads, int head_dim,
                            float scale, void* out, int32_t* status, void* stream);
 int attn_window_dispatch(const void* qkv, int dtype, int64_t windows, int H, int W, int nh, int d,
@@ -227,6 +236,34 @@ int samq_sym_dequant_i32(const int32_t* q, const void* scale_row, const void* sc
                          void* out, void* stream)
 {
     return samq::sym_dequant_i32_dispatch(q, scale_row, scale_col, rows, cols, out, stream);
+}
+
+int samq_rms_norm_quant_i8(const void* x, const void* residual, const void* weight, int dtype, int64_t M, int64_t K,
+                           int64_t ldx, int64_t ldr, float eps, int n_bits, void* residual_out, int64_t ldo,
+                           int8_t* q_out, float* scale_out, void* fq_out, void* stream)
+{
+    return samq::rms_norm_quant_dispatch(x, residual, weight, dtype, M, K, ldx, ldr, eps, n_bits, residual_out, ldo,
+                                         q_out, scale_out, fq_out, stream);
+}
+
+size_t samq_fp4_scale_bytes(int format, int64_t rows, int64_t K)
+{
+    if (!samq::fp4::known_format(format) || rows <= 0 || K <= 0) return 0;
+    return (size_t)((rows + samq::fp4::TILE_ROWS - 1) / samq::fp4::TILE_ROWS * samq::fp4::groups_of(format, K)) * samq::fp4::TILE_BYTES;
+}
+
+int samq_quant_fp4(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, int format, float global_scale,
+                   uint8_t* codes, int64_t ldq, uint8_t* scales, void* fq_out, void* stream)
+{
+    return samq::quant_fp4_dispatch(x, dtype, M, K, ldx, format, global_scale, codes, ldq, scales, fq_out, stream);
+}
+
+int samq_gemm_fp4(const uint8_t* A, int64_t lda, const uint8_t* a_scales, const uint8_t* W, int64_t ldw, const uint8_t* w_scales,
+                  int64_t M, int64_t N, int64_t K, int format, float alpha, const void* bias, const void* residual, int64_t ldr,
+                  int activation, void* out, int out_dtype, int64_t ldo, int32_t* status, void* stream)
+{
+    return samq::gemm_fp4_dispatch(A, lda, a_scales, W, ldw, w_scales, M, N, K, format, alpha, bias, residual, ldr,
+                                   activation, out, out_dtype, ldo, status, stream);
 }
 
 int samq_gemm_set_pair_mode(int mode)

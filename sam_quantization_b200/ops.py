@@ -7,6 +7,7 @@ outputs.  CPU tensors are rejected: this package has no CPU compute path.
 from __future__ import annotations
 
 import ctypes
+import math
 import weakref
 from dataclasses import dataclass
 from typing import Optional, Tuple
@@ -415,6 +416,193 @@ def gemm_i8(a_q: torch.Tensor, w_q: torch.Tensor,
             _ptr(bias), _ptr(residual), ldr, activation,
             _ptr(out), _OUT_CODE[out_dtype], N, _ptr(status_word(dev)), _stream()))
     return out.view(*lead, N)
+
+
+# ---- RMS norm with an 8-bit output -----------------------------------------------------------------
+
+def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None,
+                      codes: bool = True, fake_quant: bool = False, n_bits: int = 8,
+                      residual_out: Optional[torch.Tensor] = None) -> dict:
+    """RMS norm of ``x`` ([..., K]; fp16 / bf16 / fp32), or of ``x + residual``, quantized per row in the same pass
+    (``samq_rms_norm_quant_i8``).
+
+    Returns a dict with ``q`` int8 [..., K] (unless ``codes=False``) and ``scale`` fp32 [...], what ``gemm_i8`` takes,
+    ``fq`` (with ``fake_quant``) the values ``q * scale`` in the tensor dtype and, with a ``residual``, ``residual``:
+    the sum ``x + residual`` in the tensor dtype, in a new tensor or in ``residual_out`` (which may be ``residual`` or
+    ``x`` itself).  The normed value is quantized from fp32, without a rounding to the tensor dtype in between."""
+    _require_cuda(x, "x")
+    if x.dtype not in _DTYPE_CODE:
+        raise TypeError(f"unsupported dtype {x.dtype}")
+    lib = _lib.load()
+    lead, dev = x.shape[:-1], x.device
+    x2, M, K, ldx = _as_rows(x)
+    if weight.numel() != K:
+        raise ValueError("weight must have K elements")
+    weight = weight.detach().reshape(-1).to(device=dev, dtype=x.dtype).contiguous()
+    res2 = h2 = h = None
+    ldr = ldo = 0
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != dev:
+            raise ValueError("residual must have the shape, dtype and device of x")
+        res2, _, _, ldr = _as_rows(residual)
+        h = torch.empty((M, K), dtype=x.dtype, device=dev) if residual_out is None else residual_out
+        h2, hm, hk, ldo = _as_rows(h)
+        if residual_out is not None:
+            if h.dtype != x.dtype or h.device != dev or hm != M or hk != K or h2.data_ptr() != h.data_ptr():
+                raise ValueError("residual_out must be rows of K contiguous elements with the shape, dtype and device of x")
+    elif residual_out is not None:
+        raise ValueError("residual_out without a residual")
+    q = torch.empty((M, K), dtype=torch.int8, device=dev) if codes else None
+    scale = torch.empty((M,), dtype=torch.float32, device=dev)
+    fq = torch.empty((M, K), dtype=x.dtype, device=dev) if fake_quant else None
+    nbytes = M * K * (x.element_size() * (1 + (2 if residual is not None else 0) + (1 if fake_quant else 0)) + (1 if codes else 0)) + 4 * M
+    with torch.cuda.device(dev), _Timed("rms_norm_quant", nbytes):
+        _lib.check(lib.samq_rms_norm_quant_i8(_ptr(x2), _ptr(res2), _ptr(weight), _DTYPE_CODE[x.dtype], M, K, ldx, ldr, float(eps),
+                                              int(n_bits), _ptr(h2), ldo, _ptr(q), _ptr(scale), _ptr(fq), _stream()))
+    out = {"scale": scale.view(lead)}
+    if codes:
+        out["q"] = q.view(*lead, K)
+    if fake_quant:
+        out["fq"] = fq.view(*lead, K)
+    if residual is not None:
+        out["residual"] = h.view(x.shape) if residual_out is None else residual_out
+    return out
+
+
+# ---- microscaled 4-bit floating point ----------------------------------------------------------------
+
+FP4_FORMATS = {"mxfp4": _lib.FP4_MX, "nvfp4": _lib.FP4_NV}
+FP4_BLOCK = {"mxfp4": 32, "nvfp4": 16}
+_E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def fp4_scale_shape(fmt: str, rows: int, K: int) -> Tuple[int, ...]:
+    """Shape of the scale tiles of a [rows, K] operand (include/samq.h gives their order)."""
+    return ((rows + 127) // 128, (K + 255) // 256 * (64 // FP4_BLOCK[fmt]), 32, 4, 4)
+
+
+def fp4_global_scale(absmax: float) -> float:
+    """The power of two that brings the largest nvfp4 block scale of a tensor with this largest magnitude into
+    (224, 448], the top of e4m3; 1.0 for a tensor of zeros."""
+    absmax = float(absmax)
+    if not math.isfinite(absmax):
+        raise ValueError("a global scale needs a finite largest magnitude")
+    if absmax <= 0.0:
+        return 1.0
+    return min(max(2.0 ** math.ceil(math.log2(absmax / (6.0 * 448.0))), 2.0 ** -64), 2.0 ** 64)
+
+
+class Fp4Tensor:
+    """A [rows, K] operand in microscaled 4-bit floating point: ``codes`` uint8 [rows, pitch], ``scales`` uint8 in the
+    tiles of ``fp4_scale_shape``, ``fmt`` "mxfp4" or "nvfp4", ``global_scale`` a float that multiplies every value."""
+
+    __slots__ = ("codes", "scales", "rows", "K", "fmt", "global_scale")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, K: int, fmt: str, global_scale: float = 1.0):
+        if fmt not in FP4_FORMATS:
+            raise ValueError(f"Invalid 4-bit format: {fmt}")
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError("codes and scales must be uint8")
+        if codes.dim() != 2 or codes.shape[0] != rows or codes.shape[1] < (K + 1) // 2 or codes.stride(1) != 1:
+            raise ValueError(f"codes must be [{rows}, >= {(K + 1) // 2}] with contiguous rows")
+        if scales.device != codes.device or not scales.is_contiguous() or tuple(scales.shape) != fp4_scale_shape(fmt, rows, K):
+            raise ValueError(f"scales must be a contiguous {fp4_scale_shape(fmt, rows, K)} tensor on the device of codes")
+        self.codes, self.scales, self.rows, self.K, self.fmt, self.global_scale = codes, scales, rows, K, fmt, float(global_scale)
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values [rows, K], rounded once to ``dtype`` (off the hot path: plain torch)."""
+        b = FP4_BLOCK[self.fmt]
+        table = torch.tensor(_E2M1 + tuple(-v for v in _E2M1), device=self.device)
+        v = table[torch.stack((self.codes & 15, self.codes >> 4), -1).flatten(1)[:, :self.K].long()]
+        nb = (self.K + b - 1) // b
+        byte = self.scales.permute(0, 3, 2, 1, 4).reshape(-1, 4 * self.scales.shape[1])[:self.rows, :nb]
+        if self.fmt == "mxfp4":
+            s = byte.contiguous().view(torch.float8_e8m0fnu).float()
+        else:
+            s = byte.contiguous().view(torch.float8_e4m3fn).float() * self.global_scale
+        return (v * s.repeat_interleave(b, 1)[:, :self.K]).to(dtype)
+
+
+def quantize_fp4(x: torch.Tensor, fmt: str = "nvfp4", global_scale: float = 1.0, fake_quant: bool = False) -> dict:
+    """Quantize ``x`` ([..., K]; fp16 / bf16 / fp32) to microscaled 4-bit floating point (``samq_quant_fp4``).
+
+    Returns a dict with ``q``, an ``Fp4Tensor`` of the rows of ``x``, and with ``fake_quant`` ``fq``, the values it
+    stands for in the dtype and shape of ``x``.  ``global_scale`` (nvfp4) is a power of two, see ``fp4_global_scale``."""
+    _require_cuda(x, "x")
+    if x.dtype not in _DTYPE_CODE:
+        raise TypeError(f"unsupported dtype {x.dtype}")
+    if fmt not in FP4_FORMATS:
+        raise ValueError(f"Invalid 4-bit format: {fmt}")
+    lib = _lib.load()
+    x2, M, K, ldx = _as_rows(x)
+    dev = x.device
+    pitch = (K + 31) // 32 * 16
+    codes = torch.empty((M, pitch), dtype=torch.uint8, device=dev)
+    scales = torch.empty(fp4_scale_shape(fmt, M, K), dtype=torch.uint8, device=dev)
+    fq = torch.empty((M, K), dtype=x.dtype, device=dev) if fake_quant else None
+    nbytes = M * K * x.element_size() * (2 if fake_quant else 1) + codes.numel() + scales.numel()
+    with torch.cuda.device(dev), _Timed("quant_fp4", nbytes):
+        _lib.check(lib.samq_quant_fp4(_ptr(x2), _DTYPE_CODE[x.dtype], M, K, ldx, FP4_FORMATS[fmt], float(global_scale), _ptr(codes), pitch,
+                                      _ptr(scales), _ptr(fq), _stream()))
+    out = {"q": Fp4Tensor(codes, scales, M, K, fmt, global_scale)}
+    if fake_quant:
+        out["fq"] = fq.view(x.shape)
+    return out
+
+
+def _linear_args(N: int, M: int, bias, residual, out_dtype, out, dev):
+    """Checked bias, residual rows and output of a linear layer's epilogue, as ``gemm_i8`` takes them."""
+    if out_dtype not in _DTYPE_CODE:
+        raise TypeError(f"unsupported out_dtype {out_dtype}")
+    if bias is not None:
+        bias = _bias_as(bias, out_dtype, dev)
+        if bias.numel() != N:
+            raise ValueError("bias must have N elements")
+    ldr = 0
+    if residual is not None:
+        if residual.device != dev:
+            raise ValueError("residual must be on the device of the operands")
+        if residual.dtype != out_dtype:
+            raise TypeError("residual must have the output dtype")
+        residual, rm, rn, ldr = _as_rows(residual)
+        if rm != M or rn != N:
+            raise ValueError("residual must be [..., N] with the rows of the activation")
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype, device=dev)
+    elif out.dtype != out_dtype or out.device != dev or out.shape[-1] != N or out.numel() != M * N or not out.is_contiguous():
+        raise ValueError("out has the wrong dtype, device, shape or layout")
+    return bias, residual, ldr, out
+
+
+def gemm_fp4(a: Fp4Tensor, w: Fp4Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+             activation: int = ACT_NONE, out_dtype: torch.dtype = torch.float16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``act(a @ w.T + bias) + residual`` -> [a.rows, w.rows] of ``out_dtype`` from two 4-bit operands of one format, on
+    the tensor cores' block-scaled kinds (``samq_gemm_fp4``)."""
+    _require_cuda(a.codes, "a")
+    if a.fmt != w.fmt or a.K != w.K or a.device != w.device:
+        raise ValueError(f"operands must share format, K and device: {a.fmt} [{a.rows}, {a.K}] and {w.fmt} [{w.rows}, {w.K}]")
+    lib = _lib.load()
+    M, N, K, dev = a.rows, w.rows, a.K, a.device
+    bias, residual, ldr, out = _linear_args(N, M, bias, residual, out_dtype, out, dev)
+    with torch.cuda.device(dev), _Timed("gemm_fp4", 2.0 * M * N * K):
+        _lib.check(lib.samq_gemm_fp4(_ptr(a.codes), a.codes.stride(0), _ptr(a.scales), _ptr(w.codes), w.codes.stride(0), _ptr(w.scales),
+                                     M, N, K, FP4_FORMATS[a.fmt], a.global_scale * w.global_scale, _ptr(bias), _ptr(residual), ldr,
+                                     activation, _ptr(out), _DTYPE_CODE[out_dtype], N, _ptr(status_word(dev)), _stream()))
+    return out
+
+
+def linear_fp4(x: torch.Tensor, w: Fp4Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+               activation: int = ACT_NONE, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``x`` ([..., K]) quantized to the format of ``w`` (without a global scale) and multiplied with it:
+    ``act(q(x) @ w.T + bias) + residual`` -> [..., N], of ``x.dtype`` unless ``out_dtype`` says otherwise."""
+    if x.shape[-1] != w.K:
+        raise ValueError(f"x must be [..., {w.K}]")
+    y = gemm_fp4(quantize_fp4(x, w.fmt)["q"], w, bias=bias, residual=residual, activation=activation, out_dtype=out_dtype or x.dtype)
+    return y.view(*x.shape[:-1], w.rows)
 
 
 def gemm_stall_selftest(a_q: torch.Tensor, w_q: torch.Tensor, skip_kblock: int = 0, wait_limit_cycles: int = 2_000_000) -> torch.Tensor:

@@ -1,0 +1,265 @@
+"""Microscaled 4-bit floating point on the GPU: the quantizer bit for bit against the 64-bit checker, the product
+exactly where its sums are exact, and within derived bounds elsewhere."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import fp4 as F
+from sam_quantization_b200 import ops
+
+pytestmark = pytest.mark.gpu
+FORMATS = ["mxfp4", "nvfp4"]
+HALF = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+
+
+def _values(M, K, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed + 17 * M + K)
+    x = torch.randn(M, K, generator=g) * torch.exp(2.0 * torch.randn(M, 1, generator=g))
+    x = x * (1.0 + 19.0 * (torch.rand(K, generator=g) < 0.02))
+    return x.to(dtype)
+
+
+def _check_quantized(x, out, fmt, g=1.0):
+    M, K = x.shape
+    code, byte, value = F.quantize(x.double().cpu().numpy(), fmt, g)
+    q = out["q"]
+    assert (q.rows, q.K, q.fmt, q.global_scale) == (M, K, fmt, g)
+    assert np.array_equal(q.codes.cpu().numpy(), F.pack_codes(code, q.codes.shape[1]))
+    assert np.array_equal(q.scales.cpu().numpy(), F.tile_scales(byte, fmt, K))
+    want = torch.from_numpy(value).to(x.dtype)
+    assert torch.equal(torch.nan_to_num(out["fq"].cpu(), nan=-77.0), torch.nan_to_num(want, nan=-77.0))
+    assert torch.equal(torch.nan_to_num(q.dequantize(x.dtype).cpu(), nan=-77.0), torch.nan_to_num(want, nan=-77.0))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,K", [(1, 1), (1, 16), (3, 31), (5, 33), (128, 256), (129, 257), (130, 1283), (7, 5120), (300, 64), (33, 1023)])
+def test_quantizer_equals_the_checker(cuda_device, fmt, dtype, M, K):
+    x = _values(M, K, dtype)
+    _check_quantized(x, ops.quantize_fp4(x.to(cuda_device), fmt, fake_quant=True), fmt)
+
+
+@pytest.mark.parametrize("g", [2.0 ** -14, 0.5, 8.0])
+def test_global_scale(cuda_device, g):
+    x = _values(65, 200, torch.float32) * 0.02
+    _check_quantized(x, ops.quantize_fp4(x.to(cuda_device), "nvfp4", global_scale=g, fake_quant=True), "nvfp4", g)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_borders_between_codes_and_scales(cuda_device, fmt):
+    """Every border of a code and its neighbours in fp32, under scales of every mantissa; block maxima at and next to
+    the borders of the scale."""
+    rows = []
+    for m in (8, 9, 10, 11, 12, 13, 14, 15):
+        s = m / 8.0 if fmt == "nvfp4" else 2.0 ** (m - 10)
+        for b in list(F.BORDERS) + [6.0, 0.5]:
+            v = np.float32(b * s)
+            rows.append([np.float32(6 * s), v, np.nextafter(v, np.float32(0)), np.nextafter(v, np.float32(99)), -v] + [0.0] * 11)
+    mids = (F.E4M3[1:] + F.E4M3[:-1]) / 2 * 6
+    for v in list(mids) + list(F.E4M3 * 6) + [2.0 ** i for i in range(-20, 20)]:
+        v = np.float32(v)
+        for t in (v, np.nextafter(v, np.float32(0)), np.nextafter(v, np.float32(1e9))):
+            rows.append([t] + [0.3 * t, -0.7 * t] + [0.0] * 13)
+    x = torch.tensor(np.array(rows, np.float32))
+    x = torch.cat((x, x.flip(0)), 1)
+    _check_quantized(x, ops.quantize_fp4(x.to(cuda_device), fmt, fake_quant=True), fmt)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_extreme_values(cuda_device, fmt):
+    x = torch.zeros(9, 70)
+    x[1] = 3e38 * torch.linspace(-1, 1, 70)
+    x[2] = 1e-38 * torch.linspace(-1, 1, 70)
+    x[3] = 1e-44
+    x[4, 3] = float("nan")
+    x[5, 40] = float("inf")
+    x[6, 69] = -float("inf")
+    x[7] = torch.linspace(-1e-3, 1e-3, 70)
+    x[8] = -0.0
+    _check_quantized(x, ops.quantize_fp4(x.to(cuda_device), fmt, fake_quant=True), fmt)
+    x16 = x.clamp(-65504, 65504)
+    x16[4, 3], x16[5, 40] = float("nan"), float("inf")
+    x16 = x16.half()
+    _check_quantized(x16, ops.quantize_fp4(x16.to(cuda_device), fmt, fake_quant=True), fmt)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("K,pitch,offset", [(256, 264, 0), (256, 259, 0), (250, 300, 3)])
+def test_rows_with_a_pitch(cuda_device, fmt, K, pitch, offset):
+    x = _values(20, pitch, torch.bfloat16).to(cuda_device)[:, offset:offset + K]
+    _check_quantized(x.cpu(), ops.quantize_fp4(x, fmt, fake_quant=True), fmt)
+    x = _values(12, K, torch.float16).to(cuda_device)
+    out = ops.quantize_fp4(x.view(3, 4, K), fmt, fake_quant=True)
+    assert out["fq"].shape == (3, 4, K)
+    _check_quantized(x.cpu(), {"q": out["q"], "fq": out["fq"].view(12, K)}, fmt)
+
+
+def test_no_rows(cuda_device):
+    x = torch.empty(0, 64, dtype=torch.float16, device=cuda_device)
+    w = ops.quantize_fp4(_values(24, 64, torch.float16).to(cuda_device))["q"]
+    out = ops.quantize_fp4(x, fake_quant=True)
+    assert out["fq"].shape == (0, 64)
+    assert ops.gemm_fp4(out["q"], w).shape == (0, 24) and ops.linear_fp4(x, w).shape == (0, 24)
+
+
+# ---- the product ----------------------------------------------------------------------------------------
+
+def _exact_operand(rows, K, fmt, dev, seed):
+    """Random codes under scales of two neighbouring exponents (and e4m3 mantissas): every product and partial sum is a
+    multiple of 2^-6 below 2^17, exact in fp32 in any order."""
+    rng = np.random.default_rng(seed)
+    code = rng.integers(0, 16, (rows, K)).astype(np.uint8)
+    nb = -(-K // F.BLOCK[fmt])
+    byte = (rng.integers(126, 128, (rows, nb)) if fmt == "mxfp4" else rng.integers(0x30, 0x3B, (rows, nb)) & 0xFE).astype(np.uint8)
+    pitch = (K + 31) // 32 * 16
+    q = ops.Fp4Tensor(torch.from_numpy(F.pack_codes(code, pitch)).to(dev), torch.from_numpy(F.tile_scales(byte, fmt, K)).to(dev), rows, K, fmt)
+    value = F.code_value(code) * np.repeat(F.scale_value(byte, fmt), F.BLOCK[fmt], 1)[:, :K]
+    return q, value
+
+
+SHAPES = [(1, 1, 1), (1, 8, 64), (3, 130, 31), (1, 5120, 1280), (128, 128, 256), (129, 257, 300), (200, 40, 1283), (64, 1001, 512), (16, 300, 2048),
+          (17, 65, 96), (40, 200, 4100), (260, 520, 768), (1000, 384, 200), (300, 1280, 5120)]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_product_is_exact_where_its_sums_are(cuda_device, fmt, M, N, K):
+    a, av = _exact_operand(M, K, fmt, cuda_device, M + K)
+    w, wv = _exact_operand(N, K, fmt, cuda_device, N + K + 1)
+    y = ops.gemm_fp4(a, w, out_dtype=torch.float32)
+    torch.cuda.synchronize()
+    ops.check_status()
+    assert np.array_equal(y.cpu().numpy().astype(np.float64), av @ wv.T)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,N,K", [(1, 300, 1280), (5, 72, 100), (40, 1001, 2000), (130, 257, 1283), (600, 640, 512)])
+@pytest.mark.parametrize("bias,gelu,residual", [(True, False, False), (True, True, False), (False, False, True), (True, True, True)])
+def test_epilogue(cuda_device, fmt, dtype, M, N, K, bias, gelu, residual):
+    """Exact sums, so only the epilogue rounds: alpha and bias in one fused step (u), GELU (3e-7 absolute and 2e-5
+    relative, csrc/gemm_common.cuh), the residual's addition (u) and the rounding to the output type."""
+    a, av = _exact_operand(M, K, fmt, cuda_device, 1)
+    w, wv = _exact_operand(N, K, fmt, cuda_device, 2)
+    a.global_scale, w.global_scale = 0.25, 2.0 ** -6
+    g = torch.Generator().manual_seed(5)
+    b = torch.randn(N, generator=g).to(dtype) if bias else None
+    r = torch.randn(M, N, generator=g).to(dtype) if residual else None
+    y = ops.gemm_fp4(a, w, bias=None if b is None else b.to(cuda_device), residual=None if r is None else r.to(cuda_device),
+                     activation=ops.ACT_GELU if gelu else ops.ACT_NONE, out_dtype=dtype)
+    ops.check_status()
+    z = (av @ wv.T) * 2.0 ** -8
+    if b is not None:
+        z = z + b.double().numpy()
+    u = 2.0 ** -24
+    tol = u * np.abs(z)
+    if gelu:
+        tol = tol * 1.2 + 3e-7 + 2e-5 * np.abs(z)                      # |gelu'| < 1.13
+        z = F.gelu(z)
+    if r is not None:
+        z = z + r.double().numpy()
+        tol = tol + u * np.abs(z)
+    tol = tol + HALF[dtype] * (np.abs(z) + tol) + (2.0 ** -25 if dtype == torch.float16 else 0)
+    assert np.all(np.abs(y.double().cpu().numpy() - z) <= tol)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N,K", [(1, 640, 1280), (37, 200, 1283), (300, 300, 5120)])
+def test_product_of_quantized_data(cuda_device, fmt, M, N, K):
+    """Scales over many exponents.  fp32 accumulation of at most K terms, each addition off by at most a step of the sum
+    of magnitudes S: K * 2^-23 * S."""
+    x = _values(M, K, torch.bfloat16)
+    wt = (torch.randn(N, K, generator=torch.Generator().manual_seed(1)) * 0.02)
+    g = ops.fp4_global_scale(float(wt.abs().max())) if fmt == "nvfp4" else 1.0
+    w = ops.quantize_fp4(wt.to(cuda_device), fmt, global_scale=g)["q"]
+    y = ops.gemm_fp4(ops.quantize_fp4(x.to(cuda_device), fmt)["q"], w, out_dtype=torch.float32)
+    ops.check_status()
+    av, wv = F.quantize(x.double().numpy(), fmt)[2], F.quantize(wt.double().numpy(), fmt, g)[2]
+    tol = K * 2.0 ** -23 * (np.abs(av) @ np.abs(wv).T)
+    assert np.all(np.abs(y.double().cpu().numpy() - av @ wv.T) <= tol + 1e-30)
+    # and the layer in one call is the two calls
+    z = ops.linear_fp4(x.to(cuda_device), w, out_dtype=torch.float32)
+    assert np.all(np.abs(z.double().cpu().numpy() - av @ wv.T) <= tol + 1e-30)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M", [1, 200])
+def test_rows_that_are_not_finite_stay_apart(cuda_device, fmt, M):
+    x = _values(M, 300, torch.float16)
+    x[M // 2, 299] = float("nan")
+    w, wv = _exact_operand(50, 300, fmt, cuda_device, 3)
+    y = ops.linear_fp4(x.to(cuda_device), w)
+    ops.check_status()
+    rows = [m for m in range(M) if m != M // 2]
+    assert y[M // 2].isnan().all() and not y[rows].isnan().any()
+
+
+@pytest.mark.parametrize("M", [3, 200, 700])
+def test_strided_outputs_and_operands(cuda_device, M):
+    a, av = _exact_operand(M, 320, "nvfp4", cuda_device, 1)
+    w, wv = _exact_operand(130, 320, "nvfp4", cuda_device, 2)
+    wide = torch.zeros(M, 192, dtype=torch.uint8, device=cuda_device)
+    wide[:, :160] = a.codes
+    wide[:, 160:] = 255                                                  # never read: behind K
+    a2 = ops.Fp4Tensor(wide, a.scales, M, 320, "nvfp4")
+    assert np.array_equal(ops.gemm_fp4(a2, w, out_dtype=torch.float32).double().cpu().numpy(), av @ wv.T)
+    res = torch.randn(M, 140, device=cuda_device)[:, 3:133]              # a residual of unaligned rows
+    y = ops.gemm_fp4(a, w, residual=res, out_dtype=torch.float32)
+    assert np.array_equal(y.double().cpu().numpy(), np.float32(np.float32(av @ wv.T) + res.cpu().numpy()).astype(np.float64))
+    out = torch.full((M + 2, 130), 9.0, dtype=torch.float32, device=cuda_device)
+    ops.gemm_fp4(a, w, out_dtype=torch.float32, out=out[1:M + 1])
+    assert (out[0] == 9).all() and (out[-1] == 9).all()                  # rows before and behind stay
+    assert np.array_equal(out[1:M + 1].double().cpu().numpy(), av @ wv.T)
+
+
+def test_refusals(cuda_device):
+    a, _ = _exact_operand(4, 64, "nvfp4", cuda_device, 1)
+    w, _ = _exact_operand(8, 64, "nvfp4", cuda_device, 2)
+    m, _ = _exact_operand(8, 64, "mxfp4", cuda_device, 2)
+    k, _ = _exact_operand(8, 96, "nvfp4", cuda_device, 2)
+    x = torch.zeros(4, 64, dtype=torch.float16, device=cuda_device)
+    for bad in (lambda: ops.gemm_fp4(a, m), lambda: ops.gemm_fp4(a, k), lambda: ops.linear_fp4(x, k), lambda: ops.quantize_fp4(x, "int4"),
+                lambda: ops.gemm_fp4(a, w, bias=torch.zeros(7, dtype=torch.float16, device=cuda_device)),
+                lambda: ops.gemm_fp4(a, w, residual=x), lambda: ops.gemm_fp4(a, w, out=x)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(TypeError):
+        ops.gemm_fp4(a, w, out_dtype=torch.int32)
+    with pytest.raises(TypeError):
+        ops.gemm_fp4(a, w, residual=torch.zeros(4, 8, device=cuda_device))
+    with pytest.raises(RuntimeError, match="global_scale"):
+        ops.quantize_fp4(x, "nvfp4", global_scale=3.0)
+    with pytest.raises(RuntimeError, match="mxfp4"):
+        ops.quantize_fp4(x, "mxfp4", global_scale=2.0)
+
+
+def _same(a, b):
+    """Bit for bit (a row of these values can hold an fp16 infinity, and is then NaN on both sides)."""
+    return torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+@pytest.mark.parametrize("M", [2, 150])
+def test_captured_replayed_and_on_two_streams(cuda_device, M):
+    x = _values(M, 640, torch.float16).to(cuda_device)
+    x2 = _values(M, 640, torch.float16, seed=4).to(cuda_device)
+    w = ops.quantize_fp4((torch.randn(300, 640, generator=torch.Generator().manual_seed(1)) * 0.02).to(cuda_device))["q"]
+    want, want2 = ops.linear_fp4(x, w), ops.linear_fp4(x2, w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):                                                   # two calls at once
+        with torch.cuda.stream(side):
+            y2 = ops.linear_fp4(x2, w)
+        y = ops.linear_fp4(x, w)
+    torch.cuda.current_stream().wait_stream(side)
+    assert _same(y, want) and _same(y2, want2)
+    graphs = []
+    for src in (x, x2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.linear_fp4(src, w)
+        graphs.append((graph, out))
+    for _ in range(3):
+        for graph, _ in graphs:
+            graph.replay()
+    assert _same(graphs[0][1], want) and _same(graphs[1][1], want2)
+    ops.check_status()
