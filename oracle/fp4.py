@@ -86,5 +86,5 @@ def rms_norm(h, w, eps, qmax=127.0):
 
 
 def gelu(y):
-    from math import erf
-    return 0.5 * y * (1.0 + np.vectorize(erf)(y / np.sqrt(2.0)))
+    import torch
+    return 0.5 * y * (1.0 + torch.erf(torch.from_numpy(y / np.sqrt(2.0))).numpy())

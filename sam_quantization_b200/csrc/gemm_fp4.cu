@@ -6,17 +6,16 @@
 // tcgen05.mma with block scaling (kind::mxf4 for mxfp4, kind::mxf4nvf4 for nvfp4) takes K = 64 columns an
 // instruction: 32 bytes of codes from shared memory (128-byte swizzle, as the int8 product) and the scales of both
 // operands from tensor memory, where tcgen05.cp puts a stage's tiles before its MMAs.  Accumulators are fp32.
-#include "fp4.cuh"
-#include "gemm_common.cuh"
+#include "fp4_gemm.cuh"
 
 namespace samq {
 
-using namespace sm100;
-using namespace gemm;
+using namespace fp4;
 
 namespace {
 
-using namespace fp4;
+// 256 x 256 tiles from which the pair kernel has enough to do
+constexpr int PAIR_MIN_TILES = 32;
 
 constexpr int BM = 128;
 constexpr int BN = 128;
@@ -25,7 +24,6 @@ constexpr int A_BYTES = BM * BK;                 // BK = 128 bytes = 256 columns
 constexpr int B_BYTES = BN * BK;
 constexpr int EPI_WARPS = 4;
 constexpr int THREADS = 64 + EPI_WARPS * 32;
-constexpr int UKB = 32;                          // bytes of K of one MMA
 constexpr int TMEM_COLS = 256;
 constexpr int SFA_COL = BN;                      // scale columns behind the accumulator
 
@@ -45,13 +43,6 @@ template <int FMT> struct Shape {
     static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + BN * sizeof(float) + sizeof(Control);
 };
 
-// Instruction descriptor of the block-scaled kinds: B's scale id in [4,6); A, B = e2m1 (1) in [7,10) and [10,12);
-// both K-major; N >> 3 in [17,23); scale type in bit 23 (0 ue4m3, 1 ue8m0); M >> 7 in [27,29); A's scale id in [29,31).
-__host__ __device__ constexpr uint32_t instr_desc(int fmt, int m, int n, uint32_t sf_id) {
-    return (sf_id << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) |
-           ((fmt == SAMQ_FP4_MX ? 1u : 0u) << 23) | ((uint32_t)(m >> 7) << 27) | (sf_id << 29);
-}
-
 struct Fp4Params {
     int M, N, K;
     const uint8_t* a_scales;
@@ -66,28 +57,6 @@ struct Fp4Params {
     int32_t* status;
 };
 
-template <int FMT>
-__device__ __forceinline__ void mma_fp4(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-    if constexpr (FMT == SAMQ_FP4_MX)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                     "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-                     ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
-    else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                     "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-                     ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
-}
-// 32 rows x 16 bytes of shared memory to four columns of tensor memory, repeated in all four lane quadrants
-__device__ __forceinline__ void tmem_copy_scales(uint32_t tmem, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
-}
-// rows of 16 bytes, no swizzle, eight rows (128 bytes) a core matrix
-__device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
-    uint64_t d = (uint64_t)((smem_addr >> 4) & 0x3FFFu);
-    d |= (uint64_t)(128 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    return d;
-}
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
@@ -158,8 +127,8 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 const uint32_t ss = smem_u32(sf + (size_t)st * 2 * S::SF_BYTES);
 #pragma unroll
                 for (int g = 0; g < S::GROUPS; ++g) {
-                    tmem_copy_scales(tmem + SFA_COL + 4 * g, scale_desc(ss + g * TILE_BYTES));
-                    tmem_copy_scales(tmem + S::SFB_COL + 4 * g, scale_desc(ss + S::SF_BYTES + g * TILE_BYTES));
+                    tmem_copy_scales<1>(tmem + SFA_COL + 4 * g, scale_desc(ss + g * TILE_BYTES));
+                    tmem_copy_scales<1>(tmem + S::SFB_COL + 4 * g, scale_desc(ss + S::SF_BYTES + g * TILE_BYTES));
                 }
                 const uint64_t adesc = make_smem_desc(sa), bdesc = make_smem_desc(sa + A_BYTES);
 #pragma unroll
@@ -167,7 +136,7 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                     // mxfp4: a word of four scales serves two MMAs, the second taking its upper half (scale id 2)
                     const int g = FMT == SAMQ_FP4_MX ? k / 2 : k;
                     const uint32_t id = FMT == SAMQ_FP4_MX ? 2u * (k & 1) : 0u;
-                    mma_fp4<FMT>(tmem, adesc + (uint64_t)(k * (UKB >> 4)), bdesc + (uint64_t)(k * (UKB >> 4)), instr_desc(FMT, BM, BN, id),
+                    mma_fp4<FMT, 1>(tmem, adesc + (uint64_t)(k * (UKB >> 4)), bdesc + (uint64_t)(k * (UKB >> 4)), instr_desc(FMT, BM, BN, id),
                                  tmem + SFA_COL + 4 * g, tmem + S::SFB_COL + 4 * g, (kb | k) != 0 ? 1u : 0u);
                 }
                 tcgen05_commit(smem_u32(&ctl->empty[st]));
@@ -263,6 +232,22 @@ int gemm_fp4_dispatch(const uint8_t* A, int64_t lda, const uint8_t* a_scales, co
     const size_t esz = out_dtype == SAMQ_F32 ? 4 : 2;
     if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(residual)) & (esz - 1))
         return fail(SAMQ_ERR_ALIGNMENT, "out, bias and residual must be aligned to their elements");
+    Fp4Call c;
+    c.A = A; c.lda = lda; c.a_scales = a_scales; c.W = W; c.ldw = ldw; c.w_scales = w_scales;
+    c.M = M; c.N = N; c.K = K; c.fmt = fmt; c.out_dtype = out_dtype; c.gelu = activation == SAMQ_ACT_GELU;
+    c.status = status; c.stream = static_cast<cudaStream_t>(stream);
+    c.epi.M = (int)M; c.epi.N = (int)N; c.epi.alpha = alpha; c.epi.bias = bias; c.epi.residual = residual; c.epi.ldr = ldr;
+    c.epi.out = out; c.epi.ldo = ldo;
+    c.epi.tma_out = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (ldo * esz) % 16 == 0;
+    c.epi.tma_res = residual != nullptr && (reinterpret_cast<uintptr_t>(residual) & 15) == 0 && (ldr * esz) % 16 == 0;
+    if ((M + 255) / 256 * ((N + 255) / 256) >= PAIR_MIN_TILES) {
+        memset(&c.map_out, 0, sizeof(c.map_out));
+        memset(&c.map_res, 0, sizeof(c.map_res));
+        int rc = SAMQ_OK;
+        if (c.epi.tma_out) rc = make_row_map(&c.map_out, out, M, N, ldo, (int)esz);
+        if (rc == SAMQ_OK && c.epi.tma_res) rc = make_row_map(&c.map_res, residual, M, N, ldr, (int)esz);
+        return rc != SAMQ_OK ? rc : gemm_fp4_pair(c);
+    }
     CUtensorMap ma, mw;
     int rc = make_operand_map(&ma, reinterpret_cast<const int8_t*>(A), M, (K + 1) / 2, lda, BM);
     if (rc != SAMQ_OK) return rc;
@@ -273,7 +258,7 @@ int gemm_fp4_dispatch(const uint8_t* A, int64_t lda, const uint8_t* a_scales, co
     p.groups = (int)groups_of(fmt, K); p.alpha = alpha; p.bias = bias; p.residual = residual; p.ldr = ldr;
     p.out = out; p.ldo = ldo; p.gelu = activation == SAMQ_ACT_GELU; p.status = status;
     p.vec_ok = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (ldo * esz) % 16 == 0;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaStream_t st = c.stream;
     switch (out_dtype) {
     case SAMQ_F16:  return launch<__half>(fmt, ma, mw, p, st);
     case SAMQ_BF16: return launch<__nv_bfloat16>(fmt, ma, mw, p, st);

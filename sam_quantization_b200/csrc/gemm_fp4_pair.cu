@@ -1,0 +1,292 @@
+// The 4-bit product for many rows: a persistent kernel on CTA pairs (tcgen05 cta_group::2).
+//
+// A pair owns a 256 x 256 output tile.  Each CTA loads its own 128 rows of A with their scales, half of the W tile (128
+// of 256 rows) and the scales of the whole W tile: 38 KiB (nvfp4) or 35 KiB (mxfp4) a stage of 256 columns, four stages.
+// The leader copies both operands' scales to tensor memory (in both CTAs, each from its own shared memory) and issues
+// the stage's four MMAs (M = 256, N = 256, K = 64).  cp and mma of one thread run in order, so the scale columns are
+// simply overwritten by the next stage.
+//
+// Tensor memory: two accumulators of 256 columns do not fit beside 48 columns of scales, so they overlap: buffer 0 is
+// columns [0, 256), buffer 1 [208, 464), the scales [464, 512).  The epilogue warps read their 64 columns at once and
+// hand them back before they compute; the MMAs of the next tile start when the four warps that hold the shared columns
+// have done so.
+//
+// Sixteen epilogue warps (32 rows x 64 columns each): with GELU a tile takes about as many issue slots as its K = 1280
+// main loop takes tensor-core clocks, so the epilogue needs the whole SM.  The residual comes in by TMA into the warp's
+// staging buffer while the tile is computed, the result leaves from there by TMA.  Every wait is bounded.
+#include "fp4_gemm.cuh"
+
+namespace samq {
+namespace fp4 {
+
+namespace {
+
+constexpr int BM = 128;                          // rows of A of a CTA
+constexpr int BN = 256;                          // columns of the pair's tile
+constexpr int BNH = BN / 2;                      // rows of W of a CTA
+constexpr int STAGES = 4;
+constexpr int A_BYTES = BM * BK;
+constexpr int B_BYTES = BNH * BK;
+constexpr int EPI_WARPS = 4 * (BN / EPI_COLS);
+constexpr int THREADS = 64 + EPI_WARPS * 32;
+constexpr int TMEM_COLS = 512;
+constexpr int SF_COL = 464;
+constexpr int ACC1_COL = SF_COL - BN;            // 208: the second accumulator shares [208, 256) with the first
+
+template <int FMT> struct Shape {
+    static constexpr int GROUPS = groups_per_kpad(FMT);
+    static constexpr int SFA_BYTES = GROUPS * TILE_BYTES;
+    static constexpr int SFB_BYTES = 2 * GROUPS * TILE_BYTES;
+    static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
+    static constexpr int SFB_COL = SF_COL + 4 * GROUPS;
+    static_assert(SFB_COL + 8 * GROUPS <= TMEM_COLS, "the scales of a stage behind the accumulators");
+};
+
+struct __align__(8) Control {
+    uint64_t full[STAGES];
+    uint64_t empty[STAGES];
+    uint64_t acc_full[2];
+    uint64_t acc_empty[2];
+    uint64_t shared_empty;                        // the columns that the two accumulators share
+    uint64_t res[EPI_WARPS];
+    uint32_t tmem_base;
+    uint32_t abort_flag;
+};
+
+template <int FMT>
+constexpr size_t smem_bytes() {
+    return 1024 + (size_t)STAGES * Shape<FMT>::STAGE_BYTES + (size_t)EPI_WARPS * (STAGING_BYTES + EPI_COLS * sizeof(float)) + sizeof(Control);
+}
+
+struct PairParams {
+    EpiParams epi;
+    int K, groups;
+    int32_t* status;
+};
+
+template <typename OutT, int FMT, bool GELU, bool RES>
+__global__ void __launch_bounds__(THREADS, 1)
+gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+                     const __grid_constant__ CUtensorMap map_sfa, const __grid_constant__ CUtensorMap map_sfw,
+                     const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_res,
+                     const __grid_constant__ PairParams p)
+{
+    using S = Shape<FMT>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_addr = smem_u32(smem_raw);
+    uint8_t* tiles = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);              // 1024-byte aligned
+    uint8_t* staging = tiles + (size_t)STAGES * (A_BYTES + B_BYTES);                     // 1024-byte aligned
+    uint8_t* sf = staging + (size_t)EPI_WARPS * STAGING_BYTES;
+    float* bias_s = reinterpret_cast<float*>(sf + (size_t)STAGES * (S::SFA_BYTES + S::SFB_BYTES));
+    Control* ctl = reinterpret_cast<Control*>(bias_s + EPI_WARPS * EPI_COLS);
+    volatile uint32_t* abort_flag = &ctl->abort_flag;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();                       // 0 = leader of the pair
+    const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+    const int m_blocks = (p.epi.M + 2 * BM - 1) / (2 * BM);
+    const int n_blocks = (p.epi.N + BN - 1) / BN;
+    const int k_blocks = (p.K + KPAD - 1) / KPAD;
+    const int num_tiles = m_blocks * n_blocks;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) { mbar_init(smem_u32(&ctl->full[s]), 1); mbar_init(smem_u32(&ctl->empty[s]), 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(smem_u32(&ctl->acc_full[b]), 1); mbar_init(smem_u32(&ctl->acc_empty[b]), 2 * EPI_WARPS); }
+        mbar_init(smem_u32(&ctl->shared_empty), 2 * 4);
+        for (int w = 0; w < EPI_WARPS; ++w) mbar_init(smem_u32(&ctl->res[w]), 1);
+        ctl->abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(&ctl->tmem_base)), "r"((uint32_t)TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    cluster_sync();                                                // both CTAs' barriers exist before any remote arrival
+    tcgen05_fence_after();
+    const uint32_t tmem = ctl->tmem_base;
+
+    if (warp == 0) {
+        // ---------------- TMA producer ----------------
+        if (lane == 0) {
+            int stage = 0; uint32_t phase = 0;
+            bool ok = true;
+            for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+                const int mt = (tile / n_blocks) * 2 + (int)rank;          // this CTA's 128-row tile of A
+                const int nt = (tile % n_blocks) * 2;                      // first 128-row tile of W
+                for (int kb = 0; kb < k_blocks; ++kb) {
+                    if (!mbar_wait(smem_u32(&ctl->empty[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
+                    const uint32_t bar = smem_u32(&ctl->full[stage]);
+                    const uint32_t leader_bar = map_to_cta(bar, 0);
+                    const uint32_t sa = smem_u32(tiles + (size_t)stage * (A_BYTES + B_BYTES));
+                    const uint32_t ss = smem_u32(sf + (size_t)stage * (S::SFA_BYTES + S::SFB_BYTES));
+                    if (rank == 0) mbar_expect_tx(bar, 2 * S::STAGE_BYTES);       // bytes of both CTAs
+                    tma_load_2d_pair(sa, &map_a, leader_bar, kb * BK, mt * BM);
+                    tma_load_2d_pair(sa + A_BYTES, &map_w, leader_bar, kb * BK, (nt + (int)rank) * BNH);
+                    tma_load_2d_pair(ss, &map_sfa, leader_bar, 0, mt * p.groups + kb * S::GROUPS);
+                    tma_load_2d_pair(ss + S::SFA_BYTES, &map_sfw, leader_bar, 0, nt * p.groups + kb * S::GROUPS);
+                    tma_load_2d_pair(ss + S::SFA_BYTES + S::SFB_BYTES / 2, &map_sfw, leader_bar, 0, (nt + 1) * p.groups + kb * S::GROUPS);
+                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                }
+            }
+            // every stage has been handed back: no completion from the leader's MMA thread can still be on its way
+            // to this CTA's barriers when the CTA retires
+            for (int s = 0; s < STAGES && ok; ++s) {
+                if (!mbar_wait(smem_u32(&ctl->empty[stage]), phase ^ 1u, abort_flag)) ok = false;
+                if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+            }
+            if (!ok) {
+                const long long t0 = clock64();
+                while (clock64() - t0 < 2000000LL) { }              // copies in flight land before the CTA retires
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer ----------------
+        if (lane == 0 && rank == 0) {
+            int stage = 0; uint32_t phase = 0;
+            int acc = 0; uint32_t acc_phase = 0, shared_phase = 1;
+            bool ok = true;
+            for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+                // the buffer itself (two tiles ago) and the columns that the previous tile's buffer shares with it
+                if (!mbar_wait(smem_u32(&ctl->acc_empty[acc]), acc_phase ^ 1u, abort_flag) ||
+                    !mbar_wait(smem_u32(&ctl->shared_empty), shared_phase, abort_flag)) { ok = false; break; }
+                shared_phase ^= 1u;
+                tcgen05_fence_after();
+                const uint32_t tmem_d = tmem + (uint32_t)(acc * ACC1_COL);
+                for (int kb = 0; kb < k_blocks; ++kb) {
+                    if (!mbar_wait(smem_u32(&ctl->full[stage]), phase, abort_flag)) { ok = false; break; }
+                    tcgen05_fence_after();
+                    const uint32_t sa = smem_u32(tiles + (size_t)stage * (A_BYTES + B_BYTES));
+                    const uint32_t ss = smem_u32(sf + (size_t)stage * (S::SFA_BYTES + S::SFB_BYTES));
+#pragma unroll
+                    for (int g = 0; g < S::GROUPS; ++g) {
+                        tmem_copy_scales<2>(tmem + SF_COL + 4 * g, scale_desc(ss + g * TILE_BYTES));
+                        tmem_copy_scales<2>(tmem + S::SFB_COL + 8 * g, scale_desc(ss + S::SFA_BYTES + g * TILE_BYTES));
+                        tmem_copy_scales<2>(tmem + S::SFB_COL + 8 * g + 4, scale_desc(ss + S::SFA_BYTES + S::SFB_BYTES / 2 + g * TILE_BYTES));
+                    }
+                    const uint64_t adesc = make_smem_desc(sa), bdesc = make_smem_desc(sa + A_BYTES);
+#pragma unroll
+                    for (int k = 0; k < BK / UKB; ++k) {
+                        // mxfp4: a word of four scales serves two MMAs, the second taking its upper half (scale id 2)
+                        const int g = FMT == SAMQ_FP4_MX ? k / 2 : k;
+                        const uint32_t id = FMT == SAMQ_FP4_MX ? 2u * (k & 1) : 0u;
+                        mma_fp4<FMT, 2>(tmem_d, adesc + (uint64_t)(k * (UKB >> 4)), bdesc + (uint64_t)(k * (UKB >> 4)),
+                                        instr_desc(FMT, 2 * BM, BN, id), tmem + SF_COL + 4 * g, tmem + S::SFB_COL + 8 * g, (kb | k) != 0 ? 1u : 0u);
+                    }
+                    tcgen05_commit_pair(map_to_cta(smem_u32(&ctl->empty[stage]), 0));
+                    tcgen05_commit_pair(map_to_cta(smem_u32(&ctl->empty[stage]), 1));
+                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                }
+                if (!ok) break;
+                tcgen05_commit_pair(map_to_cta(smem_u32(&ctl->acc_full[acc]), 0));
+                tcgen05_commit_pair(map_to_cta(smem_u32(&ctl->acc_full[acc]), 1));
+                if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+            }
+        }
+    } else {
+        // ---------------- epilogue ----------------
+        const int ew = warp - 2;
+        const int quad = warp & 3;                                  // TMEM lane quadrant this warp may read
+        const int cg = ew >> 2;                                     // which 64 columns
+        EpiWarp<OutT, GELU, RES> epi{p.epi, &map_out, &map_res, staging + (size_t)ew * STAGING_BYTES, bias_s + ew * EPI_COLS,
+                                     smem_u32(&ctl->res[ew]), 0u, abort_flag, lane};
+        int acc = 0; uint32_t acc_phase = 0;
+        for (int tile = pair; tile < num_tiles; tile += num_pairs) {
+            const int row0 = (tile / n_blocks) * (2 * BM) + (int)rank * BM + quad * 32;
+            const int col0 = (tile % n_blocks) * BN + cg * EPI_COLS;
+            epi.before(row0, col0);
+            if (!mbar_wait(smem_u32(&ctl->acc_full[acc]), acc_phase, abort_flag)) break;
+            tcgen05_fence_after();
+            uint32_t r[EPI_COLS];
+            tmem_ld64(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * ACC1_COL + cg * EPI_COLS), r);
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (cg == (acc == 0 ? BN / EPI_COLS - 1 : 0)) mbar_arrive_cluster(map_to_cta(smem_u32(&ctl->shared_empty), 0));
+                mbar_arrive_cluster(map_to_cta(smem_u32(&ctl->acc_empty[acc]), 0));
+            }
+            if (!epi.finish(row0, col0, r)) break;
+            if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+        }
+        if (lane == 0) bulk_wait0();                                // this warp's stores have completed
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    cluster_sync();                                   // no remote arrival or MMA read of the peer is still in flight
+    if (warp == 1) {
+        __syncwarp();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)TMEM_COLS) : "memory");
+    }
+    if (threadIdx.x == 0 && ctl->abort_flag != 0 && p.status != nullptr) atomicExch(p.status, 1);
+}
+
+template <typename OutT, int FMT, bool GELU, bool RES>
+int launch(const Fp4Call& c, const CUtensorMap& ma, const CUtensorMap& mw, const CUtensorMap& msa, const CUtensorMap& msw, const PairParams& p) {
+    auto kernel = gemm_fp4_pair_kernel<OutT, FMT, GELU, RES>;
+    SAMQ_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<FMT>()));
+    const int64_t tiles = ((c.M + 2 * BM - 1) / (2 * BM)) * ((c.N + BN - 1) / BN);
+    if (tiles > 2147483647LL - 256) return fail(SAMQ_ERR_TOO_LARGE, "product of %lld x %lld outputs is too large", (long long)c.M, (long long)c.N);
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = smem_bytes<FMT>(); cfg.stream = c.stream;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    // how many pairs the device can hold at once (GPCs with an odd number of SMs leave one out)
+    static thread_local int pairs_cached[64] = {0};
+    int dev = 0;
+    SAMQ_CUDA_TRY(cudaGetDevice(&dev));
+    int max_pairs = (dev >= 0 && dev < 64) ? pairs_cached[dev] : 0;
+    if (max_pairs == 0) {
+        cfg.gridDim = dim3(2 * (sm_count() / 2));
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) { (void)cudaGetLastError(); n = sm_count() / 2 - 4; }
+        max_pairs = n;
+        if (dev >= 0 && dev < 64) pairs_cached[dev] = n;
+    }
+    const int pairs = tiles < max_pairs ? (int)tiles : max_pairs;
+    cfg.gridDim = dim3(2 * pairs);
+    SAMQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, ma, mw, msa, msw, c.map_out, c.map_res, p));
+    return SAMQ_OK;
+}
+
+template <typename OutT, int FMT>
+int launch(const Fp4Call& c) {
+    CUtensorMap ma, mw, msa, msw;
+    const int64_t row_bytes = (c.K + 1) / 2;
+    int rc = make_operand_map(&ma, reinterpret_cast<const int8_t*>(c.A), c.M, row_bytes, c.lda, BM);
+    if (rc == SAMQ_OK) rc = make_operand_map(&mw, reinterpret_cast<const int8_t*>(c.W), c.N, row_bytes, c.ldw, BNH);
+    const int64_t groups = groups_of(FMT, c.K);
+    if (rc == SAMQ_OK) rc = make_scale_map(&msa, c.a_scales, (c.M + TILE_ROWS - 1) / TILE_ROWS * groups, Shape<FMT>::GROUPS);
+    if (rc == SAMQ_OK) rc = make_scale_map(&msw, c.w_scales, (c.N + TILE_ROWS - 1) / TILE_ROWS * groups, Shape<FMT>::GROUPS);
+    if (rc != SAMQ_OK) return rc;
+    PairParams p;
+    p.epi = c.epi; p.K = (int)c.K; p.groups = (int)groups; p.status = c.status;
+    const bool res = c.epi.residual != nullptr;
+    if (c.gelu && res) return launch<OutT, FMT, true, true>(c, ma, mw, msa, msw, p);
+    if (c.gelu) return launch<OutT, FMT, true, false>(c, ma, mw, msa, msw, p);
+    if (res) return launch<OutT, FMT, false, true>(c, ma, mw, msa, msw, p);
+    return launch<OutT, FMT, false, false>(c, ma, mw, msa, msw, p);
+}
+
+template <typename OutT>
+int launch(const Fp4Call& c) {
+    return c.fmt == SAMQ_FP4_MX ? launch<OutT, SAMQ_FP4_MX>(c) : launch<OutT, SAMQ_FP4_NV>(c);
+}
+
+}  // namespace
+
+int gemm_fp4_pair(const Fp4Call& c) {
+    switch (c.out_dtype) {
+    case SAMQ_F16:  return launch<__half>(c);
+    case SAMQ_BF16: return launch<__nv_bfloat16>(c);
+    default:        return launch<float>(c);
+    }
+}
+
+}  // namespace fp4
+}  // namespace samq

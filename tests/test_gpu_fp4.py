@@ -118,7 +118,7 @@ def _exact_operand(rows, K, fmt, dev, seed):
 
 
 SHAPES = [(1, 1, 1), (1, 8, 64), (3, 130, 31), (1, 5120, 1280), (128, 128, 256), (129, 257, 300), (200, 40, 1283), (64, 1001, 512), (16, 300, 2048),
-          (17, 65, 96), (40, 200, 4100), (260, 520, 768), (1000, 384, 200), (300, 1280, 5120)]
+          (17, 65, 96), (40, 200, 4100), (260, 520, 768), (1000, 384, 200), (300, 1280, 5120), (2600, 1300, 600), (8200, 257, 1283), (290, 8210, 300), (4096, 2304, 768)]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -134,7 +134,7 @@ def test_product_is_exact_where_its_sums_are(cuda_device, fmt, M, N, K):
 
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("M,N,K", [(1, 300, 1280), (5, 72, 100), (40, 1001, 2000), (130, 257, 1283), (600, 640, 512)])
+@pytest.mark.parametrize("M,N,K", [(1, 300, 1280), (5, 72, 100), (40, 1001, 2000), (130, 257, 1283), (600, 640, 512), (2050, 1096, 300), (2050, 1101, 300)])
 @pytest.mark.parametrize("bias,gelu,residual", [(True, False, False), (True, True, False), (False, False, True), (True, True, True)])
 def test_epilogue(cuda_device, fmt, dtype, M, N, K, bias, gelu, residual):
     """Exact sums, so only the epilogue rounds: alpha and bias in one fused step (u), GELU (3e-7 absolute and 2e-5
@@ -183,7 +183,7 @@ def test_product_of_quantized_data(cuda_device, fmt, M, N, K):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("M", [1, 200])
+@pytest.mark.parametrize("M", [1, 200, 9000])
 def test_rows_that_are_not_finite_stay_apart(cuda_device, fmt, M):
     x = _values(M, 300, torch.float16)
     x[M // 2, 299] = float("nan")
@@ -194,7 +194,7 @@ def test_rows_that_are_not_finite_stay_apart(cuda_device, fmt, M):
     assert y[M // 2].isnan().all() and not y[rows].isnan().any()
 
 
-@pytest.mark.parametrize("M", [3, 200, 700])
+@pytest.mark.parametrize("M", [3, 200, 700, 9000])
 def test_strided_outputs_and_operands(cuda_device, M):
     a, av = _exact_operand(M, 320, "nvfp4", cuda_device, 1)
     w, wv = _exact_operand(130, 320, "nvfp4", cuda_device, 2)
