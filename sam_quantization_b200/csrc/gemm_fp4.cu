@@ -14,7 +14,7 @@ using namespace fp4;
 
 namespace {
 
-// 256 x 256 tiles from which the pair kernel has enough to do
+// 256 x 192 tiles from which the pair kernel has enough to do
 constexpr int PAIR_MIN_TILES = 32;
 
 constexpr int BM = 128;
@@ -240,7 +240,7 @@ int gemm_fp4_dispatch(const uint8_t* A, int64_t lda, const uint8_t* a_scales, co
     c.epi.out = out; c.epi.ldo = ldo;
     c.epi.tma_out = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (ldo * esz) % 16 == 0;
     c.epi.tma_res = residual != nullptr && (reinterpret_cast<uintptr_t>(residual) & 15) == 0 && (ldr * esz) % 16 == 0;
-    if ((M + 255) / 256 * ((N + 255) / 256) >= PAIR_MIN_TILES) {
+    if ((M + 255) / 256 * ((N + 191) / 192) >= PAIR_MIN_TILES) {
         memset(&c.map_out, 0, sizeof(c.map_out));
         memset(&c.map_res, 0, sizeof(c.map_res));
         int rc = SAMQ_OK;

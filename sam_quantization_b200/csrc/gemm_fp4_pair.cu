@@ -1,19 +1,20 @@
 // The 4-bit product for many rows: a persistent kernel on CTA pairs (tcgen05 cta_group::2).
 //
-// A pair owns a 256 x 256 output tile.  Each CTA loads its own 128 rows of A with their scales, half of the W tile (128
-// of 256 rows) and the scales of the whole W tile: 38 KiB (nvfp4) or 35 KiB (mxfp4) a stage of 256 columns, four stages.
-// The leader copies both operands' scales to tensor memory (in both CTAs, each from its own shared memory) and issues
-// the stage's four MMAs (M = 256, N = 256, K = 64).  cp and mma of one thread run in order, so the scale columns are
-// simply overwritten by the next stage.
+// A pair owns a 256 x 192 output tile.  Each CTA loads its own 128 rows of A with their scales, half of the W tile (96
+// of 192 rows) and the scales of the whole W tile: 34 KiB (nvfp4) or 31 KiB (mxfp4) a stage of 256 columns, five stages.
+// Per stage the leader issues four MMAs (M = 256, N = 192, K = 64).
 //
-// Tensor memory: two accumulators of 256 columns do not fit beside 48 columns of scales, so they overlap: buffer 0 is
-// columns [0, 256), buffer 1 [208, 464), the scales [464, 512).  The epilogue warps read their 64 columns at once and
-// hand them back before they compute; the MMAs of the next tile start when the four warps that hold the shared columns
-// have done so.
+// The scales reach tensor memory by tcgen05.cp, 12 copies of 512 bytes a stage for nvfp4 and 6 for mxfp4, each about 40
+// clocks.  Issued by the MMA thread they run in order with its MMAs and their time adds up; a thread of its own issues
+// them, so that they run beside the MMAs, half a stage (two MMAs) at a time into a ring of four buffers.  Measured at
+// 32768 x 5120 x 5120 with 256-column tiles: 516 us in the MMA thread, 384 beside it (nvfp4), 405 and 301 (mxfp4).
 //
-// Sixteen epilogue warps (32 rows x 64 columns each): with GELU a tile takes about as many issue slots as its K = 1280
-// main loop takes tensor-core clocks, so the epilogue needs the whole SM.  The residual comes in by TMA into the warp's
-// staging buffer while the tile is computed, the result leaves from there by TMA.  Every wait is bounded.
+// Two accumulators of 192 columns and the ring fill tensor memory.  256-column tiles would have to share columns between
+// the two accumulators; the hand-over across the pair that this needs took 1.5 us a tile.
+//
+// Twelve epilogue warps (32 rows x 64 columns each) read their columns at once and hand them back before they compute.
+// The residual comes in by TMA into the warp's staging buffer while the tile is computed, the result leaves from there
+// by TMA.  Every wait is bounded.
 #include "fp4_gemm.cuh"
 
 namespace samq {
@@ -22,24 +23,25 @@ namespace fp4 {
 namespace {
 
 constexpr int BM = 128;                          // rows of A of a CTA
-constexpr int BN = 256;                          // columns of the pair's tile
+constexpr int BN = 192;                          // columns of the pair's tile
 constexpr int BNH = BN / 2;                      // rows of W of a CTA
-constexpr int STAGES = 4;
+constexpr int STAGES = 5;
 constexpr int A_BYTES = BM * BK;
 constexpr int B_BYTES = BNH * BK;
 constexpr int EPI_WARPS = 4 * (BN / EPI_COLS);
-constexpr int THREADS = 64 + EPI_WARPS * 32;
+constexpr int FIRST_EPI_WARP = 4;                // TMA, MMA, scale copies, one idle
+constexpr int THREADS = (FIRST_EPI_WARP + EPI_WARPS) * 32;
 constexpr int TMEM_COLS = 512;
-constexpr int SF_COL = 464;
-constexpr int ACC1_COL = SF_COL - BN;            // 208: the second accumulator shares [208, 256) with the first
+constexpr int SF_COL = 2 * BN;                   // the ring of scale columns behind the accumulators
 
 template <int FMT> struct Shape {
-    static constexpr int GROUPS = groups_per_kpad(FMT);
+    static constexpr int GROUPS = groups_per_kpad(FMT);            // scale tiles of 128 rows a stage
+    static constexpr int UNIT_COLS = 12 * GROUPS;                  // a buffer of the ring: per group 4 columns for A, 8 for W
+    static constexpr int UNITS = FMT == SAMQ_FP4_MX ? 4 : 2;
+    static_assert(SF_COL + UNITS * UNIT_COLS <= TMEM_COLS, "accumulators and scales fit tensor memory");
     static constexpr int SFA_BYTES = GROUPS * TILE_BYTES;
-    static constexpr int SFB_BYTES = 2 * GROUPS * TILE_BYTES;
+    static constexpr int SFB_BYTES = 2 * GROUPS * TILE_BYTES;      // 192 rows of W lie in two tiles of 128
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
-    static constexpr int SFB_COL = SF_COL + 4 * GROUPS;
-    static_assert(SFB_COL + 8 * GROUPS <= TMEM_COLS, "the scales of a stage behind the accumulators");
 };
 
 struct __align__(8) Control {
@@ -47,7 +49,7 @@ struct __align__(8) Control {
     uint64_t empty[STAGES];
     uint64_t acc_full[2];
     uint64_t acc_empty[2];
-    uint64_t shared_empty;                        // the columns that the two accumulators share
+    uint64_t sf_ready[4];                         // scale columns written (the leader's only)
     uint64_t res[EPI_WARPS];
     uint32_t tmem_base;
     uint32_t abort_flag;
@@ -92,7 +94,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(smem_u32(&ctl->full[s]), 1); mbar_init(smem_u32(&ctl->empty[s]), 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(smem_u32(&ctl->acc_full[b]), 1); mbar_init(smem_u32(&ctl->acc_empty[b]), 2 * EPI_WARPS); }
-        mbar_init(smem_u32(&ctl->shared_empty), 2 * 4);
+        for (int u = 0; u < 4; ++u) mbar_init(smem_u32(&ctl->sf_ready[u]), 1);
         for (int w = 0; w < EPI_WARPS; ++w) mbar_init(smem_u32(&ctl->res[w]), 1);
         ctl->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -115,7 +117,8 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             bool ok = true;
             for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
                 const int mt = (tile / n_blocks) * 2 + (int)rank;          // this CTA's 128-row tile of A
-                const int nt = (tile % n_blocks) * 2;                      // first 128-row tile of W
+                const int n0 = (tile % n_blocks) * BN;
+                const int nt = n0 / TILE_ROWS;                             // first of W's two scale tiles
                 for (int kb = 0; kb < k_blocks; ++kb) {
                     if (!mbar_wait(smem_u32(&ctl->empty[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
                     const uint32_t bar = smem_u32(&ctl->full[stage]);
@@ -124,7 +127,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                     const uint32_t ss = smem_u32(sf + (size_t)stage * (S::SFA_BYTES + S::SFB_BYTES));
                     if (rank == 0) mbar_expect_tx(bar, 2 * S::STAGE_BYTES);       // bytes of both CTAs
                     tma_load_2d_pair(sa, &map_a, leader_bar, kb * BK, mt * BM);
-                    tma_load_2d_pair(sa + A_BYTES, &map_w, leader_bar, kb * BK, (nt + (int)rank) * BNH);
+                    tma_load_2d_pair(sa + A_BYTES, &map_w, leader_bar, kb * BK, n0 + (int)rank * BNH);
                     tma_load_2d_pair(ss, &map_sfa, leader_bar, 0, mt * p.groups + kb * S::GROUPS);
                     tma_load_2d_pair(ss + S::SFA_BYTES, &map_sfw, leader_bar, 0, nt * p.groups + kb * S::GROUPS);
                     tma_load_2d_pair(ss + S::SFA_BYTES + S::SFB_BYTES / 2, &map_sfw, leader_bar, 0, (nt + 1) * p.groups + kb * S::GROUPS);
@@ -144,50 +147,84 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             int stage = 0; uint32_t phase = 0;
-            int acc = 0; uint32_t acc_phase = 0, shared_phase = 1;
+            int acc = 0; uint32_t acc_phase = 0;
+            int unit = 0; uint32_t unit_phase = 0;
             bool ok = true;
             for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
-                // the buffer itself (two tiles ago) and the columns that the previous tile's buffer shares with it
-                if (!mbar_wait(smem_u32(&ctl->acc_empty[acc]), acc_phase ^ 1u, abort_flag) ||
-                    !mbar_wait(smem_u32(&ctl->shared_empty), shared_phase, abort_flag)) { ok = false; break; }
-                shared_phase ^= 1u;
-                tcgen05_fence_after();
-                const uint32_t tmem_d = tmem + (uint32_t)(acc * ACC1_COL);
+                if (!mbar_wait(smem_u32(&ctl->acc_empty[acc]), acc_phase ^ 1u, abort_flag)) break;
+                const uint32_t tmem_d = tmem + (uint32_t)(acc * BN);
+                // an odd tile's 192 rows begin in the middle of a scale tile: skip its first 64 rows, two columns
+                const uint32_t sf_shift = (uint32_t)((tile % n_blocks) & 1) * 2u;
                 for (int kb = 0; kb < k_blocks; ++kb) {
-                    if (!mbar_wait(smem_u32(&ctl->full[stage]), phase, abort_flag)) { ok = false; break; }
+                    ok = mbar_wait(smem_u32(&ctl->full[stage]), phase, abort_flag) &&
+                         mbar_wait(smem_u32(&ctl->sf_ready[unit]), unit_phase, abort_flag);
+                    if (!ok) break;
                     tcgen05_fence_after();
                     const uint32_t sa = smem_u32(tiles + (size_t)stage * (A_BYTES + B_BYTES));
-                    const uint32_t ss = smem_u32(sf + (size_t)stage * (S::SFA_BYTES + S::SFB_BYTES));
-#pragma unroll
-                    for (int g = 0; g < S::GROUPS; ++g) {
-                        tmem_copy_scales<2>(tmem + SF_COL + 4 * g, scale_desc(ss + g * TILE_BYTES));
-                        tmem_copy_scales<2>(tmem + S::SFB_COL + 8 * g, scale_desc(ss + S::SFA_BYTES + g * TILE_BYTES));
-                        tmem_copy_scales<2>(tmem + S::SFB_COL + 8 * g + 4, scale_desc(ss + S::SFA_BYTES + S::SFB_BYTES / 2 + g * TILE_BYTES));
-                    }
                     const uint64_t adesc = make_smem_desc(sa), bdesc = make_smem_desc(sa + A_BYTES);
+                    const uint32_t sfa = tmem + SF_COL + (uint32_t)(unit * S::UNIT_COLS);
+                    const uint32_t sfb = sfa + 4 * S::GROUPS + sf_shift;
+                    if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < BK / UKB; ++k) {
-                        // mxfp4: a word of four scales serves two MMAs, the second taking its upper half (scale id 2)
-                        const int g = FMT == SAMQ_FP4_MX ? k / 2 : k;
-                        const uint32_t id = FMT == SAMQ_FP4_MX ? 2u * (k & 1) : 0u;
-                        mma_fp4<FMT, 2>(tmem_d, adesc + (uint64_t)(k * (UKB >> 4)), bdesc + (uint64_t)(k * (UKB >> 4)),
-                                        instr_desc(FMT, 2 * BM, BN, id), tmem + SF_COL + 4 * g, tmem + S::SFB_COL + 8 * g, (kb | k) != 0 ? 1u : 0u);
+                        for (int k = 0; k < BK / UKB; ++k) {
+                            // mxfp4: a word of four scales serves two MMAs, the second taking its upper half (scale id 2)
+                            const int g = FMT == SAMQ_FP4_MX ? k / 2 : k;
+                            const uint32_t id = FMT == SAMQ_FP4_MX ? 2u * (k & 1) : 0u;
+                            mma_fp4<FMT, 2>(tmem_d, adesc + (uint64_t)(k * (UKB >> 4)), bdesc + (uint64_t)(k * (UKB >> 4)),
+                                            instr_desc(FMT, 2 * BM, BN, id), sfa + 4 * g, sfb + 8 * g, (kb | k) != 0 ? 1u : 0u);
+                        }
+                        tcgen05_commit_both(smem_u32(&ctl->empty[stage]));
+                        if (kb == k_blocks - 1) tcgen05_commit_both(smem_u32(&ctl->acc_full[acc]));
                     }
-                    tcgen05_commit_pair(map_to_cta(smem_u32(&ctl->empty[stage]), 0));
-                    tcgen05_commit_pair(map_to_cta(smem_u32(&ctl->empty[stage]), 1));
+                    __syncwarp();
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                    if (++unit == S::UNITS) { unit = 0; unit_phase ^= 1u; }
                 }
-                if (!ok) break;
-                tcgen05_commit_pair(map_to_cta(smem_u32(&ctl->acc_full[acc]), 0));
-                tcgen05_commit_pair(map_to_cta(smem_u32(&ctl->acc_full[acc]), 1));
                 if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
             }
         }
-    } else {
+    } else if (warp == 2) {
+        // ---------------- scale copies ----------------
+        if (rank == 0) {
+            int stage = 0; uint32_t phase = 0;
+            int unit = 0;
+            int old_stage = 0; uint32_t old_phase = 0;             // the stage that last used the buffer
+            int filled = 0;
+            bool ok = true;
+            for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+                for (int kb = 0; kb < k_blocks; ++kb) {
+                    ok = mbar_wait(smem_u32(&ctl->full[stage]), phase, abort_flag);
+                    if (ok && filled == S::UNITS) {
+                        ok = mbar_wait(smem_u32(&ctl->empty[old_stage]), old_phase, abort_flag);
+                        if (++old_stage == STAGES) { old_stage = 0; old_phase ^= 1u; }
+                    } else {
+                        ++filled;
+                    }
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                    const uint32_t ss = smem_u32(sf + (size_t)stage * (S::SFA_BYTES + S::SFB_BYTES));
+                    const uint32_t sfa = tmem + SF_COL + (uint32_t)(unit * S::UNIT_COLS);
+                    const uint32_t sfb = sfa + 4 * S::GROUPS;
+                    if (elect_one()) {
+#pragma unroll
+                        for (int g = 0; g < S::GROUPS; ++g) {
+                            tmem_copy_scales<2>(sfa + 4 * g, scale_desc(ss + g * TILE_BYTES));
+                            tmem_copy_scales<2>(sfb + 8 * g, scale_desc(ss + S::SFA_BYTES + g * TILE_BYTES));
+                            tmem_copy_scales<2>(sfb + 8 * g + 4, scale_desc(ss + S::SFA_BYTES + S::SFB_BYTES / 2 + g * TILE_BYTES));
+                        }
+                        tcgen05_commit_pair(smem_u32(&ctl->sf_ready[unit]));
+                    }
+                    __syncwarp();
+                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                    if (++unit == S::UNITS) unit = 0;
+                }
+            }
+        }
+    } else if (warp >= FIRST_EPI_WARP) {
         // ---------------- epilogue ----------------
-        const int ew = warp - 2;
+        const int ew = warp - FIRST_EPI_WARP;
         const int quad = warp & 3;                                  // TMEM lane quadrant this warp may read
         const int cg = ew >> 2;                                     // which 64 columns
         EpiWarp<OutT, GELU, RES> epi{p.epi, &map_out, &map_res, staging + (size_t)ew * STAGING_BYTES, bias_s + ew * EPI_COLS,
@@ -200,13 +237,10 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             if (!mbar_wait(smem_u32(&ctl->acc_full[acc]), acc_phase, abort_flag)) break;
             tcgen05_fence_after();
             uint32_t r[EPI_COLS];
-            tmem_ld64(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * ACC1_COL + cg * EPI_COLS), r);
+            tmem_ld64(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN + cg * EPI_COLS), r);
             tcgen05_fence_before();
             __syncwarp();
-            if (lane == 0) {
-                if (cg == (acc == 0 ? BN / EPI_COLS - 1 : 0)) mbar_arrive_cluster(map_to_cta(smem_u32(&ctl->shared_empty), 0));
-                mbar_arrive_cluster(map_to_cta(smem_u32(&ctl->acc_empty[acc]), 0));
-            }
+            if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&ctl->acc_empty[acc]), 0));
             if (!epi.finish(row0, col0, r)) break;
             if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
         }

@@ -5,6 +5,9 @@
     python -m sam_quantization_b200.kernel_bench attn  --windows 200 --H 14 --W 14 --heads 16 --head-dim 80
     python -m sam_quantization_b200.kernel_bench attn-global --images 8 --H 64 --heads 16 --head-dim 80
     python -m sam_quantization_b200.kernel_bench attn-window14 --windows 200 --heads 16 --head-dim 80
+    python -m sam_quantization_b200.kernel_bench fp4-gemm --M 32768 --N 5120 --K 1280 --fmt nvfp4 --gelu [--linear]
+    python -m sam_quantization_b200.kernel_bench fp4-quant --M 32768 --K 5120 --fmt mxfp4 [--values]
+    python -m sam_quantization_b200.kernel_bench rms-norm --M 32768 --K 1280 [--residual] [--values]
     python -m sam_quantization_b200.kernel_bench sweep            # the W8A8 GEMM sweep: M x (K, N) x granularity
     python -m sam_quantization_b200.kernel_bench library --M 32768 --N 5120 --K 1280   # cuBLASLt int8 / fp16 bars
 
@@ -164,6 +167,55 @@ def bench_quant(M, K, dtype=torch.float16, ln=False, gather=False, hadamard=None
             "hadamard": hadamard, "granularity": granularity, "ms": round(ms, 5), "gbs": round(nbytes / ms / 1e6, 1)}
 
 
+def bench_fp4_gemm(M, N, K, fmt="nvfp4", gelu=False, residual=False, linear=False, dtype=torch.float16, iters=50, warmup=10):
+    """The 4-bit product (``linear``: with the activation's quantization in front), TFLOP/s over 2*M*N*K."""
+    dev = torch.device("cuda")
+    wt = torch.randn((N, K), device=dev) * 0.02
+    w = ops.quantize_fp4(wt, fmt, global_scale=ops.fp4_global_scale(float(wt.abs().max())) if fmt == "nvfp4" else 1.0)["q"]
+    nbuf = max(1, min(8, (256 << 20) // (M * K * (2 if linear else 1) // 2 + M * N * 2) + 1))
+    xs = [synthetic_activation(M, K, dtype, dev, seed=5 + i) for i in range(nbuf)]
+    acts = xs if linear else [ops.quantize_fp4(x, fmt)["q"] for x in xs]
+    outs = [torch.empty((M, N), dtype=dtype, device=dev) for _ in range(nbuf)]
+    bias = (torch.randn(N, device=dev) * 0.1).to(dtype)
+    res = torch.randn((M, N), device=dev, dtype=dtype) if residual else None
+    act = ops.ACT_GELU if gelu else ops.ACT_NONE
+
+    def run(i):
+        if linear:
+            ops.linear_fp4(acts[i % nbuf], w, bias=bias, residual=res, activation=act)
+        else:
+            ops.gemm_fp4(acts[i % nbuf], w, bias=bias, residual=res, activation=act, out_dtype=dtype, out=outs[i % nbuf])
+
+    ms = _time(run, iters, warmup)
+    ops.check_status()
+    return {"kernel": "linear_fp4" if linear else "gemm_fp4", "M": M, "N": N, "K": K, "fmt": fmt, "dtype": str(dtype).split(".")[-1],
+            "gelu": gelu, "residual": residual, "ms": round(ms, 5), "tflops": round(2.0 * M * N * K / ms / 1e9, 1)}
+
+
+def bench_fp4_quant(M, K, fmt="nvfp4", dtype=torch.float16, values=False, iters=50, warmup=10):
+    dev = torch.device("cuda")
+    esz = torch.empty((), dtype=dtype).element_size()
+    nbuf = max(1, min(8, (256 << 20) // (M * K * esz) + 1))
+    xs = [synthetic_activation(M, K, dtype, dev, seed=9 + i) for i in range(nbuf)]
+    ms = _time(lambda i: ops.quantize_fp4(xs[i % nbuf], fmt, fake_quant=values), iters, warmup)
+    nbytes = M * K * (esz * (2 if values else 1) + 0.5 + 1.0 / ops.FP4_BLOCK[fmt])
+    return {"kernel": "quant_fp4", "M": M, "K": K, "fmt": fmt, "dtype": str(dtype).split(".")[-1], "values": values,
+            "ms": round(ms, 5), "gbs": round(nbytes / ms / 1e6, 1)}
+
+
+def bench_rms_norm(M, K, dtype=torch.float16, residual=False, values=False, iters=50, warmup=10):
+    dev = torch.device("cuda")
+    esz = torch.empty((), dtype=dtype).element_size()
+    nbuf = max(1, min(8, (256 << 20) // (M * K * esz) + 1))
+    xs = [synthetic_activation(M, K, dtype, dev, seed=9 + i) for i in range(nbuf)]
+    rs = [synthetic_activation(M, K, dtype, dev, seed=90 + i) for i in range(nbuf)] if residual else [None] * nbuf
+    w = torch.ones(K, device=dev, dtype=dtype)
+    ms = _time(lambda i: ops.rms_norm_quantize(xs[i % nbuf], w, residual=rs[i % nbuf], fake_quant=values), iters, warmup)
+    nbytes = M * K * (esz * (1 + 2 * residual + values) + 1) + 4 * M
+    return {"kernel": "rms_norm_quant", "M": M, "K": K, "dtype": str(dtype).split(".")[-1], "residual": residual, "values": values,
+            "ms": round(ms, 5), "gbs": round(nbytes / ms / 1e6, 1)}
+
+
 def bench_window_attention(windows, H, W, heads, head_dim, dtype=torch.bfloat16, iters=50, warmup=10):
     dev = torch.device("cuda")
     L, C = H * W, heads * head_dim
@@ -316,6 +368,23 @@ def main():
     ag.add_argument("--head-dim", dest="head_dim", type=int, default=80)
     ag.add_argument("--iters", type=int, default=20)
     ag.add_argument("--warmup", type=int, default=5)
+    for name in ("fp4-gemm", "fp4-quant", "rms-norm"):
+        f = sub.add_parser(name)
+        f.add_argument("--M", type=int, default=32768)
+        f.add_argument("--K", type=int, default=1280)
+        f.add_argument("--dtype", default="float16", choices=["float16", "bfloat16", "float32"])
+        f.add_argument("--iters", type=int, default=50)
+        f.add_argument("--warmup", type=int, default=10)
+        if name != "rms-norm":
+            f.add_argument("--fmt", default="nvfp4", choices=list(ops.FP4_FORMATS))
+        if name == "fp4-gemm":
+            f.add_argument("--N", type=int, default=5120)
+            f.add_argument("--gelu", action="store_true")
+            f.add_argument("--linear", action="store_true", help="quantize the activation in the timed call")
+        else:
+            f.add_argument("--values", action="store_true", help="also write the dequantized values")
+        if name != "fp4-quant":
+            f.add_argument("--residual", action="store_true")
     s = sub.add_parser("sweep")
     s.add_argument("--iters", type=int, default=100)
     s.add_argument("--warmup", type=int, default=20)
@@ -344,6 +413,14 @@ def main():
     elif args.cmd == "quant":
         print(json.dumps(bench_quant(args.M, args.K, getattr(torch, args.dtype), args.ln, args.gather, args.hadamard,
                                      args.granularity, iters=args.iters, warmup=args.warmup)))
+    elif args.cmd == "fp4-gemm":
+        print(json.dumps(bench_fp4_gemm(args.M, args.N, args.K, args.fmt, args.gelu, args.residual, args.linear, getattr(torch, args.dtype),
+                                        iters=args.iters, warmup=args.warmup)))
+    elif args.cmd == "fp4-quant":
+        print(json.dumps(bench_fp4_quant(args.M, args.K, args.fmt, getattr(torch, args.dtype), args.values, iters=args.iters, warmup=args.warmup)))
+    elif args.cmd == "rms-norm":
+        print(json.dumps(bench_rms_norm(args.M, args.K, getattr(torch, args.dtype), args.residual, args.values, iters=args.iters,
+                                        warmup=args.warmup)))
     elif args.cmd == "library":
         print(json.dumps(bench_library(args.M, args.N, args.K, iters=args.iters, warmup=args.warmup)))
     else:
