@@ -149,6 +149,8 @@ def check_status(device=None) -> None:
 def _as_rows(x: torch.Tensor) -> Tuple[torch.Tensor, int, int, int]:
     """View x as [M, K] with a row stride; copies only if the last dim is not contiguous."""
     K = x.shape[-1]
+    if K and x.is_contiguous():
+        return x, x.numel() // K, K, K
     if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= K:
         return x, x.shape[0], K, x.stride(0)
     x2 = x.reshape(-1, K)
@@ -419,6 +421,31 @@ def gemm_i8(a_q: torch.Tensor, w_q: torch.Tensor,
 
 
 # ---- RMS norm with an 8-bit output -----------------------------------------------------------------
+#
+# The calls below serve single tokens too, where the host's time per call is the call's time: pointers go to ctypes
+# as plain integers, and the device is only switched when it is not the current one.
+
+def _data_ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _call(dev: torch.device, kind: str, work: float, fn, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of ``dev``, counted (and timed) like every launch."""
+    if _timing_on or torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev), _Timed(kind, work):
+            _lib.check(fn(*args, torch.cuda.current_stream().cuda_stream))
+        return
+    global _launches
+    _launches += 1
+    code = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if code:
+        _lib.check(code)
+
+
+def _status_ptr(dev: torch.device) -> int:
+    word = _status_words.get(dev.index)
+    return (status_word(dev) if word is None else word).data_ptr()
+
 
 def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None,
                       codes: bool = True, fake_quant: bool = False, n_bits: int = 8,
@@ -430,42 +457,44 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, 
     ``fq`` (with ``fake_quant``) the values ``q * scale`` in the tensor dtype and, with a ``residual``, ``residual``:
     the sum ``x + residual`` in the tensor dtype, in a new tensor or in ``residual_out`` (which may be ``residual`` or
     ``x`` itself).  The normed value is quantized from fp32, without a rounding to the tensor dtype in between."""
-    _require_cuda(x, "x")
-    if x.dtype not in _DTYPE_CODE:
-        raise TypeError(f"unsupported dtype {x.dtype}")
-    lib = _lib.load()
-    lead, dev = x.shape[:-1], x.device
+    if not x.is_cuda:
+        _require_cuda(x, "x")
+    dtype, dev, shape = x.dtype, x.device, x.shape
+    code = _DTYPE_CODE.get(dtype)
+    if code is None:
+        raise TypeError(f"unsupported dtype {dtype}")
     x2, M, K, ldx = _as_rows(x)
     if weight.numel() != K:
         raise ValueError("weight must have K elements")
-    weight = weight.detach().reshape(-1).to(device=dev, dtype=x.dtype).contiguous()
+    if weight.dtype != dtype or weight.device != dev or not weight.is_contiguous():
+        weight = weight.detach().reshape(-1).to(device=dev, dtype=dtype).contiguous()
     res2 = h2 = h = None
     ldr = ldo = 0
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != dev:
+        if residual.shape != shape or residual.dtype != dtype or residual.device != dev:
             raise ValueError("residual must have the shape, dtype and device of x")
         res2, _, _, ldr = _as_rows(residual)
-        h = torch.empty((M, K), dtype=x.dtype, device=dev) if residual_out is None else residual_out
-        h2, hm, hk, ldo = _as_rows(h)
-        if residual_out is not None:
-            if h.dtype != x.dtype or h.device != dev or hm != M or hk != K or h2.data_ptr() != h.data_ptr():
+        if residual_out is None:
+            h = h2 = torch.empty(shape, dtype=dtype, device=dev)
+            ldo = K
+        else:
+            h = residual_out
+            h2, hm, hk, ldo = _as_rows(h)
+            if h.dtype != dtype or h.device != dev or hm != M or hk != K or h2.data_ptr() != h.data_ptr():
                 raise ValueError("residual_out must be rows of K contiguous elements with the shape, dtype and device of x")
     elif residual_out is not None:
         raise ValueError("residual_out without a residual")
-    q = torch.empty((M, K), dtype=torch.int8, device=dev) if codes else None
-    scale = torch.empty((M,), dtype=torch.float32, device=dev)
-    fq = torch.empty((M, K), dtype=x.dtype, device=dev) if fake_quant else None
-    nbytes = M * K * (x.element_size() * (1 + (2 if residual is not None else 0) + (1 if fake_quant else 0)) + (1 if codes else 0)) + 4 * M
-    with torch.cuda.device(dev), _Timed("rms_norm_quant", nbytes):
-        _lib.check(lib.samq_rms_norm_quant_i8(_ptr(x2), _ptr(res2), _ptr(weight), _DTYPE_CODE[x.dtype], M, K, ldx, ldr, float(eps),
-                                              int(n_bits), _ptr(h2), ldo, _ptr(q), _ptr(scale), _ptr(fq), _stream()))
-    out = {"scale": scale.view(lead)}
+    out = {"scale": torch.empty(shape[:-1], dtype=torch.float32, device=dev)}
+    q = fq = None
     if codes:
-        out["q"] = q.view(*lead, K)
+        out["q"] = q = torch.empty(shape, dtype=torch.int8, device=dev)
     if fake_quant:
-        out["fq"] = fq.view(*lead, K)
-    if residual is not None:
-        out["residual"] = h.view(x.shape) if residual_out is None else residual_out
+        out["fq"] = fq = torch.empty(shape, dtype=dtype, device=dev)
+    if h is not None:
+        out["residual"] = h
+    nbytes = M * K * (dtype.itemsize * (1 + (2 if h is not None else 0) + (1 if fake_quant else 0)) + (1 if codes else 0)) + 4 * M
+    _call(dev, "rms_norm_quant", nbytes, _lib.load().samq_rms_norm_quant_i8, x2.data_ptr(), _data_ptr(res2), weight.data_ptr(), code, M, K,
+          ldx, ldr, eps, n_bits, _data_ptr(h2), ldo, _data_ptr(q), out["scale"].data_ptr(), _data_ptr(fq))
     return out
 
 
@@ -505,7 +534,7 @@ class Fp4Tensor:
             raise TypeError("codes and scales must be uint8")
         if codes.dim() != 2 or codes.shape[0] != rows or codes.shape[1] < (K + 1) // 2 or codes.stride(1) != 1:
             raise ValueError(f"codes must be [{rows}, >= {(K + 1) // 2}] with contiguous rows")
-        if scales.device != codes.device or not scales.is_contiguous() or tuple(scales.shape) != fp4_scale_shape(fmt, rows, K):
+        if scales.device != codes.device or not scales.is_contiguous() or scales.shape != fp4_scale_shape(fmt, rows, K):
             raise ValueError(f"scales must be a contiguous {fp4_scale_shape(fmt, rows, K)} tensor on the device of codes")
         self.codes, self.scales, self.rows, self.K, self.fmt, self.global_scale = codes, scales, rows, K, fmt, float(global_scale)
 
@@ -532,31 +561,33 @@ def quantize_fp4(x: torch.Tensor, fmt: str = "nvfp4", global_scale: float = 1.0,
 
     Returns a dict with ``q``, an ``Fp4Tensor`` of the rows of ``x``, and with ``fake_quant`` ``fq``, the values it
     stands for in the dtype and shape of ``x``.  ``global_scale`` (nvfp4) is a power of two, see ``fp4_global_scale``."""
-    _require_cuda(x, "x")
-    if x.dtype not in _DTYPE_CODE:
-        raise TypeError(f"unsupported dtype {x.dtype}")
-    if fmt not in FP4_FORMATS:
-        raise ValueError(f"Invalid 4-bit format: {fmt}")
-    lib = _lib.load()
-    x2, M, K, ldx = _as_rows(x)
+    if not x.is_cuda:
+        _require_cuda(x, "x")
     dev = x.device
+    code = _DTYPE_CODE.get(x.dtype)
+    if code is None:
+        raise TypeError(f"unsupported dtype {x.dtype}")
+    fcode = FP4_FORMATS.get(fmt)
+    if fcode is None:
+        raise ValueError(f"Invalid 4-bit format: {fmt}")
+    x2, M, K, ldx = _as_rows(x)
     pitch = (K + 31) // 32 * 16
     codes = torch.empty((M, pitch), dtype=torch.uint8, device=dev)
     scales = torch.empty(fp4_scale_shape(fmt, M, K), dtype=torch.uint8, device=dev)
-    fq = torch.empty((M, K), dtype=x.dtype, device=dev) if fake_quant else None
-    nbytes = M * K * x.element_size() * (2 if fake_quant else 1) + codes.numel() + scales.numel()
-    with torch.cuda.device(dev), _Timed("quant_fp4", nbytes):
-        _lib.check(lib.samq_quant_fp4(_ptr(x2), _DTYPE_CODE[x.dtype], M, K, ldx, FP4_FORMATS[fmt], float(global_scale), _ptr(codes), pitch,
-                                      _ptr(scales), _ptr(fq), _stream()))
+    fq = torch.empty(x.shape, dtype=x.dtype, device=dev) if fake_quant else None
+    nbytes = M * K * x.dtype.itemsize * (2 if fake_quant else 1) + codes.numel() + scales.numel()
+    _call(dev, "quant_fp4", nbytes, _lib.load().samq_quant_fp4, x2.data_ptr(), code, M, K, ldx, fcode, global_scale, codes.data_ptr(), pitch,
+          scales.data_ptr(), _data_ptr(fq))
     out = {"q": Fp4Tensor(codes, scales, M, K, fmt, global_scale)}
     if fake_quant:
-        out["fq"] = fq.view(x.shape)
+        out["fq"] = fq
     return out
 
 
-def _linear_args(N: int, M: int, bias, residual, out_dtype, out, dev):
-    """Checked bias, residual rows and output of a linear layer's epilogue, as ``gemm_i8`` takes them."""
-    if out_dtype not in _DTYPE_CODE:
+def _linear_args(N: int, M: int, bias, residual, out_dtype, dev):
+    """Checked dtype code, bias and residual rows of a linear layer's epilogue, as ``gemm_i8`` takes them."""
+    code = _DTYPE_CODE.get(out_dtype)
+    if code is None:
         raise TypeError(f"unsupported out_dtype {out_dtype}")
     if bias is not None:
         bias = _bias_as(bias, out_dtype, dev)
@@ -571,27 +602,28 @@ def _linear_args(N: int, M: int, bias, residual, out_dtype, out, dev):
         residual, rm, rn, ldr = _as_rows(residual)
         if rm != M or rn != N:
             raise ValueError("residual must be [..., N] with the rows of the activation")
-    if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=dev)
-    elif out.dtype != out_dtype or out.device != dev or out.shape[-1] != N or out.numel() != M * N or not out.is_contiguous():
-        raise ValueError("out has the wrong dtype, device, shape or layout")
-    return bias, residual, ldr, out
+    return code, bias, residual, ldr
 
 
 def gemm_fp4(a: Fp4Tensor, w: Fp4Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
              activation: int = ACT_NONE, out_dtype: torch.dtype = torch.float16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``act(a @ w.T + bias) + residual`` -> [a.rows, w.rows] of ``out_dtype`` from two 4-bit operands of one format, on
     the tensor cores' block-scaled kinds (``samq_gemm_fp4``)."""
-    _require_cuda(a.codes, "a")
-    if a.fmt != w.fmt or a.K != w.K or a.device != w.device:
+    ac, wc = a.codes, w.codes
+    dev = ac.device
+    if not ac.is_cuda:
+        _require_cuda(ac, "a")
+    if a.fmt != w.fmt or a.K != w.K or dev != wc.device:
         raise ValueError(f"operands must share format, K and device: {a.fmt} [{a.rows}, {a.K}] and {w.fmt} [{w.rows}, {w.K}]")
-    lib = _lib.load()
-    M, N, K, dev = a.rows, w.rows, a.K, a.device
-    bias, residual, ldr, out = _linear_args(N, M, bias, residual, out_dtype, out, dev)
-    with torch.cuda.device(dev), _Timed("gemm_fp4", 2.0 * M * N * K):
-        _lib.check(lib.samq_gemm_fp4(_ptr(a.codes), a.codes.stride(0), _ptr(a.scales), _ptr(w.codes), w.codes.stride(0), _ptr(w.scales),
-                                     M, N, K, FP4_FORMATS[a.fmt], a.global_scale * w.global_scale, _ptr(bias), _ptr(residual), ldr,
-                                     activation, _ptr(out), _DTYPE_CODE[out_dtype], N, _ptr(status_word(dev)), _stream()))
+    M, N, K = a.rows, w.rows, a.K
+    code, bias, residual, ldr = _linear_args(N, M, bias, residual, out_dtype, dev)
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype, device=dev)
+    elif out.dtype != out_dtype or out.device != dev or out.shape[-1] != N or out.numel() != M * N or not out.is_contiguous():
+        raise ValueError("out has the wrong dtype, device, shape or layout")
+    _call(dev, "gemm_fp4", 2.0 * M * N * K, _lib.load().samq_gemm_fp4, ac.data_ptr(), ac.stride(0), a.scales.data_ptr(), wc.data_ptr(),
+          wc.stride(0), w.scales.data_ptr(), M, N, K, FP4_FORMATS[a.fmt], a.global_scale * w.global_scale, _data_ptr(bias),
+          _data_ptr(residual), ldr, activation, out.data_ptr(), code, N, _status_ptr(dev))
     return out
 
 
@@ -601,8 +633,22 @@ def linear_fp4(x: torch.Tensor, w: Fp4Tensor, bias: Optional[torch.Tensor] = Non
     ``act(q(x) @ w.T + bias) + residual`` -> [..., N], of ``x.dtype`` unless ``out_dtype`` says otherwise."""
     if x.shape[-1] != w.K:
         raise ValueError(f"x must be [..., {w.K}]")
+    if not x.is_cuda:
+        _require_cuda(x, "x")
+    N, K, dev = w.rows, w.K, x.device
+    if x.numel() <= _lib.LINEAR_FP4_MAX_ROWS * K and (out_dtype is None or out_dtype == x.dtype):
+        # a few rows: one kernel quantizes and multiplies
+        if dev != w.codes.device:
+            raise ValueError("x must be on the device of w")
+        x2, M, _, ldx = _as_rows(x)
+        code, bias, residual, ldr = _linear_args(N, M, bias, residual, x.dtype, dev)
+        out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
+        _call(dev, "linear_fp4", 2.0 * M * N * K, _lib.load().samq_linear_fp4, x2.data_ptr(), code, ldx, w.codes.data_ptr(), w.codes.stride(0),
+              w.scales.data_ptr(), M, N, K, FP4_FORMATS[w.fmt], w.global_scale, _data_ptr(bias), _data_ptr(residual), ldr, activation,
+              out.data_ptr(), N, _status_ptr(dev))
+        return out
     y = gemm_fp4(quantize_fp4(x, w.fmt)["q"], w, bias=bias, residual=residual, activation=activation, out_dtype=out_dtype or x.dtype)
-    return y.view(*x.shape[:-1], w.rows)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
 
 def gemm_stall_selftest(a_q: torch.Tensor, w_q: torch.Tensor, skip_kblock: int = 0, wait_limit_cycles: int = 2_000_000) -> torch.Tensor:

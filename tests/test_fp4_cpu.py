@@ -76,7 +76,9 @@ def _calls(lib):
                 stream=None)
     gemm = dict(A=one, lda=32, sa=one, W=one, ldw=32, sw=one, M=4, N=8, K=64, fmt=_lib.FP4_NV, alpha=1.0, bias=None, res=None, ldr=0,
                 act=0, out=one, odt=_lib.F16, ldo=8, status=None, stream=None)
-    return {"quant": (lib.samq_quant_fp4, quant), "norm": (lib.samq_rms_norm_quant_i8, norm), "gemm": (lib.samq_gemm_fp4, gemm)}
+    lin = dict(x=one, dtype=_lib.F16, ldx=64, W=one, ldw=32, sw=one, M=4, N=8, K=64, fmt=_lib.FP4_NV, alpha=1.0, bias=None, res=None, ldr=0,
+               act=0, out=one, ldo=8, status=None, stream=None)
+    return {"linear": (lib.samq_linear_fp4, lin), "quant": (lib.samq_quant_fp4, quant), "norm": (lib.samq_rms_norm_quant_i8, norm), "gemm": (lib.samq_gemm_fp4, gemm)}
 
 
 @pytest.mark.parametrize("name,change,code", [
@@ -91,6 +93,8 @@ def _calls(lib):
     ("gemm", {"A": None}, -1), ("gemm", {"sw": None}, -1), ("gemm", {"out": None}, -1), ("gemm", {"N": 0}, -1), ("gemm", {"K": -1}, -1),
     ("gemm", {"fmt": 5}, -1), ("gemm", {"act": 4}, -1), ("gemm", {"odt": _lib.I32}, -1), ("gemm", {"lda": 16}, -1), ("gemm", {"ldo": 7}, -1),
     ("gemm", {"res": 1 << 20, "ldr": 7}, -1), ("gemm", {"lda": 40}, -3), ("gemm", {"W": (1 << 20) + 8}, -3), ("gemm", {"sa": (1 << 20) + 4}, -3),
+    ("linear", {"x": None}, -1), ("linear", {"M": 33}, -6), ("linear", {"ldx": 63}, -1), ("linear", {"x": (1 << 20) + 1}, -3), ("linear", {"W": None}, -1),
+    ("linear", {"sw": (1 << 20) + 8}, -3), ("linear", {"dtype": _lib.I32}, -1), ("linear", {"K": 0}, -1), ("linear", {"fmt": -1}, -1),
     ("gemm", {"out": (1 << 20) + 1}, -3), ("gemm", {"M": 1 << 31}, -6),
 ])
 def test_entry_points_refuse_bad_arguments(name, change, code):

@@ -118,7 +118,7 @@ def _exact_operand(rows, K, fmt, dev, seed):
 
 
 SHAPES = [(1, 1, 1), (1, 8, 64), (3, 130, 31), (1, 5120, 1280), (128, 128, 256), (129, 257, 300), (200, 40, 1283), (64, 1001, 512), (16, 300, 2048),
-          (17, 65, 96), (40, 200, 4100), (260, 520, 768), (1000, 384, 200), (300, 1280, 5120), (2600, 1300, 600), (8200, 257, 1283), (290, 8210, 300), (4096, 2304, 768)]
+          (17, 65, 96), (40, 200, 4100), (260, 520, 768), (1000, 384, 200), (300, 1280, 5120), (1, 20000, 300), (200, 7000, 256), (24, 2304, 768), (2600, 1300, 600), (8200, 257, 1283), (290, 8210, 300), (4096, 2304, 768)]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -183,7 +183,45 @@ def test_product_of_quantized_data(cuda_device, fmt, M, N, K):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("M", [1, 200, 9000])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 640, 1280), (3, 131, 33), (8, 300, 5120), (9, 1000, 300), (17, 200, 1283), (32, 257, 2048)])
+def test_one_kernel_layer_equals_its_two_halves(cuda_device, fmt, dtype, M, N, K):
+    """linear_fp4 of at most 32 rows quantizes inside the product.  Exactly representable data: the layer's output is the
+    quantizer's values times the weight, exactly, in any order of summation."""
+    rng = np.random.default_rng(M + N + K)
+    w, wv = _exact_operand(N, K, fmt, cuda_device, 7)
+    # code values under block scales 2^-1 and 2^0, each block with a 6 so that quantization gives the values back
+    b = F.BLOCK[fmt]
+    nb = -(-K // b)
+    v = F.code_value(rng.integers(0, 16, (M, nb, b)))
+    v[:, :, 0] = 6.0
+    xv = (v * rng.choice([0.5, 1.0], (M, nb, 1))).reshape(M, nb * b)[:, :K]
+    x = torch.from_numpy(xv).to(dtype).to(cuda_device)
+    g = torch.Generator().manual_seed(5)
+    bias, res = torch.randn(N, generator=g).to(dtype), torch.randn(M, N, generator=g).to(dtype)
+    y = ops.linear_fp4(x, w, bias=bias.to(cuda_device), residual=res.to(cuda_device))
+    ops.check_status()
+    z = xv @ wv.T + bias.double().numpy()
+    u = 2.0 ** -24
+    tol = u * np.abs(z)
+    z = z + res.double().numpy()
+    tol = tol + u * np.abs(z)
+    tol = tol + HALF[dtype] * (np.abs(z) + tol)
+    finite = np.abs(z) < (60000 if dtype == torch.float16 else 1e30)
+    assert np.all(np.abs(y.double().cpu().numpy() - z)[finite] <= tol[finite])
+    # a pitch, an offset that no vector may start at, and a leading shape
+    wide = torch.randn(M, K + 5, device=cuda_device).to(dtype)
+    wide[:, 3:K + 3] = x
+    assert _same_bytes(ops.linear_fp4(wide[:, 3:K + 3], w, bias=bias.to(cuda_device), residual=res.to(cuda_device)), y)
+    assert ops.linear_fp4(x.view(M, 1, K), w).shape == (M, 1, N)
+
+
+def _same_bytes(a, b):
+    return torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M", [1, 33, 200, 9000])
 def test_rows_that_are_not_finite_stay_apart(cuda_device, fmt, M):
     x = _values(M, 300, torch.float16)
     x[M // 2, 299] = float("nan")
