@@ -12,6 +12,7 @@
 #pragma once
 
 #include "common.cuh"
+#include <type_traits>
 
 namespace samq {
 namespace fp4 {
@@ -44,11 +45,100 @@ __device__ __forceinline__ uint32_t pack_e2m1x8(const float* v) {
         : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
     return r;
 }
-// the magnitude bits and sign of a 4-bit code as the float it stands for
-__device__ __forceinline__ float e2m1_value(uint32_t code) {
-    // 0, .5, 1, 1.5, 2, 3, 4, 6 : doubled they are the integers of this table, four bits each
-    const float mag = 0.5f * (float)((0xC8643210u >> (4 * (code & 7u))) & 15u);
-    return (code & 8u) ? -mag : mag;
+// the eight values of eight codes
+__device__ __forceinline__ void unpack_e2m1x8(uint32_t codes, float2 (&v)[4]) {
+    uint32_t h[4];
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(codes));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+}
+
+// Sixteen columns of a row as the threads hold them: packed pairs of a 16-bit type, or fp32.
+template <typename T> struct Chunk {
+    uint32_t w[8];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ void set(int i, T v) {
+        const uint32_t b = *reinterpret_cast<const uint16_t*>(&v);
+        w[i >> 1] = (i & 1) ? (w[i >> 1] & 0xFFFFu) | (b << 16) : b;
+    }
+    __device__ __forceinline__ float2 pair(int i) const {
+        if constexpr (sizeof(T) == 2) {
+            if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            else return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+        }
+    }
+    // the largest |x| as fp32 bits; a NaN or an infinity counts as larger than every number
+    __device__ __forceinline__ uint32_t amax_bits() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+        m = max(m & 0xFFFFu, m >> 16);
+        if constexpr (std::is_same<T, __half>::value) {
+            const uint16_t h = (uint16_t)m;
+            return __float_as_uint(__half2float(*reinterpret_cast<const __half*>(&h)));
+        } else {
+            return m << 16;
+        }
+    }
+};
+template <> struct Chunk<float> {
+    float f[16];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f[i] = 0.0f;
+    }
+    __device__ __forceinline__ void set(int i, float v) { f[i] = v; }
+    __device__ __forceinline__ float2 pair(int i) const { return make_float2(f[2 * i], f[2 * i + 1]); }
+    __device__ __forceinline__ uint32_t amax_bits() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(f[i]) & 0x7FFFFFFFu);
+        return m;
+    }
+};
+
+// 32 bytes in one access (the address on 32 bytes)
+__device__ __forceinline__ void load32(const void* p, uint32_t* w) {
+    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
+}
+__device__ __forceinline__ void store32(void* p, const uint32_t* w) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+
+// how a row's chunks may be accessed: by 32 bytes, by 16, or element by element
+enum Access { BY_ELEMENT = 0, BY_16 = 1, BY_32 = 2 };
+inline int row_access(const void* base, int64_t ld_bytes) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(base) | (uintptr_t)ld_bytes;
+    return (a & 31) == 0 ? BY_32 : (a & 15) == 0 ? BY_16 : BY_ELEMENT;
+}
+
+// `n` (1 to 16) columns at x, zeros behind them
+template <typename T>
+__device__ __forceinline__ void load_chunk(Chunk<T>& c, const T* x, int n, int access) {
+    constexpr int WORDS = 16 * (int)sizeof(T) / 4;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&c);
+    if (n >= 16 && access == BY_32) {
+#pragma unroll
+        for (int i = 0; i < WORDS; i += 8) load32(reinterpret_cast<const uint32_t*>(x) + i, w + i);
+    } else if (n >= 16 && access == BY_16) {
+#pragma unroll
+        for (int i = 0; i < WORDS; i += 4) *reinterpret_cast<uint4*>(w + i) = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(x) + i);
+    } else {
+        c.zero();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) if (i < n) c.set(i, x[i]);
+    }
 }
 
 // Scale of a block from its largest magnitude, given as the bits of |x| (compared as integers, so that a NaN
@@ -57,7 +147,7 @@ __device__ __forceinline__ float e2m1_value(uint32_t code) {
 struct Scale { uint32_t byte; float value; };
 
 template <int FMT>
-__device__ __forceinline__ Scale block_scale(uint32_t amax_bits, float global_scale) {
+__device__ __forceinline__ Scale block_scale(uint32_t amax_bits, float global_scale, float inv_global_scale) {
     Scale s;
     const bool finite = amax_bits < 0x7F800000u;
     if constexpr (FMT == SAMQ_FP4_MX) {
@@ -68,36 +158,59 @@ __device__ __forceinline__ Scale block_scale(uint32_t amax_bits, float global_sc
         s.value = __uint_as_float(s.byte > 0 ? s.byte << 23 : 0x00400000u);
     } else {
         // amax / (6 g) to e4m3, at most 448, and at least its smallest value 2^-9 (the block's own values are
-        // then still resolved below the point where the scale alone would round to zero).  6 g has few
+        // then still resolved below the point where the scale alone would round to zero).  6 has few
         // significant bits, so the correctly rounded quotient never reaches a tie that amax itself missed.
-        const float q = __fdiv_rn(__uint_as_float(amax_bits), 6.0f * global_scale);
+        // g is a power of two: amax / g is exact, and a sixth of it is one correctly rounded quotient by a constant
+        const float a = __uint_as_float(amax_bits) * inv_global_scale;
+        const float sixth = 1.0f / 6.0f;
+        const float q0 = a * sixth;
+        const float q = fmaf(fmaf(-q0, 6.0f, a), sixth, q0);
         uint16_t two;
         asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(0.0f), "f"(q));
         s.byte = finite ? max((uint32_t)two & 0x7Fu, 1u) : 0x7Fu;
-        const uint32_t e = s.byte >> 3, m = s.byte & 7u;
-        const float v = e ? __uint_as_float(((e + 120u) << 23) | (m << 20)) : (float)m * 0x1p-9f;
-        s.value = finite ? v * global_scale : __uint_as_float(0x7FC00000u);
+        uint32_t h;
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)s.byte));
+        s.value = __low2float(*reinterpret_cast<const __half2*>(&h)) * global_scale;
     }
     if (!finite) s.value = __uint_as_float(0x7FC00000u);
     return s;
 }
 
-// x / scale for a finite block.  mxfp4: a product with the exact reciprocal.  nvfp4: the correctly rounded
-// quotient (a scale has four significant bits and a border between codes three, so a quotient that rounds to a
-// border lies on it).
+// x / scale for a finite block, two values at a time.  mxfp4: a product with the exact reciprocal.  nvfp4: Markstein's
+// correction of an approximate quotient, y = y0 + (x - y0 s) / s: exact where x / s is a number of few bits, so on every
+// border between codes, and a correct rounding elsewhere up to 2^-45; a scale has four significant bits and a border
+// three, so a value beside a border stays beside it.  The correction loses the sign of -0, which is put back.
 template <int FMT>
 struct ToCode {
-    Divider d;
-    float inv;
+    float2 s2, inv2;
     __device__ __forceinline__ explicit ToCode(const Scale& s) {
+        float inv;
         if constexpr (FMT == SAMQ_FP4_MX) inv = __uint_as_float((254u - s.byte) << 23);
-        else d = make_divider(s.value);
+        else asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s.value));
+        inv2 = make_float2(inv, inv);
+        s2 = make_float2(-s.value, -s.value);
     }
-    __device__ __forceinline__ float operator()(float x) const {
-        if constexpr (FMT == SAMQ_FP4_MX) return x * inv;
-        else return copysignf(div_exact(x, d), x);        // the correction step loses the sign of -0
+    __device__ __forceinline__ float2 operator()(float2 x) const {
+        if constexpr (FMT == SAMQ_FP4_MX) return __fmul2_rn(x, inv2);
+        const float2 y0 = __fmul2_rn(x, inv2);
+        const float2 y = __ffma2_rn(__ffma2_rn(y0, s2, x), inv2, y0);
+        return make_float2(copysignf(y.x, x.x), copysignf(y.y, x.y));
     }
 };
+
+// The codes of a chunk under its block's scale, eight a word; zero where the block is not finite.
+template <int FMT, typename T>
+__device__ __forceinline__ uint2 encode_chunk(const Chunk<T>& c, const Scale& s, bool finite) {
+    const ToCode<FMT> to_code(s);
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float2 y = to_code(c.pair(i));
+        v[2 * i] = y.x; v[2 * i + 1] = y.y;
+    }
+    const uint2 q = make_uint2(pack_e2m1x8(v), pack_e2m1x8(v + 8));
+    return finite ? q : make_uint2(0u, 0u);
+}
 
 }  // namespace fp4
 }  // namespace samq

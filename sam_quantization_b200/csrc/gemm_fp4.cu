@@ -43,7 +43,7 @@ struct SmallParams {
     int groups;
     const uint8_t* a_scales;                      // unless the kernel quantizes
     const uint8_t* w_scales;
-    const void* x; int64_t ldx; int vec_x;        // the activation, if the kernel quantizes it
+    const void* x; int64_t ldx; int access_x;     // the activation, if the kernel quantizes it
     int tmem_cols;
     float alpha;
     const void* bias;
@@ -76,25 +76,6 @@ __device__ __forceinline__ float ld_cluster(uint32_t cluster_addr) {
     float v;
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
     return v;
-}
-
-// 16 columns of row `row` of the activation as fp32, zeros outside
-template <typename T>
-__device__ __forceinline__ void load_chunk(const SmallParams& p, int row, int col, float (&f)[16]) {
-    const T* x = static_cast<const T*>(p.x) + (int64_t)row * p.ldx + col;
-    if (row < p.M && p.vec_x && col + 16 <= p.K) {
-        constexpr int E = Elem<T>::kPerVec;
-#pragma unroll
-        for (int v = 0; v < 16 / E; ++v) {
-            T t[E];
-            *reinterpret_cast<uint4*>(t) = __ldg(reinterpret_cast<const uint4*>(x) + v);
-#pragma unroll
-            for (int e = 0; e < E; ++e) f[v * E + e] = Elem<T>::up(t[e]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] = (row < p.M && col + i < p.K) ? Elem<T>::up(x[i]) : 0.0f;
-    }
 }
 
 // QUANT: the activation is `x` of type OutT, quantized here; otherwise codes and scales are loaded.
@@ -207,18 +188,12 @@ gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                 uint8_t* scales = sf + (size_t)s * 2 * S::SF_BYTES + S::SF_BYTES;
                 for (int c = tid; c < p.T * CHUNKS; c += EPI_THREADS) {
                     const int r = c / CHUNKS, j = c % CHUNKS, col = kb * KPAD + j * 16;
-                    float f[16];
-                    load_chunk<OutT>(p, m0 + r, col, f);
-                    uint32_t amax = 0;
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) amax = max(amax, __float_as_uint(f[e]) & 0x7FFFFFFFu);
+                    Chunk<OutT> x;
+                    load_chunk(x, static_cast<const OutT*>(p.x) + (int64_t)(m0 + r) * p.ldx + col, m0 + r < p.M ? min(16, p.K - col) : 0, p.access_x);
+                    uint32_t amax = x.amax_bits();
                     if constexpr (FMT == SAMQ_FP4_MX) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                    const Scale sc = block_scale<FMT>(amax, 1.0f);
-                    const ToCode<FMT> to_code(sc);
-                    const bool finite = amax < 0x7F800000u;
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) f[e] = finite ? to_code(f[e]) : 0.0f;
-                    *reinterpret_cast<uint2*>(codes + staged(r, j * 8)) = make_uint2(pack_e2m1x8(f), pack_e2m1x8(f + 8));
+                    const Scale sc = block_scale<FMT>(amax, 1.0f, 1.0f);
+                    *reinterpret_cast<uint2*>(codes + staged(r, j * 8)) = encode_chunk<FMT>(x, sc, amax < 0x7F800000u);
                     const int block = j * 16 / block_of(FMT);
                     if (FMT == SAMQ_FP4_NV || (j & 1) == 0)
                         scales[(block / 4) * TILE_BYTES + r * 16 + (block & 3)] = (uint8_t)(kb * KPAD + block * block_of(FMT) < p.K ? sc.byte : 0u);
@@ -314,7 +289,7 @@ int gemm_fp4_small(const Fp4Call& c, const void* x, int64_t ldx) {
     p.T = c.M >= MAX_T ? MAX_T : (int)((c.M + 7) / 8 * 8);
     p.groups = (int)groups_of(c.fmt, c.K); p.a_scales = c.a_scales; p.w_scales = c.w_scales;
     const size_t esz = c.out_dtype == SAMQ_F32 ? 4 : 2;
-    p.x = x; p.ldx = ldx; p.vec_x = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * esz) % 16 == 0;
+    p.x = x; p.ldx = ldx; p.access_x = row_access(x, ldx * (int64_t)esz);
     p.alpha = c.epi.alpha; p.bias = c.epi.bias; p.residual = c.epi.residual; p.ldr = c.epi.ldr; p.out = c.epi.out; p.ldo = c.epi.ldo;
     p.gelu = c.gelu; p.status = c.status;
     CUtensorMap ma, mw;

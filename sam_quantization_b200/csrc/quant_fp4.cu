@@ -18,30 +18,25 @@ constexpr int WARPS = 8;
 struct QuantFp4Params {
     const void* x; int64_t ldx;
     int64_t M; int64_t K;
-    float global_scale;
+    float global_scale, inv_global_scale;
     uint8_t* codes; int64_t ldq;
     uint8_t* scales; int64_t groups;
     void* fq;
     int col_blocks;
-    int vec_x, vec_q, vec_fq;                    // rows start on 16 (8 for the codes) bytes: vectors may be used
+    int access_x, access_fq;                     // see Access
+    int vec_q;                                   // rows of codes start on 8 bytes
 };
-
-template <typename T>
-__device__ __forceinline__ void load_chunk(const T* p, float (&f)[CHUNK]) {
-    constexpr int E = Elem<T>::kPerVec;
-#pragma unroll
-    for (int v = 0; v < CHUNK / E; ++v) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + v);
-        T t[E];
-        *reinterpret_cast<uint4*>(t) = u;
-#pragma unroll
-        for (int e = 0; e < E; ++e) f[v * E + e] = Elem<T>::up(t[e]);
-    }
-}
 
 // A warp takes the rows that share 32 (nvfp4) or 16 (mxfp4) bytes of a scale tile, so that its scales leave as
 // whole pieces: nvfp4 8 rows (r, r + 1, each + 0, 32, 64, 96) x 4 chunks, mxfp4 4 rows (r + 0, 32, 64, 96) x 8 chunks.
-template <typename T, int FMT, bool FQ>
+template <int FMT>
+__device__ __forceinline__ int unit_row(int unit, int sub) {
+    return FMT == SAMQ_FP4_MX ? unit + 32 * sub : 2 * unit + (sub >> 2) + 32 * (sub & 3);
+}
+constexpr int STAGED_PITCH = CHUNK + 1;
+
+// STAGED: rows of x or fq that do not start on 16 bytes pass through shared memory
+template <typename T, int FMT, bool FQ, bool STAGED>
 __global__ void __launch_bounds__(WARPS * 32)
 quant_fp4_kernel(const QuantFp4Params p)
 {
@@ -54,32 +49,41 @@ quant_fp4_kernel(const QuantFp4Params p)
     constexpr int UNITS = 128 / ROWS;                              // row units of a tile
     const int64_t tile = row_unit / UNITS;
     const int sub = lane / LANES;
-    const int r = FMT == SAMQ_FP4_MX ? (int)(row_unit % UNITS) + 32 * sub
-                                     : 2 * (int)(row_unit % UNITS) + (sub >> 2) + 32 * (sub & 3);
+    const int r = unit_row<FMT>((int)(row_unit % UNITS), sub);
     const int64_t row = tile * TILE_ROWS + r;
     const int64_t col = (group * LANES + lane % LANES) * CHUNK;
     const bool row_ok = row < p.M;
 
-    float f[CHUNK];
-    const T* x = static_cast<const T*>(p.x) + row * p.ldx + col;
-    const bool whole = col + CHUNK <= p.K;
-    if (row_ok && whole && p.vec_x) {
-        load_chunk<T>(x, f);
+    const int left = row_ok ? (int)min((int64_t)CHUNK, p.K - col) : 0;          // columns of the chunk (0 or less: none)
+    Chunk<T> x;
+    __shared__ T staged[STAGED ? WARPS * 32 * STAGED_PITCH : 1];
+    T* const mine = staged + (STAGED ? warp * 32 * STAGED_PITCH : 0);
+    constexpr int SPAN = LANES * CHUNK;                            // columns of a row in the warp
+    const int64_t first_col = group * SPAN;
+    if constexpr (STAGED) {
+        // rows that no vector may start at: the warp reads 32 neighbouring elements an instruction and turns them into
+        // its lanes' chunks in shared memory
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            const int64_t rr = tile * TILE_ROWS + unit_row<FMT>((int)(row_unit % UNITS), i);
+#pragma unroll
+            for (int j = 0; j < SPAN; j += 32) {
+                const int c = j + lane;
+                const bool in = rr < p.M && first_col + c < p.K;
+                mine[(i * LANES + c / CHUNK) * STAGED_PITCH + c % CHUNK] = in ? static_cast<const T*>(p.x)[rr * p.ldx + first_col + c] : Elem<T>::down(0.0f);
+            }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < CHUNK; ++i) x.set(i, mine[lane * STAGED_PITCH + i]);
+        __syncwarp();
     } else {
-#pragma unroll
-        for (int i = 0; i < CHUNK; ++i) f[i] = (row_ok && col + i < p.K) ? Elem<T>::up(x[i]) : 0.0f;
+        load_chunk(x, static_cast<const T*>(p.x) + row * p.ldx + col, left, p.access_x);
     }
-    uint32_t amax = 0;
-#pragma unroll
-    for (int i = 0; i < CHUNK; ++i) amax = max(amax, __float_as_uint(f[i]) & 0x7FFFFFFFu);
+    uint32_t amax = x.amax_bits();
     if constexpr (FMT == SAMQ_FP4_MX) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    const Scale s = block_scale<FMT>(amax, p.global_scale);
-    const ToCode<FMT> to_code(s);
-    const bool finite = amax < 0x7F800000u;
-    float v[CHUNK];
-#pragma unroll
-    for (int i = 0; i < CHUNK; ++i) v[i] = finite ? to_code(f[i]) : 0.0f;
-    const uint2 q = make_uint2(pack_e2m1x8(v), pack_e2m1x8(v + 8));
+    const Scale s = block_scale<FMT>(amax, p.global_scale, p.inv_global_scale);
+    const uint2 q = encode_chunk<FMT>(x, s, amax < 0x7F800000u);
 
     // the word of four scales is put together by the group's first lane; blocks behind K and rows behind M are zero
     const int64_t block_col = col / block_of(FMT) * block_of(FMT);
@@ -90,10 +94,10 @@ quant_fp4_kernel(const QuantFp4Params p)
     for (int o = STEP; o < LANES; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
     if (lane % LANES == 0)
         *reinterpret_cast<uint32_t*>(p.scales + (tile * p.groups + group) * TILE_BYTES + (r & 31) * 16 + (r >> 5) * 4) = word;
-    if (!row_ok) return;
+    if constexpr (!STAGED) { if (!row_ok) return; }
 
     const int64_t cbyte = col / 2;
-    if (cbyte < p.ldq) {
+    if (row_ok && cbyte < p.ldq) {
         uint8_t* o = p.codes + row * p.ldq + cbyte;
         if (p.vec_q && cbyte + 8 <= p.ldq) {
             *reinterpret_cast<uint2*>(o) = q;
@@ -103,20 +107,47 @@ quant_fp4_kernel(const QuantFp4Params p)
         }
     }
     if constexpr (FQ) {
+        if constexpr (!STAGED) { if (left <= 0) return; }
         T* o = static_cast<T*>(p.fq) + row * p.K + col;
         T t[CHUNK];
+        const float2 s2 = make_float2(s.value, s.value);
 #pragma unroll
-        for (int i = 0; i < CHUNK; ++i) {
-            const uint32_t c = ((i < 8 ? q.x : q.y) >> (4 * (i & 7))) & 15u;
-            t[i] = Elem<T>::down(e2m1_value(c) * s.value);
+        for (int h = 0; h < 2; ++h) {
+            float2 v[4];
+            unpack_e2m1x8(h ? q.y : q.x, v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 y = __fmul2_rn(v[i], s2);
+                if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<__half2*>(t + 8 * h + 2 * i) = __floats2half2_rn(y.x, y.y);
+                else if constexpr (std::is_same<T, __nv_bfloat16>::value) *reinterpret_cast<__nv_bfloat162*>(t + 8 * h + 2 * i) = __floats2bfloat162_rn(y.x, y.y);
+                else { t[8 * h + 2 * i] = y.x; t[8 * h + 2 * i + 1] = y.y; }
+            }
         }
-        if (whole && p.vec_fq) {
-            constexpr int E = Elem<T>::kPerVec;
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(t);
+        constexpr int WORDS = CHUNK * (int)sizeof(T) / 4;
+        if constexpr (STAGED) {
 #pragma unroll
-            for (int k = 0; k < CHUNK / E; ++k) reinterpret_cast<uint4*>(o)[k] = *reinterpret_cast<const uint4*>(t + k * E);
+            for (int i = 0; i < CHUNK; ++i) mine[lane * STAGED_PITCH + i] = t[i];
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) {
+                const int64_t rr = tile * TILE_ROWS + unit_row<FMT>((int)(row_unit % UNITS), i);
+#pragma unroll
+                for (int j = 0; j < SPAN; j += 32) {
+                    const int c = j + lane;
+                    if (rr < p.M && first_col + c < p.K)
+                        static_cast<T*>(p.fq)[rr * p.K + first_col + c] = mine[(i * LANES + c / CHUNK) * STAGED_PITCH + c % CHUNK];
+                }
+            }
+        } else if (left >= CHUNK && p.access_fq == BY_32) {
+#pragma unroll
+            for (int i = 0; i < WORDS; i += 8) store32(reinterpret_cast<uint32_t*>(o) + i, w + i);
+        } else if (left >= CHUNK && p.access_fq == BY_16) {
+#pragma unroll
+            for (int i = 0; i < WORDS; i += 4) *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(o) + i) = *reinterpret_cast<const uint4*>(w + i);
         } else {
 #pragma unroll
-            for (int i = 0; i < CHUNK; ++i) if (col + i < p.K) o[i] = t[i];
+            for (int i = 0; i < CHUNK; ++i) if (i < left) o[i] = t[i];
         }
     }
 }
@@ -127,8 +158,15 @@ int launch_quant_fp4(const QuantFp4Params& p, cudaStream_t st) {
     const int64_t units = (p.M + TILE_ROWS - 1) / TILE_ROWS * (TILE_ROWS / ROWS);
     const int64_t blocks = units * p.col_blocks;
     if (blocks > 2147483647LL) return fail(SAMQ_ERR_TOO_LARGE, "quantization to 4 bits: %lld x %lld is too large", (long long)p.M, (long long)p.K);
-    if (p.fq != nullptr) quant_fp4_kernel<T, FMT, true><<<(unsigned)blocks, WARPS * 32, 0, st>>>(p);
-    else quant_fp4_kernel<T, FMT, false><<<(unsigned)blocks, WARPS * 32, 0, st>>>(p);
+    const bool staged = p.access_x == BY_ELEMENT || (p.fq != nullptr && p.access_fq == BY_ELEMENT);
+    const unsigned grid = (unsigned)blocks;
+    if (p.fq != nullptr) {
+        if (staged) quant_fp4_kernel<T, FMT, true, true><<<grid, WARPS * 32, 0, st>>>(p);
+        else quant_fp4_kernel<T, FMT, true, false><<<grid, WARPS * 32, 0, st>>>(p);
+    } else {
+        if (staged) quant_fp4_kernel<T, FMT, false, true><<<grid, WARPS * 32, 0, st>>>(p);
+        else quant_fp4_kernel<T, FMT, false, false><<<grid, WARPS * 32, 0, st>>>(p);
+    }
     SAMQ_CUDA_TRY(cudaGetLastError());
     return SAMQ_OK;
 }
@@ -157,12 +195,12 @@ int quant_fp4_dispatch(const void* x, int dtype, int64_t M, int64_t K, int64_t l
     const size_t esz = dtype == SAMQ_F32 ? 4 : 2;
     if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(fq)) & (esz - 1)) return fail(SAMQ_ERR_ALIGNMENT, "x and fq_out must be aligned to their elements");
     QuantFp4Params p;
-    p.x = x; p.ldx = ldx; p.M = M; p.K = K; p.global_scale = global_scale;
+    p.x = x; p.ldx = ldx; p.M = M; p.K = K; p.global_scale = global_scale; p.inv_global_scale = 1.0f / global_scale;
     p.codes = codes; p.ldq = ldq; p.scales = scales; p.groups = fp4::groups_of(fmt, K); p.fq = fq;
     p.col_blocks = (int)((p.groups + WARPS - 1) / WARPS);
-    p.vec_x = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * esz) % 16 == 0;
+    p.access_x = row_access(x, ldx * (int64_t)esz);
+    p.access_fq = row_access(fq, K * (int64_t)esz);
     p.vec_q = (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && ldq % 8 == 0;
-    p.vec_fq = (reinterpret_cast<uintptr_t>(fq) & 15) == 0 && (K * esz) % 16 == 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (dtype) {
     case SAMQ_F16:  return launch_quant_fp4<__half>(fmt, p, st);

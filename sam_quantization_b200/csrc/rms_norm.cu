@@ -8,6 +8,7 @@
 // One pass: a row stays in registers between the two reductions (sum of squares, largest magnitude).  Bound: HBM,
 // 2 + 2 + 2 + 1 bytes an element of a 16-bit type (x, residual, h, q), 2 more for the dequantized values.
 #include "common.cuh"
+#include <type_traits>
 
 namespace samq {
 
@@ -24,79 +25,102 @@ struct RmsNormParams {
     int vec;                                       // every row of every tensor starts on 16 bytes and K fills vectors
 };
 
-// sum and integer maximum over the `warps` warps that share a row
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-__device__ __forceinline__ uint32_t warp_umax(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+// the larger of a and |b|; a NaN wins
+__device__ __forceinline__ float max_abs_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+    return r;
+}
 
-template <typename T, int E>
-__device__ __forceinline__ void load_vec(const T* p, float (&f)[E]) {
-    if constexpr (E == 1) {
-        f[0] = Elem<T>::up(*p);
-    } else {
-        T t[E];
-        *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(p);
+// E elements of a row as fp32 pairs (E = 1: the second of the pair is 0)
+template <typename T, int E> struct Vec {
+    static constexpr int P = E == 1 ? 1 : E / 2;
+    float2 v[P];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (E == 1) {
+            v[0] = make_float2(Elem<T>::up(*p), 0.0f);
+        } else {
+            T t[E];
+            *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(p);
 #pragma unroll
-        for (int e = 0; e < E; ++e) f[e] = Elem<T>::up(t[e]);
+            for (int i = 0; i < P; ++i) v[i] = make_float2(Elem<T>::up(t[2 * i]), Elem<T>::up(t[2 * i + 1]));
+        }
     }
-}
-template <typename T, int E>
-__device__ __forceinline__ void store_vec(T* p, const float (&f)[E]) {
-    if constexpr (E == 1) {
-        *p = Elem<T>::down(f[0]);
-    } else {
-        T t[E];
+    // rounds to T on the way out, and keeps what was stored
+    __device__ __forceinline__ void round_and_store(T* p) {
+        if constexpr (E == 1) {
+            const T t = Elem<T>::down(v[0].x);
+            *p = t;
+            v[0].x = Elem<T>::up(t);
+        } else {
+            T t[E];
+            pack(t);
+            *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(t);
 #pragma unroll
-        for (int e = 0; e < E; ++e) t[e] = Elem<T>::down(f[e]);
-        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(t);
+            for (int i = 0; i < P; ++i) v[i] = make_float2(Elem<T>::up(t[2 * i]), Elem<T>::up(t[2 * i + 1]));
+        }
     }
-}
+    __device__ __forceinline__ void pack(T (&t)[E]) const {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<__half2*>(t + 2 * i) = __float22half2_rn(v[i]);
+            else if constexpr (std::is_same<T, __nv_bfloat16>::value) *reinterpret_cast<__nv_bfloat162*>(t + 2 * i) = __float22bfloat162_rn(v[i]);
+            else { t[2 * i] = v[i].x; t[2 * i + 1] = v[i].y; }
+        }
+    }
+};
 
 // E elements a load (a 16-byte vector, or one where rows are not aligned), NV loads a thread, RW warps a row.
 template <typename T, int E, int NV, int RW>
-__global__ void __launch_bounds__(RW >= 8 ? RW * 32 : 256)
+__global__ void __launch_bounds__(RW >= 4 ? RW * 32 : 128)
 rms_norm_quant_kernel(const RmsNormParams p)
 {
-    constexpr int ROWS = RW >= 8 ? 1 : 8 / RW;     // rows of a block
+    using V = Vec<T, E>;
+    constexpr int P = V::P;
+    constexpr int ROWS = RW >= 4 ? 1 : 4 / RW;     // rows of a block
     constexpr int T_ROW = RW * 32;                 // threads of a row
     __shared__ float red_sum[RW > 1 ? ROWS * RW : 1];
-    __shared__ uint32_t red_max[RW > 1 ? ROWS * RW : 1];
+    __shared__ float red_max[RW > 1 ? ROWS * RW : 1];
     const int sub = threadIdx.x / T_ROW, t = threadIdx.x % T_ROW;
     const int64_t row = (int64_t)blockIdx.x * ROWS + sub;
     const bool row_ok = row < p.M;                 // rows behind the last one only keep the barriers company
 
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
-    const T* res = static_cast<const T*>(p.residual) + row * p.ldr;
-    T* h_out = static_cast<T*>(p.residual_out) + row * p.ldo;
-    float h[NV][E];
-    float sum = 0.0f;
+    V h[NV];
+    bool on[NV];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-        const int c = (v * T_ROW + t) * E;
+        on[v] = row_ok && (v * T_ROW + t) * E < p.K;
 #pragma unroll
-        for (int e = 0; e < E; ++e) h[v][e] = 0.0f;
-        if (row_ok && c < p.K) load_vec<T, E>(x + c, h[v]);
+        for (int i = 0; i < P; ++i) h[v].v[i] = make_float2(0.0f, 0.0f);
+        if (on[v]) h[v].load(x + (v * T_ROW + t) * E);
     }
     if (p.residual != nullptr) {
+        const T* res = static_cast<const T*>(p.residual) + row * p.ldr;
+        T* h_out = static_cast<T*>(p.residual_out) + row * p.ldo;
+        V r[NV];
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+            if (on[v]) r[v].load(res + (v * T_ROW + t) * E);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const int c = (v * T_ROW + t) * E;
-            if (!(row_ok && c < p.K)) continue;
-            float r[E];
-            load_vec<T, E>(res + c, r);
+            if (!on[v]) continue;
 #pragma unroll
-            for (int e = 0; e < E; ++e) h[v][e] = round_to<T>(h[v][e] + r[e]);
-            store_vec<T, E>(h_out + c, h[v]);
+            for (int i = 0; i < P; ++i) h[v].v[i] = __fadd2_rn(h[v].v[i], r[v].v[i]);
+            h[v].round_and_store(h_out + (v * T_ROW + t) * E);
         }
     }
+    float2 sum2 = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int e = 0; e < E; ++e) sum = fmaf(h[v][e], h[v][e], sum);
-    sum = warp_sum(sum);
+        for (int i = 0; i < P; ++i) sum2 = __ffma2_rn(h[v].v[i], h[v].v[i], sum2);
+    float sum = warp_sum(sum2.x + sum2.y);
     if constexpr (RW > 1) {
         if ((t & 31) == 0) red_sum[sub * RW + (t >> 5)] = sum;
         __syncthreads();
@@ -105,74 +129,87 @@ rms_norm_quant_kernel(const RmsNormParams p)
         for (int w = 1; w < RW; ++w) sum += red_sum[sub * RW + w];
     }
     const float u = rsqrtf(fmaf(sum, p.inv_k, p.eps));
+    const float2 u2 = make_float2(u, u);
 
-    uint32_t amax_bits = 0;
+    float amax = 0.0f;
     const T* w = static_cast<const T*>(p.weight);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-        const int c = (v * T_ROW + t) * E;
-        if (!(row_ok && c < p.K)) continue;
-        float wv[E];
-        load_vec<T, E>(w + c, wv);
+        if (!on[v]) continue;
+        V wv;
+        wv.load(w + (v * T_ROW + t) * E);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            h[v][e] = h[v][e] * u * wv[e];
-            amax_bits = max(amax_bits, __float_as_uint(h[v][e]) & 0x7FFFFFFFu);   // as integers: a NaN wins
+        for (int i = 0; i < P; ++i) {
+            h[v].v[i] = __fmul2_rn(__fmul2_rn(h[v].v[i], u2), wv.v[i]);
+            amax = max_abs_nan(amax, h[v].v[i].x);
+            if constexpr (E > 1) amax = max_abs_nan(amax, h[v].v[i].y);
         }
     }
-    amax_bits = warp_umax(amax_bits);
+    // non-negative floats and NaNs order as integers do
+    amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax) & 0x7FFFFFFFu));
     if constexpr (RW > 1) {
-        if ((t & 31) == 0) red_max[sub * RW + (t >> 5)] = amax_bits;
+        if ((t & 31) == 0) red_max[sub * RW + (t >> 5)] = amax;
         __syncthreads();
-        amax_bits = red_max[sub * RW];
+        amax = red_max[sub * RW];
 #pragma unroll
-        for (int k = 1; k < RW; ++k) amax_bits = max(amax_bits, red_max[sub * RW + k]);
+        for (int k = 1; k < RW; ++k) amax = max_abs_nan(amax, red_max[sub * RW + k]);
     }
     if (!row_ok) return;
-    const float amax = __uint_as_float(amax_bits);
     // a row with a NaN or an infinity has a NaN scale and zero codes
-    const bool finite = amax_bits < 0x7F800000u;
+    const bool finite = (__float_as_uint(amax) & 0x7FFFFFFFu) < 0x7F800000u;
     const float s = finite ? __fdiv_rn(fmaxf(amax, 1e-5f), p.qmax) : __uint_as_float(0x7FC00000u);
     if (t == 0 && p.scale != nullptr) p.scale[row] = s;
-    const Divider d = make_divider(s);
+    // y / s, correctly rounded (a multiply by the reciprocal and one correction), plus 1.5 * 2^23: the sum rounds the
+    // quotient half to even to an integer, whose low byte is the code.  |y / s| <= q_max (1 + 2^-23), so none is clamped.
+    const float inv = finite ? __frcp_rn(s) : 0.0f;
+    const float2 inv2 = make_float2(inv, inv), ns2 = make_float2(-s, -s), magic2 = make_float2(kRoundMagic, kRoundMagic);
+    const float2 s2 = make_float2(s, s), nmagic2 = make_float2(-kRoundMagic, -kRoundMagic);
     int8_t* q_out = p.q == nullptr ? nullptr : p.q + row * (int64_t)p.K;
     T* fq = p.fq == nullptr ? nullptr : static_cast<T*>(p.fq) + row * (int64_t)p.K;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
+        if (!on[v]) continue;
         const int c = (v * T_ROW + t) * E;
-        if (c >= p.K) continue;
-        float q[E];
+        uint32_t code[2 * P];
 #pragma unroll
-        for (int e = 0; e < E; ++e) q[e] = finite ? rint_small(div_exact(h[v][e], d), h[v][e]) : 0.0f;
+        for (int i = 0; i < P; ++i) {
+            const float2 y0 = __fmul2_rn(h[v].v[i], inv2);
+            const float2 y = __ffma2_rn(__ffma2_rn(y0, ns2, h[v].v[i]), inv2, y0);
+            const float2 m = __fadd2_rn(y, magic2);
+            code[2 * i] = finite ? __float_as_uint(m.x) : 0u;
+            code[2 * i + 1] = finite ? __float_as_uint(m.y) : 0u;
+            h[v].v[i] = __fmul2_rn(__fadd2_rn(m, nmagic2), s2);
+        }
         if (q_out != nullptr) {
             if constexpr (E == 1) {
-                q_out[c] = (int8_t)code_byte(q[0], p.qmax);
+                q_out[c] = (int8_t)(code[0] & 0xFFu);
             } else {
                 uint32_t word[E / 4];
 #pragma unroll
-                for (int k = 0; k < E / 4; ++k) {
-                    word[k] = 0;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) word[k] |= code_byte(q[4 * k + e], p.qmax) << (8 * e);
-                }
+                for (int k = 0; k < E / 4; ++k)
+                    word[k] = __byte_perm(__byte_perm(code[4 * k], code[4 * k + 1], 0x0040), __byte_perm(code[4 * k + 2], code[4 * k + 3], 0x0040), 0x5410);
                 if constexpr (E == 8) *reinterpret_cast<uint2*>(q_out + c) = make_uint2(word[0], word[1]);
                 else *reinterpret_cast<uint32_t*>(q_out + c) = word[0];
             }
         }
         if (fq != nullptr) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) q[e] *= s;
-            store_vec<T, E>(fq + c, q);
+            if constexpr (E == 1) {
+                fq[c] = Elem<T>::down(h[v].v[0].x);
+            } else {
+                T o[E];
+                h[v].pack(o);
+                *reinterpret_cast<uint4*>(fq + c) = *reinterpret_cast<const uint4*>(o);
+            }
         }
     }
 }
 
 template <typename T, int E, int NV, int RW>
 int launch(const RmsNormParams& p, cudaStream_t st) {
-    constexpr int ROWS = RW >= 8 ? 1 : 8 / RW;
+    constexpr int ROWS = RW >= 4 ? 1 : 4 / RW;
     const int64_t blocks = (p.M + ROWS - 1) / ROWS;
     if (blocks > 2147483647LL) return fail(SAMQ_ERR_TOO_LARGE, "RMS norm of %lld rows is too large", (long long)p.M);
-    rms_norm_quant_kernel<T, E, NV, RW><<<(unsigned)blocks, RW >= 8 ? RW * 32 : 256, 0, st>>>(p);
+    rms_norm_quant_kernel<T, E, NV, RW><<<(unsigned)blocks, RW >= 4 ? RW * 32 : 128, 0, st>>>(p);
     SAMQ_CUDA_TRY(cudaGetLastError());
     return SAMQ_OK;
 }
@@ -193,7 +230,9 @@ int launch_rms_norm(const RmsNormParams& p, cudaStream_t st) {
     constexpr int E = Elem<T>::kPerVec;
     // 5 vectors: 1280 columns of a 16-bit type are one warp's, with no lane idle
     if (p.vec) return launch_warps<T, E, 5>(p.K / E, p, st);
-    return launch_warps<T, 1, 32>(p.K, p, st);
+    // single elements: more warps and fewer elements each, while a block can hold the row so
+    if (p.K <= 8192) return launch_warps<T, 1, 8>(p.K, p, st);
+    return launch<T, 1, 32, 32>(p, st);
 }
 
 }  // namespace

@@ -475,7 +475,7 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, 
             raise ValueError("residual must have the shape, dtype and device of x")
         res2, _, _, ldr = _as_rows(residual)
         if residual_out is None:
-            h = h2 = torch.empty(shape, dtype=dtype, device=dev)
+            h = h2 = torch.empty_like(x, memory_format=torch.contiguous_format)
             ldo = K
         else:
             h = residual_out
@@ -484,12 +484,12 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, 
                 raise ValueError("residual_out must be rows of K contiguous elements with the shape, dtype and device of x")
     elif residual_out is not None:
         raise ValueError("residual_out without a residual")
-    out = {"scale": torch.empty(shape[:-1], dtype=torch.float32, device=dev)}
+    out = {"scale": x.new_empty(shape[:-1], dtype=torch.float32)}
     q = fq = None
     if codes:
-        out["q"] = q = torch.empty(shape, dtype=torch.int8, device=dev)
+        out["q"] = q = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
     if fake_quant:
-        out["fq"] = fq = torch.empty(shape, dtype=dtype, device=dev)
+        out["fq"] = fq = torch.empty_like(x, memory_format=torch.contiguous_format)
     if h is not None:
         out["residual"] = h
     nbytes = M * K * (dtype.itemsize * (1 + (2 if h is not None else 0) + (1 if fake_quant else 0)) + (1 if codes else 0)) + 4 * M
@@ -572,9 +572,9 @@ def quantize_fp4(x: torch.Tensor, fmt: str = "nvfp4", global_scale: float = 1.0,
         raise ValueError(f"Invalid 4-bit format: {fmt}")
     x2, M, K, ldx = _as_rows(x)
     pitch = (K + 31) // 32 * 16
-    codes = torch.empty((M, pitch), dtype=torch.uint8, device=dev)
-    scales = torch.empty(fp4_scale_shape(fmt, M, K), dtype=torch.uint8, device=dev)
-    fq = torch.empty(x.shape, dtype=x.dtype, device=dev) if fake_quant else None
+    codes = x.new_empty((M, pitch), dtype=torch.uint8)
+    scales = x.new_empty(fp4_scale_shape(fmt, M, K), dtype=torch.uint8)
+    fq = torch.empty_like(x, memory_format=torch.contiguous_format) if fake_quant else None
     nbytes = M * K * x.dtype.itemsize * (2 if fake_quant else 1) + codes.numel() + scales.numel()
     _call(dev, "quant_fp4", nbytes, _lib.load().samq_quant_fp4, x2.data_ptr(), code, M, K, ldx, fcode, global_scale, codes.data_ptr(), pitch,
           scales.data_ptr(), _data_ptr(fq))
@@ -618,7 +618,7 @@ def gemm_fp4(a: Fp4Tensor, w: Fp4Tensor, bias: Optional[torch.Tensor] = None, re
     M, N, K = a.rows, w.rows, a.K
     code, bias, residual, ldr = _linear_args(N, M, bias, residual, out_dtype, dev)
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=dev)
+        out = ac.new_empty((M, N), dtype=out_dtype)
     elif out.dtype != out_dtype or out.device != dev or out.shape[-1] != N or out.numel() != M * N or not out.is_contiguous():
         raise ValueError("out has the wrong dtype, device, shape or layout")
     _call(dev, "gemm_fp4", 2.0 * M * N * K, _lib.load().samq_gemm_fp4, ac.data_ptr(), ac.stride(0), a.scales.data_ptr(), wc.data_ptr(),
@@ -642,7 +642,7 @@ def linear_fp4(x: torch.Tensor, w: Fp4Tensor, bias: Optional[torch.Tensor] = Non
             raise ValueError("x must be on the device of w")
         x2, M, _, ldx = _as_rows(x)
         code, bias, residual, ldr = _linear_args(N, M, bias, residual, x.dtype, dev)
-        out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
+        out = x.new_empty((*x.shape[:-1], N))
         _call(dev, "linear_fp4", 2.0 * M * N * K, _lib.load().samq_linear_fp4, x2.data_ptr(), code, ldx, w.codes.data_ptr(), w.codes.stride(0),
               w.scales.data_ptr(), M, N, K, FP4_FORMATS[w.fmt], w.global_scale, _data_ptr(bias), _data_ptr(residual), ldr, activation,
               out.data_ptr(), N, _status_ptr(dev))
