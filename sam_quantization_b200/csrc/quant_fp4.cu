@@ -182,6 +182,7 @@ int quant_fp4_dispatch(const void* x, int dtype, int64_t M, int64_t K, int64_t l
                        uint8_t* codes, int64_t ldq, uint8_t* scales, void* fq, void* stream)
 {
     if (M < 0 || K <= 0) return fail(SAMQ_ERR_BAD_ARG, "bad shape M=%lld K=%lld", (long long)M, (long long)K);
+    if (K > 2147483647LL - 256) return fail(SAMQ_ERR_TOO_LARGE, "K=%lld exceeds 2^31", (long long)K);
     if (dtype != SAMQ_F16 && dtype != SAMQ_BF16 && dtype != SAMQ_F32) return fail(SAMQ_ERR_BAD_ARG, "unknown dtype %d", dtype);
     if (!fp4::known_format(fmt)) return fail(SAMQ_ERR_BAD_ARG, "unknown 4-bit format %d", fmt);
     if (!fp4::good_global_scale(global_scale)) return fail(SAMQ_ERR_BAD_ARG, "global_scale must be a power of two between 2^-64 and 2^64");

@@ -37,47 +37,39 @@ __device__ __forceinline__ float max_abs_nan(float a, float b) {
     return r;
 }
 
-// E elements of a row as fp32 pairs (E = 1: the second of the pair is 0)
+// E elements of a row in the tensor type (a 16-byte vector, or one element), widened to fp32 pairs where they are used
+// (E = 1: the second of the pair is 0)
 template <typename T, int E> struct Vec {
     static constexpr int P = E == 1 ? 1 : E / 2;
-    float2 v[P];
+    union { uint4 raw; T t[E]; };
+    __device__ __forceinline__ Vec() {}
+    __device__ __forceinline__ void zero() {
+        if constexpr (E == 1) t[0] = Elem<T>::down(0.0f);
+        else raw = make_uint4(0, 0, 0, 0);
+    }
     __device__ __forceinline__ void load(const T* p) {
-        if constexpr (E == 1) {
-            v[0] = make_float2(Elem<T>::up(*p), 0.0f);
-        } else {
-            T t[E];
-            *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(p);
-#pragma unroll
-            for (int i = 0; i < P; ++i) v[i] = make_float2(Elem<T>::up(t[2 * i]), Elem<T>::up(t[2 * i + 1]));
-        }
+        if constexpr (E == 1) t[0] = *p;
+        else raw = *reinterpret_cast<const uint4*>(p);
     }
-    // rounds to T on the way out, and keeps what was stored
-    __device__ __forceinline__ void round_and_store(T* p) {
-        if constexpr (E == 1) {
-            const T t = Elem<T>::down(v[0].x);
-            *p = t;
-            v[0].x = Elem<T>::up(t);
-        } else {
-            T t[E];
-            pack(t);
-            *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(t);
-#pragma unroll
-            for (int i = 0; i < P; ++i) v[i] = make_float2(Elem<T>::up(t[2 * i]), Elem<T>::up(t[2 * i + 1]));
-        }
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (E == 1) *p = t[0];
+        else *reinterpret_cast<uint4*>(p) = raw;
     }
-    __device__ __forceinline__ void pack(T (&t)[E]) const {
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-            if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<__half2*>(t + 2 * i) = __float22half2_rn(v[i]);
-            else if constexpr (std::is_same<T, __nv_bfloat16>::value) *reinterpret_cast<__nv_bfloat162*>(t + 2 * i) = __float22bfloat162_rn(v[i]);
-            else { t[2 * i] = v[i].x; t[2 * i + 1] = v[i].y; }
-        }
+    __device__ __forceinline__ float2 pair(int i) const {
+        if constexpr (E == 1) return make_float2(Elem<T>::up(t[0]), 0.0f);
+        else return make_float2(Elem<T>::up(t[2 * i]), Elem<T>::up(t[2 * i + 1]));
+    }
+    __device__ __forceinline__ void set(int i, float2 v) {
+        if constexpr (E == 1) t[0] = Elem<T>::down(v.x);
+        else if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<__half2*>(t + 2 * i) = __float22half2_rn(v);
+        else if constexpr (std::is_same<T, __nv_bfloat16>::value) *reinterpret_cast<__nv_bfloat162*>(t + 2 * i) = __float22bfloat162_rn(v);
+        else { t[2 * i] = v.x; t[2 * i + 1] = v.y; }
     }
 };
 
 // E elements a load (a 16-byte vector, or one where rows are not aligned), NV loads a thread, RW warps a row.
-template <typename T, int E, int NV, int RW>
-__global__ void __launch_bounds__(RW >= 4 ? RW * 32 : 128)
+template <typename T, int E, int NV, int RW, bool RES>
+__global__ void __launch_bounds__(RW >= 4 ? RW * 32 : 128, 1)
 rms_norm_quant_kernel(const RmsNormParams p)
 {
     using V = Vec<T, E>;
@@ -88,38 +80,41 @@ rms_norm_quant_kernel(const RmsNormParams p)
     __shared__ float red_max[RW > 1 ? ROWS * RW : 1];
     const int sub = threadIdx.x / T_ROW, t = threadIdx.x % T_ROW;
     const int64_t row = (int64_t)blockIdx.x * ROWS + sub;
-    const bool row_ok = row < p.M;                 // rows behind the last one only keep the barriers company
+    // loads of this thread; rows behind the last one only keep the barriers company
+    const int nv = row < p.M ? (p.K / E - t + T_ROW - 1) / T_ROW : 0;
 
-    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
     V h[NV];
-    bool on[NV];
+    {
+        const T* x = static_cast<const T*>(p.x) + row * p.ldx + t * E;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        on[v] = row_ok && (v * T_ROW + t) * E < p.K;
-#pragma unroll
-        for (int i = 0; i < P; ++i) h[v].v[i] = make_float2(0.0f, 0.0f);
-        if (on[v]) h[v].load(x + (v * T_ROW + t) * E);
+        for (int v = 0; v < NV; ++v) {
+            h[v].zero();
+            if (v < nv) h[v].load(x + v * T_ROW * E);
+        }
     }
-    if (p.residual != nullptr) {
-        const T* res = static_cast<const T*>(p.residual) + row * p.ldr;
-        T* h_out = static_cast<T*>(p.residual_out) + row * p.ldo;
+    if constexpr (RES) {
+        const T* res = static_cast<const T*>(p.residual) + row * p.ldr + t * E;
+        T* h_out = static_cast<T*>(p.residual_out) + row * p.ldo + t * E;
         V r[NV];
 #pragma unroll
         for (int v = 0; v < NV; ++v)
-            if (on[v]) r[v].load(res + (v * T_ROW + t) * E);
+            if (v < nv) r[v].load(res + v * T_ROW * E);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            if (!on[v]) continue;
+            if (v >= nv) continue;
 #pragma unroll
-            for (int i = 0; i < P; ++i) h[v].v[i] = __fadd2_rn(h[v].v[i], r[v].v[i]);
-            h[v].round_and_store(h_out + (v * T_ROW + t) * E);
+            for (int i = 0; i < P; ++i) h[v].set(i, __fadd2_rn(h[v].pair(i), r[v].pair(i)));     // rounded as it is stored
+            h[v].store(h_out + v * T_ROW * E);
         }
     }
     float2 sum2 = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int i = 0; i < P; ++i) sum2 = __ffma2_rn(h[v].v[i], h[v].v[i], sum2);
+        for (int i = 0; i < P; ++i) {
+            const float2 f = h[v].pair(i);
+            sum2 = __ffma2_rn(f, f, sum2);
+        }
     float sum = warp_sum(sum2.x + sum2.y);
     if constexpr (RW > 1) {
         if ((t & 31) == 0) red_sum[sub * RW + (t >> 5)] = sum;
@@ -132,17 +127,18 @@ rms_norm_quant_kernel(const RmsNormParams p)
     const float2 u2 = make_float2(u, u);
 
     float amax = 0.0f;
-    const T* w = static_cast<const T*>(p.weight);
+    float2 y[NV][P];
+    const T* w = static_cast<const T*>(p.weight) + t * E;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-        if (!on[v]) continue;
+        if (v >= nv) continue;
         V wv;
-        wv.load(w + (v * T_ROW + t) * E);
+        wv.load(w + v * T_ROW * E);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            h[v].v[i] = __fmul2_rn(__fmul2_rn(h[v].v[i], u2), wv.v[i]);
-            amax = max_abs_nan(amax, h[v].v[i].x);
-            if constexpr (E > 1) amax = max_abs_nan(amax, h[v].v[i].y);
+            y[v][i] = __fmul2_rn(__fmul2_rn(h[v].pair(i), u2), wv.pair(i));
+            amax = max_abs_nan(amax, y[v][i].x);
+            if constexpr (E > 1) amax = max_abs_nan(amax, y[v][i].y);
         }
     }
     // non-negative floats and NaNs order as integers do
@@ -154,7 +150,7 @@ rms_norm_quant_kernel(const RmsNormParams p)
 #pragma unroll
         for (int k = 1; k < RW; ++k) amax = max_abs_nan(amax, red_max[sub * RW + k]);
     }
-    if (!row_ok) return;
+    if (row >= p.M) return;
     // a row with a NaN or an infinity has a NaN scale and zero codes
     const bool finite = (__float_as_uint(amax) & 0x7FFFFFFFu) < 0x7F800000u;
     const float s = finite ? __fdiv_rn(fmaxf(amax, 1e-5f), p.qmax) : __uint_as_float(0x7FC00000u);
@@ -164,21 +160,22 @@ rms_norm_quant_kernel(const RmsNormParams p)
     const float inv = finite ? __frcp_rn(s) : 0.0f;
     const float2 inv2 = make_float2(inv, inv), ns2 = make_float2(-s, -s), magic2 = make_float2(kRoundMagic, kRoundMagic);
     const float2 s2 = make_float2(s, s), nmagic2 = make_float2(-kRoundMagic, -kRoundMagic);
-    int8_t* q_out = p.q == nullptr ? nullptr : p.q + row * (int64_t)p.K;
-    T* fq = p.fq == nullptr ? nullptr : static_cast<T*>(p.fq) + row * (int64_t)p.K;
+    int8_t* q_out = p.q == nullptr ? nullptr : p.q + row * (int64_t)p.K + t * E;
+    T* fq = p.fq == nullptr ? nullptr : static_cast<T*>(p.fq) + row * (int64_t)p.K + t * E;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-        if (!on[v]) continue;
-        const int c = (v * T_ROW + t) * E;
+        if (v >= nv) continue;
+        const int c = v * T_ROW * E;
         uint32_t code[2 * P];
+        V o;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const float2 y0 = __fmul2_rn(h[v].v[i], inv2);
-            const float2 y = __ffma2_rn(__ffma2_rn(y0, ns2, h[v].v[i]), inv2, y0);
-            const float2 m = __fadd2_rn(y, magic2);
+            const float2 y0 = __fmul2_rn(y[v][i], inv2);
+            const float2 z = __ffma2_rn(__ffma2_rn(y0, ns2, y[v][i]), inv2, y0);
+            const float2 m = __fadd2_rn(z, magic2);
             code[2 * i] = finite ? __float_as_uint(m.x) : 0u;
             code[2 * i + 1] = finite ? __float_as_uint(m.y) : 0u;
-            h[v].v[i] = __fmul2_rn(__fadd2_rn(m, nmagic2), s2);
+            o.set(i, __fmul2_rn(__fadd2_rn(m, nmagic2), s2));
         }
         if (q_out != nullptr) {
             if constexpr (E == 1) {
@@ -192,15 +189,7 @@ rms_norm_quant_kernel(const RmsNormParams p)
                 else *reinterpret_cast<uint32_t*>(q_out + c) = word[0];
             }
         }
-        if (fq != nullptr) {
-            if constexpr (E == 1) {
-                fq[c] = Elem<T>::down(h[v].v[0].x);
-            } else {
-                T o[E];
-                h[v].pack(o);
-                *reinterpret_cast<uint4*>(fq + c) = *reinterpret_cast<const uint4*>(o);
-            }
-        }
+        if (fq != nullptr) o.store(fq + c);
     }
 }
 
@@ -209,7 +198,9 @@ int launch(const RmsNormParams& p, cudaStream_t st) {
     constexpr int ROWS = RW >= 4 ? 1 : 4 / RW;
     const int64_t blocks = (p.M + ROWS - 1) / ROWS;
     if (blocks > 2147483647LL) return fail(SAMQ_ERR_TOO_LARGE, "RMS norm of %lld rows is too large", (long long)p.M);
-    rms_norm_quant_kernel<T, E, NV, RW><<<(unsigned)blocks, RW >= 4 ? RW * 32 : 128, 0, st>>>(p);
+    const int threads = RW >= 4 ? RW * 32 : 128;
+    if (p.residual != nullptr) rms_norm_quant_kernel<T, E, NV, RW, true><<<(unsigned)blocks, threads, 0, st>>>(p);
+    else rms_norm_quant_kernel<T, E, NV, RW, false><<<(unsigned)blocks, threads, 0, st>>>(p);
     SAMQ_CUDA_TRY(cudaGetLastError());
     return SAMQ_OK;
 }
