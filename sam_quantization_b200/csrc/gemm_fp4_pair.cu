@@ -12,6 +12,10 @@
 // Two accumulators of 192 columns and the ring fill tensor memory.  256-column tiles would have to share columns between
 // the two accumulators; the hand-over across the pair that this needs took 1.5 us a tile.
 //
+// What bounds the kernel is the traffic between L2 and the SMs, about 43 bytes a clock and SM.  So where the A tile of
+// a pair fits shared memory whole (K <= 1280) it stays there (RESIDENT): a pair walks along consecutive N tiles of its
+// rows, and a stage is W's part only, 16 instead of 34 KiB.
+//
 // Twelve epilogue warps (32 rows x 64 columns each) read their columns at once and hand them back before they compute.
 // The residual comes in by TMA into the warp's staging buffer while the tile is computed, the result leaves from there
 // by TMA.  Every wait is bounded.
@@ -31,6 +35,7 @@ constexpr int B_BYTES = BNH * BK;
 constexpr int EPI_WARPS = 4 * (BN / EPI_COLS);
 constexpr int FIRST_EPI_WARP = 4;                // TMA, MMA, scale copies, one idle
 constexpr int THREADS = (FIRST_EPI_WARP + EPI_WARPS) * 32;
+constexpr int RESIDENT_BLOCKS = 5;               // blocks of 256 columns of a resident A tile
 constexpr int TMEM_COLS = 512;
 constexpr int SF_COL = 2 * BN;                   // the ring of scale columns behind the accumulators
 
@@ -41,7 +46,8 @@ template <int FMT> struct Shape {
     static_assert(SF_COL + UNITS * UNIT_COLS <= TMEM_COLS, "accumulators and scales fit tensor memory");
     static constexpr int SFA_BYTES = GROUPS * TILE_BYTES;
     static constexpr int SFB_BYTES = 2 * GROUPS * TILE_BYTES;      // 192 rows of W lie in two tiles of 128
-    static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
+    static constexpr int A_BLOCK_BYTES = A_BYTES + SFA_BYTES;
+    static constexpr int W_BLOCK_BYTES = B_BYTES + SFB_BYTES;
 };
 
 struct __align__(8) Control {
@@ -51,13 +57,17 @@ struct __align__(8) Control {
     uint64_t acc_empty[2];
     uint64_t sf_ready[4];                         // scale columns written (the leader's only)
     uint64_t res[EPI_WARPS];
+    uint64_t a_full[RESIDENT_BLOCKS];             // RESIDENT: blocks of A loaded / no longer read
+    uint64_t a_empty[RESIDENT_BLOCKS];
     uint32_t tmem_base;
     uint32_t abort_flag;
 };
 
-template <int FMT>
+// A blocks: one a stage, or all of a resident tile
+constexpr int a_blocks(bool resident) { return resident ? RESIDENT_BLOCKS : STAGES; }
+template <int FMT, bool RESIDENT>
 constexpr size_t smem_bytes() {
-    return 1024 + (size_t)STAGES * Shape<FMT>::STAGE_BYTES + (size_t)EPI_WARPS * (STAGING_BYTES + EPI_COLS * sizeof(float)) + sizeof(Control);
+    return 1024 + (size_t)a_blocks(RESIDENT) * Shape<FMT>::A_BLOCK_BYTES + (size_t)STAGES * Shape<FMT>::W_BLOCK_BYTES + (size_t)EPI_WARPS * (STAGING_BYTES + EPI_COLS * sizeof(float)) + sizeof(Control);
 }
 
 struct PairParams {
@@ -66,7 +76,7 @@ struct PairParams {
     int32_t* status;
 };
 
-template <typename OutT, int FMT, bool GELU, bool RES>
+template <typename OutT, int FMT, bool GELU, bool RES, bool RESIDENT>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                      const __grid_constant__ CUtensorMap map_sfa, const __grid_constant__ CUtensorMap map_sfw,
@@ -77,9 +87,11 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = smem_u32(smem_raw);
     uint8_t* tiles = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);              // 1024-byte aligned
-    uint8_t* staging = tiles + (size_t)STAGES * (A_BYTES + B_BYTES);                     // 1024-byte aligned
-    uint8_t* sf = staging + (size_t)EPI_WARPS * STAGING_BYTES;
-    float* bias_s = reinterpret_cast<float*>(sf + (size_t)STAGES * (S::SFA_BYTES + S::SFB_BYTES));
+    uint8_t* w_tiles = tiles + (size_t)a_blocks(RESIDENT) * A_BYTES;                     // all of these 1024-byte aligned
+    uint8_t* staging = w_tiles + (size_t)STAGES * B_BYTES;
+    uint8_t* sfa_s = staging + (size_t)EPI_WARPS * STAGING_BYTES;
+    uint8_t* sfw_s = sfa_s + (size_t)a_blocks(RESIDENT) * S::SFA_BYTES;
+    float* bias_s = reinterpret_cast<float*>(sfw_s + (size_t)STAGES * S::SFB_BYTES);
     Control* ctl = reinterpret_cast<Control*>(bias_s + EPI_WARPS * EPI_COLS);
     volatile uint32_t* abort_flag = &ctl->abort_flag;
 
@@ -90,12 +102,19 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     const int n_blocks = (p.epi.N + BN - 1) / BN;
     const int k_blocks = (p.K + KPAD - 1) / KPAD;
     const int num_tiles = m_blocks * n_blocks;
+    // RESIDENT: consecutive tiles, so that A changes seldom; else the pairs work side by side
+    const int first_tile = RESIDENT ? (int)((int64_t)num_tiles * pair / num_pairs) : pair;
+    const int end_tile = RESIDENT ? (int)((int64_t)num_tiles * (pair + 1) / num_pairs) : num_tiles;
+    const int tile_step = RESIDENT ? 1 : num_pairs;
+    auto new_rows = [&](int tile) { return tile == first_tile || tile / n_blocks != (tile - 1) / n_blocks; };
+    auto rows_done = [&](int tile) { return tile + 1 < end_tile && (tile + 1) / n_blocks != tile / n_blocks; };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(smem_u32(&ctl->full[s]), 1); mbar_init(smem_u32(&ctl->empty[s]), 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(smem_u32(&ctl->acc_full[b]), 1); mbar_init(smem_u32(&ctl->acc_empty[b]), 2 * EPI_WARPS); }
         for (int u = 0; u < 4; ++u) mbar_init(smem_u32(&ctl->sf_ready[u]), 1);
         for (int w = 0; w < EPI_WARPS; ++w) mbar_init(smem_u32(&ctl->res[w]), 1);
+        for (int b = 0; b < RESIDENT_BLOCKS; ++b) { mbar_init(smem_u32(&ctl->a_full[b]), 1); mbar_init(smem_u32(&ctl->a_empty[b]), 1); }
         ctl->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -112,58 +131,71 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
 
     if (warp == 0) {
         // ---------------- TMA producer ----------------
-        if (lane == 0) {
-            int stage = 0; uint32_t phase = 0;
-            bool ok = true;
-            for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
-                const int mt = (tile / n_blocks) * 2 + (int)rank;          // this CTA's 128-row tile of A
-                const int n0 = (tile % n_blocks) * BN;
-                const int nt = n0 / TILE_ROWS;                             // first of W's two scale tiles
-                for (int kb = 0; kb < k_blocks; ++kb) {
-                    if (!mbar_wait(smem_u32(&ctl->empty[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
-                    const uint32_t bar = smem_u32(&ctl->full[stage]);
-                    const uint32_t leader_bar = map_to_cta(bar, 0);
-                    const uint32_t sa = smem_u32(tiles + (size_t)stage * (A_BYTES + B_BYTES));
-                    const uint32_t ss = smem_u32(sf + (size_t)stage * (S::SFA_BYTES + S::SFB_BYTES));
-                    if (rank == 0) mbar_expect_tx(bar, 2 * S::STAGE_BYTES);       // bytes of both CTAs
-                    tma_load_2d_pair(sa, &map_a, leader_bar, kb * BK, mt * BM);
-                    tma_load_2d_pair(sa + A_BYTES, &map_w, leader_bar, kb * BK, n0 + (int)rank * BNH);
-                    tma_load_2d_pair(ss, &map_sfa, leader_bar, 0, mt * p.groups + kb * S::GROUPS);
-                    tma_load_2d_pair(ss + S::SFA_BYTES, &map_sfw, leader_bar, 0, nt * p.groups + kb * S::GROUPS);
-                    tma_load_2d_pair(ss + S::SFA_BYTES + S::SFB_BYTES / 2, &map_sfw, leader_bar, 0, (nt + 1) * p.groups + kb * S::GROUPS);
-                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        int stage = 0; uint32_t phase = 0, a_phase = 1;
+        bool ok = true;
+        for (int tile = first_tile; tile < end_tile && ok; tile += tile_step) {
+            const int mt = (tile / n_blocks) * 2 + (int)rank;              // this CTA's 128-row tile of A
+            const int n0 = (tile % n_blocks) * BN;
+            const int nt = n0 / TILE_ROWS;                                 // first of W's two scale tiles
+            const bool load_a = RESIDENT && new_rows(tile);
+            for (int kb = 0; kb < k_blocks; ++kb) {
+                if (load_a) ok = mbar_wait(smem_u32(&ctl->a_empty[kb]), a_phase, abort_flag);
+                ok = ok && mbar_wait(smem_u32(&ctl->empty[stage]), phase ^ 1u, abort_flag);
+                if (!ok) break;
+                if (elect_one()) {
+                    const uint32_t bar = smem_u32(&ctl->full[stage]), leader_bar = map_to_cta(bar, 0);
+                    if (load_a || !RESIDENT) {
+                        const int ab = RESIDENT ? kb : stage;
+                        const uint32_t a_bar = RESIDENT ? smem_u32(&ctl->a_full[kb]) : bar;
+                        const uint32_t a_leader = RESIDENT ? map_to_cta(a_bar, 0) : leader_bar;
+                        if (RESIDENT && rank == 0) mbar_expect_tx(a_bar, 2 * S::A_BLOCK_BYTES);       // bytes of both CTAs
+                        if (!RESIDENT && rank == 0) mbar_expect_tx(bar, 2 * (S::A_BLOCK_BYTES + S::W_BLOCK_BYTES));
+                        tma_load_2d_pair(smem_u32(tiles + (size_t)ab * A_BYTES), &map_a, a_leader, kb * BK, mt * BM);
+                        tma_load_2d_pair(smem_u32(sfa_s + (size_t)ab * S::SFA_BYTES), &map_sfa, a_leader, 0, mt * p.groups + kb * S::GROUPS);
+                    }
+                    if (RESIDENT && rank == 0) mbar_expect_tx(bar, 2 * S::W_BLOCK_BYTES);
+                    const uint32_t ss = smem_u32(sfw_s + (size_t)stage * S::SFB_BYTES);
+                    tma_load_2d_pair(smem_u32(w_tiles + (size_t)stage * B_BYTES), &map_w, leader_bar, kb * BK, n0 + (int)rank * BNH);
+                    tma_load_2d_pair(ss, &map_sfw, leader_bar, 0, nt * p.groups + kb * S::GROUPS);
+                    tma_load_2d_pair(ss + S::SFB_BYTES / 2, &map_sfw, leader_bar, 0, (nt + 1) * p.groups + kb * S::GROUPS);
                 }
-            }
-            // every stage has been handed back: no completion from the leader's MMA thread can still be on its way
-            // to this CTA's barriers when the CTA retires
-            for (int s = 0; s < STAGES && ok; ++s) {
-                if (!mbar_wait(smem_u32(&ctl->empty[stage]), phase ^ 1u, abort_flag)) ok = false;
+                __syncwarp();
                 if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
-            if (!ok) {
-                const long long t0 = clock64();
-                while (clock64() - t0 < 2000000LL) { }              // copies in flight land before the CTA retires
-            }
+            if (load_a) a_phase ^= 1u;
+        }
+        // every stage has been handed back: no completion from the leader's MMAs can still be on its way to this CTA's
+        // barriers when the CTA retires
+        for (int s = 0; s < STAGES && ok; ++s) {
+            ok = mbar_wait(smem_u32(&ctl->empty[stage]), phase ^ 1u, abort_flag);
+            if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) {
+            const long long t0 = clock64();
+            while (clock64() - t0 < 2000000LL) { }                  // copies in flight land before the CTA retires
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
         if (rank == 0) {
             int stage = 0; uint32_t phase = 0;
             int acc = 0; uint32_t acc_phase = 0;
-            int unit = 0; uint32_t unit_phase = 0;
+            int unit = 0; uint32_t unit_phase = 0, a_phase = 1;
             bool ok = true;
-            for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+            for (int tile = first_tile; tile < end_tile && ok; tile += tile_step) {
+                const bool wait_a = RESIDENT && new_rows(tile), free_a = RESIDENT && rows_done(tile);
+                if (wait_a) a_phase ^= 1u;
                 if (!mbar_wait(smem_u32(&ctl->acc_empty[acc]), acc_phase ^ 1u, abort_flag)) break;
                 const uint32_t tmem_d = tmem + (uint32_t)(acc * BN);
                 // an odd tile's 192 rows begin in the middle of a scale tile: skip its first 64 rows, two columns
                 const uint32_t sf_shift = (uint32_t)((tile % n_blocks) & 1) * 2u;
                 for (int kb = 0; kb < k_blocks; ++kb) {
                     ok = mbar_wait(smem_u32(&ctl->full[stage]), phase, abort_flag) &&
+                         (!wait_a || mbar_wait(smem_u32(&ctl->a_full[kb]), a_phase, abort_flag)) &&
                          mbar_wait(smem_u32(&ctl->sf_ready[unit]), unit_phase, abort_flag);
                     if (!ok) break;
                     tcgen05_fence_after();
-                    const uint32_t sa = smem_u32(tiles + (size_t)stage * (A_BYTES + B_BYTES));
-                    const uint64_t adesc = make_smem_desc(sa), bdesc = make_smem_desc(sa + A_BYTES);
+                    const uint64_t adesc = make_smem_desc(smem_u32(tiles + (size_t)(RESIDENT ? kb : stage) * A_BYTES));
+                    const uint64_t bdesc = make_smem_desc(smem_u32(w_tiles + (size_t)stage * B_BYTES));
                     const uint32_t sfa = tmem + SF_COL + (uint32_t)(unit * S::UNIT_COLS);
                     const uint32_t sfb = sfa + 4 * S::GROUPS + sf_shift;
                     if (elect_one()) {
@@ -175,6 +207,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                             mma_fp4<FMT, 2>(tmem_d, adesc + (uint64_t)(k * (UKB >> 4)), bdesc + (uint64_t)(k * (UKB >> 4)),
                                             instr_desc(FMT, 2 * BM, BN, id), sfa + 4 * g, sfb + 8 * g, (kb | k) != 0 ? 1u : 0u);
                         }
+                        if (free_a) tcgen05_commit_both(smem_u32(&ctl->a_empty[kb]));
                         tcgen05_commit_both(smem_u32(&ctl->empty[stage]));
                         if (kb == k_blocks - 1) tcgen05_commit_both(smem_u32(&ctl->acc_full[acc]));
                     }
@@ -192,10 +225,14 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             int unit = 0;
             int old_stage = 0; uint32_t old_phase = 0;             // the stage that last used the buffer
             int filled = 0;
+            uint32_t a_phase = 1;
             bool ok = true;
-            for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+            for (int tile = first_tile; tile < end_tile && ok; tile += tile_step) {
+                const bool wait_a = RESIDENT && new_rows(tile);
+                if (wait_a) a_phase ^= 1u;
                 for (int kb = 0; kb < k_blocks; ++kb) {
-                    ok = mbar_wait(smem_u32(&ctl->full[stage]), phase, abort_flag);
+                    ok = mbar_wait(smem_u32(&ctl->full[stage]), phase, abort_flag) &&
+                         (!wait_a || mbar_wait(smem_u32(&ctl->a_full[kb]), a_phase, abort_flag));
                     if (ok && filled == S::UNITS) {
                         ok = mbar_wait(smem_u32(&ctl->empty[old_stage]), old_phase, abort_flag);
                         if (++old_stage == STAGES) { old_stage = 0; old_phase ^= 1u; }
@@ -204,15 +241,16 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                     }
                     if (!ok) break;
                     tcgen05_fence_after();
-                    const uint32_t ss = smem_u32(sf + (size_t)stage * (S::SFA_BYTES + S::SFB_BYTES));
+                    const uint32_t sa = smem_u32(sfa_s + (size_t)(RESIDENT ? kb : stage) * S::SFA_BYTES);
+                    const uint32_t sw = smem_u32(sfw_s + (size_t)stage * S::SFB_BYTES);
                     const uint32_t sfa = tmem + SF_COL + (uint32_t)(unit * S::UNIT_COLS);
                     const uint32_t sfb = sfa + 4 * S::GROUPS;
                     if (elect_one()) {
 #pragma unroll
                         for (int g = 0; g < S::GROUPS; ++g) {
-                            tmem_copy_scales<2>(sfa + 4 * g, scale_desc(ss + g * TILE_BYTES));
-                            tmem_copy_scales<2>(sfb + 8 * g, scale_desc(ss + S::SFA_BYTES + g * TILE_BYTES));
-                            tmem_copy_scales<2>(sfb + 8 * g + 4, scale_desc(ss + S::SFA_BYTES + S::SFB_BYTES / 2 + g * TILE_BYTES));
+                            tmem_copy_scales<2>(sfa + 4 * g, scale_desc(sa + g * TILE_BYTES));
+                            tmem_copy_scales<2>(sfb + 8 * g, scale_desc(sw + g * TILE_BYTES));
+                            tmem_copy_scales<2>(sfb + 8 * g + 4, scale_desc(sw + S::SFB_BYTES / 2 + g * TILE_BYTES));
                         }
                         tcgen05_commit_pair(smem_u32(&ctl->sf_ready[unit]));
                     }
@@ -230,7 +268,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         EpiWarp<OutT, GELU, RES> epi{p.epi, &map_out, &map_res, staging + (size_t)ew * STAGING_BYTES, bias_s + ew * EPI_COLS,
                                      smem_u32(&ctl->res[ew]), 0u, abort_flag, lane};
         int acc = 0; uint32_t acc_phase = 0;
-        for (int tile = pair; tile < num_tiles; tile += num_pairs) {
+        for (int tile = first_tile; tile < end_tile; tile += tile_step) {
             const int row0 = (tile / n_blocks) * (2 * BM) + (int)rank * BM + quad * 32;
             const int col0 = (tile % n_blocks) * BN + cg * EPI_COLS;
             epi.before(row0, col0);
@@ -257,10 +295,11 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     if (threadIdx.x == 0 && ctl->abort_flag != 0 && p.status != nullptr) atomicExch(p.status, 1);
 }
 
-template <typename OutT, int FMT, bool GELU, bool RES>
+template <typename OutT, int FMT, bool GELU, bool RES, bool RESIDENT>
 int launch(const Fp4Call& c, const CUtensorMap& ma, const CUtensorMap& mw, const CUtensorMap& msa, const CUtensorMap& msw, const PairParams& p) {
-    auto kernel = gemm_fp4_pair_kernel<OutT, FMT, GELU, RES>;
-    SAMQ_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<FMT>()));
+    auto kernel = gemm_fp4_pair_kernel<OutT, FMT, GELU, RES, RESIDENT>;
+    constexpr size_t SMEM = smem_bytes<FMT, RESIDENT>();
+    SAMQ_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
     const int64_t tiles = ((c.M + 2 * BM - 1) / (2 * BM)) * ((c.N + BN - 1) / BN);
     if (tiles > 2147483647LL - 256) return fail(SAMQ_ERR_TOO_LARGE, "product of %lld x %lld outputs is too large", (long long)c.M, (long long)c.N);
     cudaLaunchConfig_t cfg;
@@ -268,7 +307,7 @@ int launch(const Fp4Call& c, const CUtensorMap& ma, const CUtensorMap& mw, const
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = smem_bytes<FMT>(); cfg.stream = c.stream;
+    cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM; cfg.stream = c.stream;
     cfg.attrs = attr; cfg.numAttrs = 1;
     // how many pairs the device can hold at once (GPCs with an odd number of SMs leave one out)
     static thread_local int pairs_cached[64] = {0};
@@ -288,7 +327,7 @@ int launch(const Fp4Call& c, const CUtensorMap& ma, const CUtensorMap& mw, const
     return SAMQ_OK;
 }
 
-template <typename OutT, int FMT>
+template <typename OutT, int FMT, bool RESIDENT>
 int launch(const Fp4Call& c) {
     CUtensorMap ma, mw, msa, msw;
     const int64_t row_bytes = (c.K + 1) / 2;
@@ -301,15 +340,16 @@ int launch(const Fp4Call& c) {
     PairParams p;
     p.epi = c.epi; p.K = (int)c.K; p.groups = (int)groups; p.status = c.status;
     const bool res = c.epi.residual != nullptr;
-    if (c.gelu && res) return launch<OutT, FMT, true, true>(c, ma, mw, msa, msw, p);
-    if (c.gelu) return launch<OutT, FMT, true, false>(c, ma, mw, msa, msw, p);
-    if (res) return launch<OutT, FMT, false, true>(c, ma, mw, msa, msw, p);
-    return launch<OutT, FMT, false, false>(c, ma, mw, msa, msw, p);
+    if (c.gelu && res) return launch<OutT, FMT, true, true, RESIDENT>(c, ma, mw, msa, msw, p);
+    if (c.gelu) return launch<OutT, FMT, true, false, RESIDENT>(c, ma, mw, msa, msw, p);
+    if (res) return launch<OutT, FMT, false, true, RESIDENT>(c, ma, mw, msa, msw, p);
+    return launch<OutT, FMT, false, false, RESIDENT>(c, ma, mw, msa, msw, p);
 }
 
 template <typename OutT>
 int launch(const Fp4Call& c) {
-    return c.fmt == SAMQ_FP4_MX ? launch<OutT, SAMQ_FP4_MX>(c) : launch<OutT, SAMQ_FP4_NV>(c);
+    if (c.K <= RESIDENT_BLOCKS * KPAD) return c.fmt == SAMQ_FP4_MX ? launch<OutT, SAMQ_FP4_MX, true>(c) : launch<OutT, SAMQ_FP4_NV, true>(c);
+    return c.fmt == SAMQ_FP4_MX ? launch<OutT, SAMQ_FP4_MX, false>(c) : launch<OutT, SAMQ_FP4_NV, false>(c);
 }
 
 }  // namespace
