@@ -72,6 +72,23 @@ __device__ __forceinline__ uint32_t staged(int row, uint32_t byte) {
     return (uint32_t)row * 128u + (byte ^ ((uint32_t)(row & 7) << 4));
 }
 
+// gelu_erf of two values in the fewest operations a result: with v = max(-|x|, -6.08), 2^Q(v) = Phi(v) and
+// gelu(x) = max(x, 0) + v * Phi(v).  Q is gelu_erf's polynomial with the odd coefficients' signs turned.
+__device__ __forceinline__ float2 gelu_pair(float2 x) {
+    const float2 v = make_float2(fmaxf(-fabsf(x.x), -6.08f), fmaxf(-fabsf(x.y), -6.08f));
+    float2 q = make_float2(3.586083039e-05f, 3.586083039e-05f);
+    q = __ffma2_rn(q, v, make_float2(7.942179800e-04f, 7.942179800e-04f));
+    q = __ffma2_rn(q, v, make_float2(8.166280575e-03f, 8.166280575e-03f));
+    q = __ffma2_rn(q, v, make_float2(5.355186760e-02f, 5.355186760e-02f));
+    q = __ffma2_rn(q, v, make_float2(-4.586586654e-01f, -4.586586654e-01f));
+    q = __ffma2_rn(q, v, make_float2(1.151242375e+00f, 1.151242375e+00f));
+    q = __ffma2_rn(q, v, make_float2(-9.999881387e-01f, -9.999881387e-01f));
+    float2 h;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h.x) : "f"(q.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h.y) : "f"(q.y));
+    return __ffma2_rn(v, h, make_float2(fmaxf(x.x, 0.f), fmaxf(x.y, 0.f)));
+}
+
 template <typename OutT, bool GELU, bool RES>
 struct EpiWarp {
     static constexpr int PASS_COLS = 128 / (int)sizeof(OutT);       // columns of a staging row: 64, or 32 of fp32
@@ -125,7 +142,7 @@ struct EpiWarp {
             if constexpr (GELU) {
 #pragma unroll
                 for (int j = 0; j < PASS_COLS; j += 2) {
-                    const float2 g = gelu_erf2(make_float2(y[j], y[j + 1]));
+                    const float2 g = gelu_pair(make_float2(y[j], y[j + 1]));
                     y[j] = g.x; y[j + 1] = g.y;
                 }
             }

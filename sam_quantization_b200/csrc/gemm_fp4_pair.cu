@@ -76,6 +76,28 @@ struct PairParams {
     int32_t* status;
 };
 
+// The tiles of a pair in order, without a division per tile.  RESIDENT: consecutive tiles, so that A changes seldom; else
+// the pairs work side by side.
+template <bool RESIDENT>
+struct TileWalk {
+    int n_blocks, left, m, n, step_m, step_n;
+    bool first = true;                            // nothing of the pair's rows has been done before
+    __device__ __forceinline__ TileWalk(int num_tiles, int n_blocks_, int pair, int num_pairs) : n_blocks(n_blocks_) {
+        const int begin = RESIDENT ? (int)((int64_t)num_tiles * pair / num_pairs) : pair;
+        left = RESIDENT ? (int)((int64_t)num_tiles * (pair + 1) / num_pairs) - begin : (num_tiles - pair + num_pairs - 1) / num_pairs;
+        m = begin / n_blocks; n = begin % n_blocks;
+        step_m = RESIDENT ? 0 : num_pairs / n_blocks; step_n = RESIDENT ? 1 : num_pairs % n_blocks;
+    }
+    __device__ __forceinline__ bool more() const { return left > 0; }
+    __device__ __forceinline__ void next() {
+        --left; first = false;
+        m += step_m; n += step_n;
+        if (n >= n_blocks) { n -= n_blocks; ++m; }
+    }
+    __device__ __forceinline__ bool new_rows() const { return first || n == 0; }                  // RESIDENT
+    __device__ __forceinline__ bool rows_done() const { return left > 1 && n == n_blocks - 1; }
+};
+
 template <typename OutT, int FMT, bool GELU, bool RES, bool RESIDENT>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
@@ -102,12 +124,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     const int n_blocks = (p.epi.N + BN - 1) / BN;
     const int k_blocks = (p.K + KPAD - 1) / KPAD;
     const int num_tiles = m_blocks * n_blocks;
-    // RESIDENT: consecutive tiles, so that A changes seldom; else the pairs work side by side
-    const int first_tile = RESIDENT ? (int)((int64_t)num_tiles * pair / num_pairs) : pair;
-    const int end_tile = RESIDENT ? (int)((int64_t)num_tiles * (pair + 1) / num_pairs) : num_tiles;
-    const int tile_step = RESIDENT ? 1 : num_pairs;
-    auto new_rows = [&](int tile) { return tile == first_tile || tile / n_blocks != (tile - 1) / n_blocks; };
-    auto rows_done = [&](int tile) { return tile + 1 < end_tile && (tile + 1) / n_blocks != tile / n_blocks; };
+    TileWalk<RESIDENT> walk(num_tiles, n_blocks, pair, num_pairs);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(smem_u32(&ctl->full[s]), 1); mbar_init(smem_u32(&ctl->empty[s]), 1); }
@@ -133,11 +150,11 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         // ---------------- TMA producer ----------------
         int stage = 0; uint32_t phase = 0, a_phase = 1;
         bool ok = true;
-        for (int tile = first_tile; tile < end_tile && ok; tile += tile_step) {
-            const int mt = (tile / n_blocks) * 2 + (int)rank;              // this CTA's 128-row tile of A
-            const int n0 = (tile % n_blocks) * BN;
+        for (; walk.more() && ok; walk.next()) {
+            const int mt = walk.m * 2 + (int)rank;                         // this CTA's 128-row tile of A
+            const int n0 = walk.n * BN;
             const int nt = n0 / TILE_ROWS;                                 // first of W's two scale tiles
-            const bool load_a = RESIDENT && new_rows(tile);
+            const bool load_a = RESIDENT && walk.new_rows();
             for (int kb = 0; kb < k_blocks; ++kb) {
                 if (load_a) ok = mbar_wait(smem_u32(&ctl->a_empty[kb]), a_phase, abort_flag);
                 ok = ok && mbar_wait(smem_u32(&ctl->empty[stage]), phase ^ 1u, abort_flag);
@@ -181,13 +198,13 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             int acc = 0; uint32_t acc_phase = 0;
             int unit = 0; uint32_t unit_phase = 0, a_phase = 1;
             bool ok = true;
-            for (int tile = first_tile; tile < end_tile && ok; tile += tile_step) {
-                const bool wait_a = RESIDENT && new_rows(tile), free_a = RESIDENT && rows_done(tile);
+            for (; walk.more() && ok; walk.next()) {
+                const bool wait_a = RESIDENT && walk.new_rows(), free_a = RESIDENT && walk.rows_done();
                 if (wait_a) a_phase ^= 1u;
                 if (!mbar_wait(smem_u32(&ctl->acc_empty[acc]), acc_phase ^ 1u, abort_flag)) break;
                 const uint32_t tmem_d = tmem + (uint32_t)(acc * BN);
                 // an odd tile's 192 rows begin in the middle of a scale tile: skip its first 64 rows, two columns
-                const uint32_t sf_shift = (uint32_t)((tile % n_blocks) & 1) * 2u;
+                const uint32_t sf_shift = (uint32_t)(walk.n & 1) * 2u;
                 for (int kb = 0; kb < k_blocks; ++kb) {
                     ok = mbar_wait(smem_u32(&ctl->full[stage]), phase, abort_flag) &&
                          (!wait_a || mbar_wait(smem_u32(&ctl->a_full[kb]), a_phase, abort_flag)) &&
@@ -227,8 +244,8 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             int filled = 0;
             uint32_t a_phase = 1;
             bool ok = true;
-            for (int tile = first_tile; tile < end_tile && ok; tile += tile_step) {
-                const bool wait_a = RESIDENT && new_rows(tile);
+            for (; walk.more() && ok; walk.next()) {
+                const bool wait_a = RESIDENT && walk.new_rows();
                 if (wait_a) a_phase ^= 1u;
                 for (int kb = 0; kb < k_blocks; ++kb) {
                     ok = mbar_wait(smem_u32(&ctl->full[stage]), phase, abort_flag) &&
@@ -268,9 +285,9 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         EpiWarp<OutT, GELU, RES> epi{p.epi, &map_out, &map_res, staging + (size_t)ew * STAGING_BYTES, bias_s + ew * EPI_COLS,
                                      smem_u32(&ctl->res[ew]), 0u, abort_flag, lane};
         int acc = 0; uint32_t acc_phase = 0;
-        for (int tile = first_tile; tile < end_tile; tile += tile_step) {
-            const int row0 = (tile / n_blocks) * (2 * BM) + (int)rank * BM + quad * 32;
-            const int col0 = (tile % n_blocks) * BN + cg * EPI_COLS;
+        for (; walk.more(); walk.next()) {
+            const int row0 = walk.m * (2 * BM) + (int)rank * BM + quad * 32;
+            const int col0 = walk.n * BN + cg * EPI_COLS;
             epi.before(row0, col0);
             if (!mbar_wait(smem_u32(&ctl->acc_full[acc]), acc_phase, abort_flag)) break;
             tcgen05_fence_after();
@@ -278,7 +295,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             tmem_ld64(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN + cg * EPI_COLS), r);
             tcgen05_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&ctl->acc_empty[acc]), 0));
+            if (lane == 0) mbar_arrive_remote(map_to_cta(smem_u32(&ctl->acc_empty[acc]), 0));
             if (!epi.finish(row0, col0, r)) break;
             if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
         }
