@@ -4,9 +4,11 @@
 // Few rows leave the output too small for the device, and the weight's bytes and the latency of one pass are what counts.
 // So the operands change places: 128 rows of W are the M side of the MMA, the T <= 128 rows of the activation its N side
 // (T a multiple of 8: one token costs an eighth of an N = 64 MMA), and a cluster of S CTAs splits K, each CTA with its
-// own range of 256-column blocks and all of its loads in flight at once.  The S partial tiles meet in distributed shared
-// memory: after a cluster barrier every CTA sums a share of the rows over the S copies in rank order (the result does
-// not depend on timing), finishes them and stores them.
+// own range of 256-column blocks and all of its loads in flight at once.  The S partial tiles are joined by rows: a CTA
+// owns a share of them; every CTA pushes its sums of a row into the owner's shared memory (st.async, counted by the
+// owner's barrier), and the owner adds the S copies in rank order (the result does not depend on timing), finishes
+// the row and stores it.  Nothing waits for the whole cluster but the first push, for a barrier that all have passed at
+// their start; pulling the sums after a cluster barrier and a second one before the exit took 4000 of 7400 clocks.
 //
 // samq_linear_fp4 also quantizes here: the four epilogue warps round the CTA's K range of the activation to codes and
 // scales straight into the shared-memory layout that the MMA reads, which saves a launch and the trip through memory.
@@ -21,18 +23,19 @@ namespace {
 
 constexpr int BW = 128;                          // rows of W of a CTA
 constexpr int MAX_T = 128;                       // rows of the activation of a CTA
-constexpr int STAGES = 4;
-constexpr int MAX_SPLIT = 8;
+constexpr int MIN_STAGES = 3, MAX_STAGES = 8;    // as many as leave room for two CTAs on an SM
+constexpr int MAX_SPLIT = 8;                    // the portable cluster size
 constexpr int W_BYTES = BW * BK;
-constexpr int EPI_WARPS = 4;
+constexpr int EPI_WARPS = 8;                     // two for each quarter of the 128 columns, taking turns by 16 rows
 constexpr int EPI_THREADS = EPI_WARPS * 32;
 constexpr int THREADS = 64 + EPI_THREADS;
 constexpr int FUSED_MAX_ROWS = SAMQ_LINEAR_FP4_MAX_ROWS;
 
 struct __align__(8) Control {
-    uint64_t full[STAGES];
-    uint64_t empty[STAGES];
+    uint64_t full[MAX_STAGES];
+    uint64_t empty[MAX_STAGES];
     uint64_t acc_full;
+    uint64_t joined;                              // the sums of this CTA's rows have arrived from every CTA
     uint32_t tmem_base;
     uint32_t abort_flag;
 };
@@ -40,6 +43,7 @@ struct __align__(8) Control {
 struct SmallParams {
     int M, N, K;
     int T;                                        // rows of the activation in a tile, a multiple of 8
+    int stages;
     int groups;
     const uint8_t* a_scales;                      // unless the kernel quantizes
     const uint8_t* w_scales;
@@ -60,8 +64,19 @@ template <int FMT> struct Shape {
 };
 template <int FMT>
 __host__ __device__ constexpr int stage_bytes(int T) { return W_BYTES + T * BK; }
+// rows of a tile that one of `split` CTAs owns, at most
+__host__ __device__ inline int owned_rows(int rows, int split) { return (rows + split - 1) / split; }
+constexpr size_t HALF_SM = 112 * 1024;           // shared memory of one of two CTAs on an SM
 template <int FMT>
-size_t smem_bytes(int T) { return 1024 + (size_t)STAGES * (stage_bytes<FMT>(T) + 2 * Shape<FMT>::SF_BYTES) + sizeof(Control); }
+int stages_of(int T) {
+    const int n = (int)((HALF_SM - 2048) / (stage_bytes<FMT>(T) + 2 * Shape<FMT>::SF_BYTES));
+    return n < MIN_STAGES ? MIN_STAGES : n > MAX_STAGES ? MAX_STAGES : n;
+}
+template <int FMT>
+size_t smem_bytes(int T, int stages, int split) {
+    return 1024 + (size_t)stages * (stage_bytes<FMT>(T) + 2 * Shape<FMT>::SF_BYTES) +
+           (split > 1 ? (size_t)split * owned_rows(T, split) * BW * sizeof(float) : 0) + sizeof(Control);
+}
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -72,15 +87,89 @@ __device__ __forceinline__ uint32_t cluster_nctas() {
     asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
     return r;
 }
-__device__ __forceinline__ float ld_cluster(uint32_t cluster_addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
-    return v;
+// one value into another CTA's shared memory, counted by a barrier there
+__device__ __forceinline__ void push_async(uint32_t cluster_addr, float v, uint32_t cluster_bar) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];"
+                 ::"r"(cluster_addr), "r"(__float_as_uint(v)), "r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr));
+    tmem_ld_wait();
+}
+
+// 16 neighbouring rows of output column n from row m on, `count` of them: the sums in y
+template <typename OutT>
+__device__ __forceinline__ void finish_rows(const SmallParams& p, int n, float bias, int64_t m, int count, float (&y)[16]) {
+    OutT* out = static_cast<OutT*>(p.out) + m * p.ldo + n;
+    const OutT* res = static_cast<const OutT*>(p.residual) + m * p.ldr + n;
+    const bool all = count >= 16;                                   // the same in all threads, as the other branches here
+#pragma unroll
+    for (int j = 0; j < 16; ++j) y[j] = fmaf(y[j], p.alpha, bias);
+    if (p.gelu) {
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+            const float2 g = gelu_pair(make_float2(y[j], y[j + 1]));
+            y[j] = g.x; y[j + 1] = g.y;
+        }
+    }
+    if (p.residual != nullptr) {
+        OutT r[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (all || j < count) { r[j] = *res; res += p.ldr; }
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (all || j < count) y[j] += OutOps<OutT>::up(r[j]);
+    }
+    if (all) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) { *out = OutOps<OutT>::down(y[j]); out += p.ldo; }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (j < count) { *out = OutOps<OutT>::down(y[j]); out += p.ldo; }
+    }
+}
+
+// `blocks` k-blocks of the activation from kb on, into the operand layout (128-byte swizzle) and scale tiles of as many
+// stages; rows behind M are zero.  A thread takes every EPI_THREADS-th chunk of 16 columns, four of them loaded together.
+template <typename T, int FMT>
+__device__ __forceinline__ void quantize_blocks(const SmallParams& p, int m0, int kb, int blocks, int tid, uint8_t* codes, int codes_pitch,
+                                                uint8_t* scales, int scales_pitch) {
+    constexpr int CHUNKS = KPAD / 16;                               // of a row and block
+    const int per_block = p.T * CHUNKS, total = per_block * blocks;
+    for (int c0 = tid; c0 < total; c0 += 4 * EPI_THREADS) {         // (whole warps: per_block is a multiple of 128)
+        Chunk<T> x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int c = c0 + u * EPI_THREADS;
+            if (c >= total) break;
+            const int b = c / per_block, r = c % per_block / CHUNKS, col = (kb + b) * KPAD + c % CHUNKS * 16;
+            load_chunk(x[u], static_cast<const T*>(p.x) + (int64_t)(m0 + r) * p.ldx + col, m0 + r < p.M ? min(16, p.K - col) : 0, p.access_x);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int c = c0 + u * EPI_THREADS;
+            if (c >= total) break;
+            const int b = c / per_block, r = c % per_block / CHUNKS, j = c % CHUNKS;
+            uint32_t amax = x[u].amax_bits();
+            if constexpr (FMT == SAMQ_FP4_MX) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            const Scale sc = block_scale<FMT>(amax, 1.0f, 1.0f);
+            *reinterpret_cast<uint2*>(codes + b * codes_pitch + staged(r, j * 8)) = encode_chunk<FMT>(x[u], sc, amax < 0x7F800000u);
+            const int block = j * 16 / block_of(FMT);
+            if (FMT == SAMQ_FP4_NV || (j & 1) == 0)
+                scales[b * scales_pitch + (block / 4) * TILE_BYTES + r * 16 + (block & 3)] =
+                    (uint8_t)((kb + b) * KPAD + block * block_of(FMT) < p.K ? sc.byte : 0u);
+        }
+    }
+    fence_async_smem();
 }
 
 // QUANT: the activation is `x` of type OutT, quantized here; otherwise codes and scales are loaded.
 template <typename OutT, int FMT, bool QUANT>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 2)
 gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const SmallParams p)
 {
     using S = Shape<FMT>;
@@ -88,52 +177,67 @@ gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     const uint32_t raw_addr = smem_u32(smem_raw);
     uint8_t* tiles = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
     const int st_bytes = stage_bytes<FMT>(p.T);
-    uint8_t* sf = tiles + (size_t)STAGES * st_bytes;
-    Control* ctl = reinterpret_cast<Control*>(sf + (size_t)STAGES * 2 * S::SF_BYTES);
-    float* partial = reinterpret_cast<float*>(tiles);                   // [T][128], once the stages are done with
+    const int stages = p.stages;
+    uint8_t* sf = tiles + (size_t)stages * st_bytes;
+    const int split = (int)cluster_nctas(), rank = (int)cluster_ctarank();
+    float* joined = reinterpret_cast<float*>(sf + (size_t)stages * 2 * S::SF_BYTES);     // [split][own_max][128]
+    Control* ctl = reinterpret_cast<Control*>(joined + (split > 1 ? split * owned_rows(p.T, split) * BW : 0));
     volatile uint32_t* abort_flag = &ctl->abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int split = (int)cluster_nctas(), rank = (int)cluster_ctarank();
     const int nt = blockIdx.x / split, mt = blockIdx.y;
     const int n0 = nt * BW, m0 = mt * MAX_T;
     const int k_blocks = (p.K + KPAD - 1) / KPAD;
     const int kb_first = rank * (k_blocks / split) + min(rank, k_blocks % split);
     const int kb_count = k_blocks / split + (rank < k_blocks % split ? 1 : 0);
 
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) { mbar_init(smem_u32(&ctl->full[s]), QUANT ? 1 + EPI_THREADS : 1); mbar_init(smem_u32(&ctl->empty[s]), 1); }
-        mbar_init(smem_u32(&ctl->acc_full), 1);
-        ctl->abort_flag = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (warp == 1) {
+    auto load_stage = [&](int i) {                                  // by one thread
+        const int s = i % stages, kb = kb_first + i;
+        const uint32_t bar = smem_u32(&ctl->full[s]);
+        const uint32_t sw = smem_u32(tiles + (size_t)s * st_bytes), ss = smem_u32(sf + (size_t)s * 2 * S::SF_BYTES);
+        mbar_expect_tx(bar, W_BYTES + S::SF_BYTES + (QUANT ? 0 : p.T * BK + S::SF_BYTES));
+        tma_load_2d(sw, &map_w, bar, kb * BK, n0);
+        bulk_load(ss, p.w_scales + ((int64_t)nt * p.groups + kb * S::GROUPS) * TILE_BYTES, S::SF_BYTES, bar);
+        if constexpr (!QUANT) {
+            tma_load_2d(sw + W_BYTES, &map_a, bar, kb * BK, m0);
+            bulk_load(ss + S::SF_BYTES, p.a_scales + ((int64_t)mt * p.groups + kb * S::GROUPS) * TILE_BYTES, S::SF_BYTES, bar);
+        }
+    };
+    const int rows = min(p.T, p.M - m0);
+    const int own_max = owned_rows(rows, split);
+    const int owned = max(0, min(own_max, rows - rank * own_max));  // rows of this CTA, from rank * own_max on
+
+    // The set-up of the roles runs side by side: the first warp makes the barriers and sends the first loads off, the
+    // second allocates tensor memory, the others quantize as many blocks as there are stages.
+    if (warp == 0) {
+        if (elect_one()) {
+            for (int s = 0; s < stages; ++s) { mbar_init(smem_u32(&ctl->full[s]), QUANT ? 1 + EPI_THREADS : 1); mbar_init(smem_u32(&ctl->empty[s]), 1); }
+            mbar_init(smem_u32(&ctl->acc_full), 1);
+            mbar_init(smem_u32(&ctl->joined), 1);
+            ctl->abort_flag = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            if (split > 1) mbar_expect_tx(smem_u32(&ctl->joined), (uint32_t)(split * owned * BW) * 4u);
+            for (int i = 0; i < min(kb_count, stages); ++i) load_stage(i);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32(&ctl->tmem_base)), "r"((uint32_t)p.tmem_cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else if constexpr (QUANT) {
+        quantize_blocks<OutT, FMT>(p, m0, kb_first, min(kb_count, stages), threadIdx.x - 64, tiles + W_BYTES, st_bytes, sf + S::SF_BYTES, 2 * S::SF_BYTES);
     }
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
+    if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");    // this CTA's barriers exist
     const uint32_t tmem = ctl->tmem_base;
 
     if (warp == 0) {
         bool ok = true;
-        for (int i = 0; i < kb_count; ++i) {
-            const int s = i % STAGES, kb = kb_first + i;
-            ok = mbar_wait(smem_u32(&ctl->empty[s]), ((i / STAGES) & 1) ^ 1u, abort_flag);
+        for (int i = stages; i < kb_count; ++i) {
+            ok = mbar_wait(smem_u32(&ctl->empty[i % stages]), ((i / stages) & 1) ^ 1u, abort_flag);
             if (!ok) break;
-            if (elect_one()) {
-                const uint32_t bar = smem_u32(&ctl->full[s]);
-                const uint32_t sw = smem_u32(tiles + (size_t)s * st_bytes);
-                const uint32_t ss = smem_u32(sf + (size_t)s * 2 * S::SF_BYTES);
-                mbar_expect_tx(bar, W_BYTES + S::SF_BYTES + (QUANT ? 0 : p.T * BK + S::SF_BYTES));
-                tma_load_2d(sw, &map_w, bar, kb * BK, n0);
-                bulk_load(ss, p.w_scales + ((int64_t)nt * p.groups + kb * S::GROUPS) * TILE_BYTES, S::SF_BYTES, bar);
-                if constexpr (!QUANT) {
-                    tma_load_2d(sw + W_BYTES, &map_a, bar, kb * BK, m0);
-                    bulk_load(ss + S::SF_BYTES, p.a_scales + ((int64_t)mt * p.groups + kb * S::GROUPS) * TILE_BYTES, S::SF_BYTES, bar);
-                }
-            }
+            if (elect_one()) load_stage(i);
             __syncwarp();
         }
         if (!ok) {
@@ -144,8 +248,8 @@ gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         bool ok = true;
         const uint32_t idesc_n = (uint32_t)p.T;
         for (int i = 0; i < kb_count; ++i) {
-            const int s = i % STAGES;
-            ok = mbar_wait(smem_u32(&ctl->full[s]), (i / STAGES) & 1, abort_flag);
+            const int s = i % stages;
+            ok = mbar_wait(smem_u32(&ctl->full[s]), (i / stages) & 1, abort_flag);
             if (!ok) break;
             tcgen05_fence_after();
             const uint32_t sw = smem_u32(tiles + (size_t)s * st_bytes);
@@ -173,45 +277,70 @@ gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
             __syncwarp();
         }
     } else {
-        const int quad = warp & 3;
         if constexpr (QUANT) {
-            // the CTA's columns of the activation, 16 a thread and step, into the operand layout (128-byte swizzle) and its
-            // scale tile; rows behind M are zero
-            constexpr int CHUNKS = KPAD / 16;                       // of a row and stage
-            const int tid = threadIdx.x - 64;
             bool ok = true;
             for (int i = 0; i < kb_count && ok; ++i) {
-                const int s = i % STAGES, kb = kb_first + i;
-                ok = mbar_wait(smem_u32(&ctl->empty[s]), ((i / STAGES) & 1) ^ 1u, abort_flag);
-                if (!ok) break;
-                uint8_t* codes = tiles + (size_t)s * st_bytes + W_BYTES;
-                uint8_t* scales = sf + (size_t)s * 2 * S::SF_BYTES + S::SF_BYTES;
-                for (int c = tid; c < p.T * CHUNKS; c += EPI_THREADS) {
-                    const int r = c / CHUNKS, j = c % CHUNKS, col = kb * KPAD + j * 16;
-                    Chunk<OutT> x;
-                    load_chunk(x, static_cast<const OutT*>(p.x) + (int64_t)(m0 + r) * p.ldx + col, m0 + r < p.M ? min(16, p.K - col) : 0, p.access_x);
-                    uint32_t amax = x.amax_bits();
-                    if constexpr (FMT == SAMQ_FP4_MX) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                    const Scale sc = block_scale<FMT>(amax, 1.0f, 1.0f);
-                    *reinterpret_cast<uint2*>(codes + staged(r, j * 8)) = encode_chunk<FMT>(x, sc, amax < 0x7F800000u);
-                    const int block = j * 16 / block_of(FMT);
-                    if (FMT == SAMQ_FP4_NV || (j & 1) == 0)
-                        scales[(block / 4) * TILE_BYTES + r * 16 + (block & 3)] = (uint8_t)(kb * KPAD + block * block_of(FMT) < p.K ? sc.byte : 0u);
+                const int s = i % stages;
+                if (i >= stages) {
+                    ok = mbar_wait(smem_u32(&ctl->empty[s]), ((i / stages) & 1) ^ 1u, abort_flag);
+                    if (ok) quantize_blocks<OutT, FMT>(p, m0, kb_first + i, 1, threadIdx.x - 64, tiles + (size_t)s * st_bytes + W_BYTES, st_bytes,
+                                                       sf + (size_t)s * 2 * S::SF_BYTES + S::SF_BYTES, 2 * S::SF_BYTES);
                 }
-                fence_async_smem();
                 mbar_arrive(smem_u32(&ctl->full[s]));
             }
         }
+    }
+    // all warps: the others' first pushes may come once every CTA of the cluster has made its barriers
+    __syncwarp();
+    if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (warp >= 2) {
+        const int col = (warp & 3) * 32 + lane, n = n0 + col;
+        const uint32_t acc = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const float bias = (p.bias != nullptr && n < p.N) ? OutOps<OutT>::up(static_cast<const OutT*>(p.bias)[n]) : 0.0f;
         if (mbar_wait(smem_u32(&ctl->acc_full), 0, abort_flag)) {
             tcgen05_fence_after();
-            for (int c = 0; c < p.T; c += 8) {
-                uint32_t r[8];
-                asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                             : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                             : "r"(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)c));
-                tmem_ld_wait();
+            const int turn = 16 * ((warp - 2) >> 2);                // this warp's rows: every second sixteen
+            if (split == 1) {
+                for (int c = turn; c < rows; c += 32) {
+                    uint32_t r[16];
+                    tmem_ld16(acc + (uint32_t)c, r);
+                    float y[16];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) partial[(c + j) * BW + quad * 32 + lane] = __uint_as_float(r[j]);
+                    for (int j = 0; j < 16; ++j) y[j] = __uint_as_float(r[j]);
+                    if (n < p.N) finish_rows<OutT>(p, n, bias, m0 + c, rows - c, y);
+                }
+            } else {
+                const uint32_t bar = smem_u32(&ctl->joined);
+                const uint32_t to = smem_u32(joined + rank * own_max * BW + col);
+                for (int c = turn; c < rows; c += 32) {
+                    uint32_t r[16];
+                    tmem_ld16(acc + (uint32_t)c, r);
+                    int owner = c / own_max, k = c % own_max;
+                    uint32_t at = map_to_cta(to + (uint32_t)(k * BW) * 4u, (uint32_t)owner), at_bar = map_to_cta(bar, (uint32_t)owner);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        if (c + j >= rows) break;
+                        push_async(at, __uint_as_float(r[j]), at_bar);
+                        at += BW * 4u;
+                        if (++k == own_max && c + j + 1 < rows) {
+                            k = 0; ++owner;
+                            at = map_to_cta(to, (uint32_t)owner); at_bar = map_to_cta(bar, (uint32_t)owner);
+                        }
+                    }
+                }
+                if (turn < owned && mbar_wait_cluster(bar, 0, abort_flag) && n < p.N) {
+                    for (int k = turn; k < owned; k += 32) {
+                        const float* from = joined + k * BW + col;
+                        float y[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) y[j] = 0.0f;
+                        for (int q = 0; q < split; ++q, from += own_max * BW) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) if (k + j < owned) y[j] += from[j * BW];
+                        }
+                        finish_rows<OutT>(p, n, bias, m0 + rank * own_max + k, owned - k, y);
+                    }
+                }
             }
         }
         tcgen05_fence_before();
@@ -222,51 +351,33 @@ gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         __syncwarp();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)p.tmem_cols) : "memory");
     }
-    if (split > 1) cluster_sync();                                  // every CTA's partial sums are in its shared memory
-    if (warp >= 2) {
-        const int col = (warp & 3) * 32 + lane, n = n0 + col;
-        if (n < p.N) {
-            const float bias = p.bias != nullptr ? OutOps<OutT>::up(static_cast<const OutT*>(p.bias)[n]) : 0.0f;
-            const uint32_t base = smem_u32(partial);
-            const int rows = min(p.T, p.M - m0);
-            for (int r = rank; r < rows; r += split) {              // the ranks share the rows
-                float v[MAX_SPLIT];
-#pragma unroll
-                for (int q = 0; q < MAX_SPLIT; ++q)
-                    v[q] = q < split ? ld_cluster(map_to_cta(base + (uint32_t)(r * BW + col) * 4u, (uint32_t)q)) : 0.0f;
-                float y = v[0];
-#pragma unroll
-                for (int q = 1; q < MAX_SPLIT; ++q) y += v[q];
-                y = fmaf(y, p.alpha, bias);
-                if (p.gelu) y = gelu_erf(y);
-                const int64_t m = m0 + r;
-                if (p.residual != nullptr) y += OutOps<OutT>::up(static_cast<const OutT*>(p.residual)[m * p.ldr + n]);
-                static_cast<OutT*>(p.out)[m * p.ldo + n] = OutOps<OutT>::down(y);
-            }
-        }
-    }
     if (threadIdx.x == 0 && ctl->abort_flag != 0 && p.status != nullptr) atomicExch(p.status, 1);
+    // A CTA has its rows once every other has pushed them, and nobody reads or writes its memory after that; one that gave
+    // up stays until the others have left or given up too.
     __syncwarp();
-    if (split > 1) cluster_sync();                                  // nobody reads a retired CTA's shared memory
+    if (split > 1 && *abort_flag != 0) cluster_sync();
 }
 
 template <typename OutT, int FMT, bool QUANT>
 int launch_small(const Fp4Call& c, SmallParams& p, const CUtensorMap& ma, const CUtensorMap& mw) {
     auto kernel = gemm_fp4_small_kernel<OutT, FMT, QUANT>;
-    // the largest tile's shared memory, set once per device
+    // as much shared memory as the largest tile takes, set once per device
+    constexpr size_t SMEM_MOST = 227 * 1024;
     static thread_local bool ready[64] = {false};
     int dev = 0;
     SAMQ_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !ready[dev]) {
-        SAMQ_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<FMT>(MAX_T)));
+        SAMQ_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_MOST));
         if (dev >= 0 && dev < 64) ready[dev] = true;
     }
     const int64_t n_tiles = (c.N + BW - 1) / BW, m_tiles = (c.M + MAX_T - 1) / MAX_T;
     const int64_t k_blocks = (c.K + KPAD - 1) / KPAD;
-    // split K until about two small CTAs or one large one sit on every SM
+    // Split K while SMs are idle, but leave a CTA four blocks of 256 columns at least: joining two halves costs about as
+    // much as two more blocks (one token, 1280 -> 3840: 6.2 us whole, 6.6 us in two; 5120 -> 1280: 16.4 and 8.2 in five).
     const int64_t room = (p.T <= 32 ? 2 : 1) * sm_count() / (n_tiles * m_tiles);
-    int split = (int)(room < 1 ? 1 : room > MAX_SPLIT ? MAX_SPLIT : room);
-    if (split > k_blocks) split = (int)k_blocks;
+    int64_t most = k_blocks / 4 < room ? k_blocks / 4 : room;
+    const int split = (int)(most < 1 ? 1 : most > MAX_SPLIT ? MAX_SPLIT : most);
+    p.stages = stages_of<FMT>(p.T);
     if (n_tiles * split > 2147483647LL || m_tiles > 65535) return fail(SAMQ_ERR_TOO_LARGE, "product of %lld x %lld outputs is too large", (long long)c.M, (long long)c.N);
     const int cols = p.T + 2 * Shape<FMT>::SF_COLS;
     p.tmem_cols = cols <= 64 ? 64 : cols <= 128 ? 128 : 256;
@@ -276,8 +387,10 @@ int launch_small(const Fp4Call& c, SmallParams& p, const CUtensorMap& ma, const 
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3((unsigned)(n_tiles * split), (unsigned)m_tiles);
-    cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = smem_bytes<FMT>(p.T); cfg.stream = c.stream;
+    cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = smem_bytes<FMT>(p.T, p.stages, split); cfg.stream = c.stream;
     cfg.attrs = attr; cfg.numAttrs = 1;
+    static_assert(1024 + MIN_STAGES * (stage_bytes<FMT>(MAX_T) + 2 * Shape<FMT>::SF_BYTES) + (MAX_T + MAX_SPLIT) * BW * 4 + sizeof(Control) <= SMEM_MOST &&
+                  HALF_SM + (MAX_T + MAX_SPLIT) * BW * 4 + sizeof(Control) <= SMEM_MOST, "the largest tiles and their joined rows");
     SAMQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, ma, mw, p));
     return SAMQ_OK;
 }

@@ -144,6 +144,22 @@ __device__ __forceinline__ void tcgen05_commit_pair(uint32_t cluster_bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(cluster_bar) : "memory");
 }
 
+// Bounded wait (see mbar_wait) for data that other CTAs of the cluster have written.
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
+    const long long t0 = clock64();
+    for (uint32_t spins = 1;; ++spins) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\t"
+                     "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+                     "selp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+        if ((spins & 255u) == 0) {
+            if (*abort_flag != 0) return false;
+            if (clock64() - t0 > WAIT_LIMIT_CYCLES) { *abort_flag = 1; return false; }
+        }
+    }
+}
 // An arrival in another CTA that orders only what this thread itself has completed (release at CTA scope): enough to hand
 // back tensor memory whose loads have been waited for, and without the flush that release at cluster scope costs (1700
 // clocks behind global stores).
