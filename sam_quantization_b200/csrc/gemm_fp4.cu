@@ -133,38 +133,42 @@ __device__ __forceinline__ void finish_rows(const SmallParams& p, int n, float b
     }
 }
 
-// `blocks` k-blocks of the activation from kb on, into the operand layout (128-byte swizzle) and scale tiles of as many
-// stages; rows behind M are zero.  A thread takes every EPI_THREADS-th chunk of 16 columns, four of them loaded together.
-template <typename T, int FMT>
-__device__ __forceinline__ void quantize_blocks(const SmallParams& p, int m0, int kb, int blocks, int tid, uint8_t* codes, int codes_pitch,
-                                                uint8_t* scales, int scales_pitch) {
-    constexpr int CHUNKS = KPAD / 16;                               // of a row and block
-    const int per_block = p.T * CHUNKS, total = per_block * blocks;
-    for (int c0 = tid; c0 < total; c0 += 4 * EPI_THREADS) {         // (whole warps: per_block is a multiple of 128)
-        Chunk<T> x[4];
+// Quantization of `blocks` k-blocks of the activation from kb on, into the operand layout (128-byte swizzle) and scale
+// tiles of as many stages of the ring from `stage` on; rows behind M are zero.  A thread takes every EPI_THREADS-th chunk
+// of 16 columns, BATCH of them at a time: the loads of a batch are under way together, and may be while a stage is waited
+// for.  (A block has T * 16 chunks, a multiple of 128: whole warps leave the loops together.)
+constexpr int BATCH = 4;
+constexpr int CHUNKS = KPAD / 16;                // of a row and block
+
+template <typename T>
+__device__ __forceinline__ void load_batch(const SmallParams& p, int m0, int kb, int blocks, int first, Chunk<T> (&x)[BATCH]) {
+    const int per_block = p.T * CHUNKS;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int c = c0 + u * EPI_THREADS;
-            if (c >= total) break;
-            const int b = c / per_block, r = c % per_block / CHUNKS, col = (kb + b) * KPAD + c % CHUNKS * 16;
-            load_chunk(x[u], static_cast<const T*>(p.x) + (int64_t)(m0 + r) * p.ldx + col, m0 + r < p.M ? min(16, p.K - col) : 0, p.access_x);
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int c = c0 + u * EPI_THREADS;
-            if (c >= total) break;
-            const int b = c / per_block, r = c % per_block / CHUNKS, j = c % CHUNKS;
-            uint32_t amax = x[u].amax_bits();
-            if constexpr (FMT == SAMQ_FP4_MX) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            const Scale sc = block_scale<FMT>(amax, 1.0f, 1.0f);
-            *reinterpret_cast<uint2*>(codes + b * codes_pitch + staged(r, j * 8)) = encode_chunk<FMT>(x[u], sc, amax < 0x7F800000u);
-            const int block = j * 16 / block_of(FMT);
-            if (FMT == SAMQ_FP4_NV || (j & 1) == 0)
-                scales[b * scales_pitch + (block / 4) * TILE_BYTES + r * 16 + (block & 3)] =
-                    (uint8_t)((kb + b) * KPAD + block * block_of(FMT) < p.K ? sc.byte : 0u);
-        }
+    for (int u = 0; u < BATCH; ++u) {
+        const int c = first + u * EPI_THREADS;
+        if (c >= per_block * blocks) break;
+        const int b = c / per_block, r = c % per_block / CHUNKS, col = (kb + b) * KPAD + c % CHUNKS * 16;
+        load_chunk(x[u], static_cast<const T*>(p.x) + (int64_t)(m0 + r) * p.ldx + col, m0 + r < p.M ? min(16, p.K - col) : 0, p.access_x);
     }
-    fence_async_smem();
+}
+template <typename T, int FMT>
+__device__ __forceinline__ void quantize_batch(const SmallParams& p, int kb, int blocks, int first, int stage, const Chunk<T> (&x)[BATCH],
+                                               uint8_t* tiles, int st_bytes, uint8_t* sf) {
+    const int per_block = p.T * CHUNKS;
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+        const int c = first + u * EPI_THREADS;
+        if (c >= per_block * blocks) break;
+        const int b = c / per_block, r = c % per_block / CHUNKS, j = c % CHUNKS, s = (stage + b) % p.stages;
+        uint32_t amax = x[u].amax_bits();
+        if constexpr (FMT == SAMQ_FP4_MX) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        const Scale sc = block_scale<FMT>(amax, 1.0f, 1.0f);
+        *reinterpret_cast<uint2*>(tiles + (size_t)s * st_bytes + W_BYTES + staged(r, j * 8)) = encode_chunk<FMT>(x[u], sc, amax < 0x7F800000u);
+        const int block = j * 16 / block_of(FMT);
+        if (FMT == SAMQ_FP4_NV || (j & 1) == 0)
+            sf[(size_t)(2 * s + 1) * Shape<FMT>::SF_BYTES + (block / 4) * TILE_BYTES + r * 16 + (block & 3)] =
+                (uint8_t)((kb + b) * KPAD + block * block_of(FMT) < p.K ? sc.byte : 0u);
+    }
 }
 
 // QUANT: the activation is `x` of type OutT, quantized here; otherwise codes and scales are loaded.
@@ -224,7 +228,13 @@ gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                      ::"r"(smem_u32(&ctl->tmem_base)), "r"((uint32_t)p.tmem_cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     } else if constexpr (QUANT) {
-        quantize_blocks<OutT, FMT>(p, m0, kb_first, min(kb_count, stages), threadIdx.x - 64, tiles + W_BYTES, st_bytes, sf + S::SF_BYTES, 2 * S::SF_BYTES);
+        const int tid = threadIdx.x - 64, blocks = min(kb_count, stages);
+        for (int c = tid; c < blocks * p.T * CHUNKS; c += BATCH * EPI_THREADS) {
+            Chunk<OutT> x[BATCH];
+            load_batch(p, m0, kb_first, blocks, c, x);
+            quantize_batch<OutT, FMT>(p, kb_first, blocks, c, 0, x, tiles, st_bytes, sf);
+        }
+        fence_async_smem();
     }
     tcgen05_fence_before();
     __syncthreads();
@@ -278,15 +288,20 @@ gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         }
     } else {
         if constexpr (QUANT) {
+            const int tid = threadIdx.x - 64;
+            for (int i = 0; i < min(kb_count, stages); ++i) mbar_arrive(smem_u32(&ctl->full[i]));
+            // the others a few blocks at a time: half of the ring, and no more than one batch
+            const int group = max(1, min(stages / 2, BATCH * EPI_THREADS / (p.T * CHUNKS)));
             bool ok = true;
-            for (int i = 0; i < kb_count && ok; ++i) {
-                const int s = i % stages;
-                if (i >= stages) {
-                    ok = mbar_wait(smem_u32(&ctl->empty[s]), ((i / stages) & 1) ^ 1u, abort_flag);
-                    if (ok) quantize_blocks<OutT, FMT>(p, m0, kb_first + i, 1, threadIdx.x - 64, tiles + (size_t)s * st_bytes + W_BYTES, st_bytes,
-                                                       sf + (size_t)s * 2 * S::SF_BYTES + S::SF_BYTES, 2 * S::SF_BYTES);
-                }
-                mbar_arrive(smem_u32(&ctl->full[s]));
+            for (int i = stages; i < kb_count && ok; i += group) {
+                const int blocks = min(group, kb_count - i);
+                Chunk<OutT> x[BATCH];
+                load_batch(p, m0, kb_first + i, blocks, tid, x);
+                for (int k = i; k < i + blocks && ok; ++k) ok = mbar_wait(smem_u32(&ctl->empty[k % stages]), ((k / stages) & 1) ^ 1u, abort_flag);
+                if (!ok) break;
+                quantize_batch<OutT, FMT>(p, kb_first + i, blocks, tid, i % stages, x, tiles, st_bytes, sf);
+                fence_async_smem();
+                for (int k = i; k < i + blocks; ++k) mbar_arrive(smem_u32(&ctl->full[k % stages]));
             }
         }
     }
