@@ -218,6 +218,21 @@ class W8A8Linear(nn.Module):
             y = self.output_quant(y)
         return y
 
+    @torch.no_grad()
+    def forward_rms_norm(self, x, norm_weight, eps=1e-6, residual=None, residual_out=None, activation=None, out_dtype=None):
+        """The layer behind an RMS norm of ``x`` (or of ``x + residual``), both in the activation quantizer's one pass.
+        Returns ``(y, h)``, ``h`` the new residual stream ``x + residual`` (``x`` itself without a residual).  Needs
+        per-token activations and no transform of the activation."""
+        if self.act_quant_name != "per_token" or self.smooth_divisor is not None or self.hadamard is not None:
+            raise ValueError("forward_rms_norm needs act_quant=per_token without a SmoothQuant divisor or a Hadamard transform")
+        xa = ops.rms_norm_quantize(x, norm_weight, eps, residual=residual, residual_out=residual_out, n_bits=self.n_bits)
+        y = ops.gemm_i8(xa["q"], self.qweight, xa["scale"], self.w_scale, ops.GRAN_ROW, ops.WEIGHT_GRANULARITY[self.weight_quant_name],
+                        self.group_size or 0, bias=self.bias, activation=ACT_GELU if activation == "gelu" else ACT_NONE,
+                        out_dtype=out_dtype or x.dtype)
+        if self.quantize_output:
+            y = self.output_quant(y)
+        return y, xa.get("residual", x)
+
     def can_fuse_prologue(self) -> bool:
         """True when LayerNorm / row gather may be folded into this layer's quantization kernel
         (per-token and per-group activations; a per-tensor scale needs a separate reduction)."""
