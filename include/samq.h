@@ -321,12 +321,16 @@ int samq_gemm_fp4(const uint8_t* A, int64_t lda, const uint8_t* a_scales, const 
                   int64_t M, int64_t N, int64_t K, int format, float alpha, const void* bias, const void* residual, int64_t ldr,
                   int activation, void* out, int out_dtype, int64_t ldo, int32_t* status, void* stream);
 
-/* A 4-bit linear layer for a few rows in one kernel: x [M, K] of `dtype` (M <= SAMQ_LINEAR_FP4_MAX_ROWS) is quantized as
- * samq_quant_fp4 does with global_scale 1 and multiplied as in samq_gemm_fp4; out, bias and residual are of `dtype` too. */
-#define SAMQ_LINEAR_FP4_MAX_ROWS 32
+/* A 4-bit linear layer: x [M, K] of `dtype`, row stride ldx, is quantized as samq_quant_fp4 does with global_scale 1 and
+ * multiplied as in samq_gemm_fp4.  Up to SAMQ_LINEAR_FP4_ONE_KERNEL_ROWS rows with dtype == out_dtype it is one kernel and
+ * takes no workspace (it may be NULL); otherwise the quantized activation lives in `workspace`, 16-byte aligned and of
+ * samq_linear_fp4_workspace_bytes() at least, until the call's work on the stream is done. */
+#define SAMQ_LINEAR_FP4_ONE_KERNEL_ROWS 32
+size_t samq_linear_fp4_workspace_bytes(int format, int64_t M, int64_t K);
 int samq_linear_fp4(const void* x, int dtype, int64_t ldx, const uint8_t* W, int64_t ldw, const uint8_t* w_scales,
                     int64_t M, int64_t N, int64_t K, int format, float alpha, const void* bias, const void* residual, int64_t ldr,
-                    int activation, void* out, int64_t ldo, int32_t* status, void* stream);
+                    int activation, void* out, int out_dtype, int64_t ldo, void* workspace, size_t workspace_bytes,
+                    int32_t* status, void* stream);
 
 /* Process-wide choice between the two implementations of samq_gemm_i8 for row / tensor scales
  * (no reference counterpart: the reference has a single cuBLAS-style path):

@@ -18,7 +18,7 @@ GRAN_ROW, GRAN_TENSOR, GRAN_GROUP = 0, 1, 2
 ACT_NONE, ACT_GELU = 0, 1
 HAD_NONE, HAD_FULL, HAD_PARTIAL = 0, 1, 2
 FP4_MX, FP4_NV = 0, 1
-LINEAR_FP4_MAX_ROWS = 32
+LINEAR_FP4_ONE_KERNEL_ROWS = 32
 
 EXPORTED_SYMBOLS = (
     "samq_version",
@@ -41,6 +41,7 @@ EXPORTED_SYMBOLS = (
     "samq_quant_fp4",
     "samq_gemm_fp4",
     "samq_linear_fp4",
+    "samq_linear_fp4_workspace_bytes",
     "samq_attn_window_prep",
     "samq_attn_rel_bias",
     "samq_attn_windowed",
@@ -181,9 +182,11 @@ def load() -> ctypes.CDLL:
         c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p,        # x, dtype, ldx, W, ldw, w_scales
         c_int64, c_int64, c_int64, c_int, c_float,                    # M, N, K, format, alpha
         c_void_p, c_void_p, c_int64,                                  # bias, residual, ldr
-        c_int, c_void_p, c_int64,                                     # activation, out, ldo
-        c_void_p, c_void_p,                                           # status, stream
+        c_int, c_void_p, c_int, c_int64,                              # activation, out, out_dtype, ldo
+        c_void_p, c_size_t, c_void_p, c_void_p,                       # workspace, bytes, status, stream
     ]
+    lib.samq_linear_fp4_workspace_bytes.restype = c_size_t
+    lib.samq_linear_fp4_workspace_bytes.argtypes = [c_int, c_int64, c_int64]
     lib.samq_gemm_set_pair_mode.restype = c_int
     lib.samq_gemm_set_pair_mode.argtypes = [c_int]
     lib.samq_attn_transpose_v.restype = c_int

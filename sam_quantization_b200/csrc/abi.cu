@@ -74,7 +74,9 @@ int gemm_fp4_dispatch(const uint8_t* A, int64_t lda, const uint8_t* a_scales, co
                       int activation, void* out, int out_dtype, int64_t ldo, int32_t* status, void* stream);
 int linear_fp4_dispatch(const void* x, int dtype, int64_t ldx, const uint8_t* W, int64_t ldw, const uint8_t* w_scales,
                         int64_t M, int64_t N, int64_t K, int fmt, float alpha, const void* bias, const void* residual, int64_t ldr,
-                        int activation, void* out, int64_t ldo, int32_t* status, void* stream);
+                        int activation, void* out, int out_dtype, int64_t ldo, void* workspace, size_t workspace_bytes,
+                        int32_t* status, void* stream);
+size_t linear_fp4_workspace(int fmt, int64_t M, int64_t K);
 int attn_window14_dispatch(const void* qkv, const void* table, int table_rows, int dtype, int64_t windows, int heads, int head_dim,
                            float scale, void* out, int32_t* status, void* stream);
 int attn_window_dispatch(const void* qkv, int dtype, int64_t windows, int H, int W, int nh, int d,
@@ -271,10 +273,16 @@ int samq_gemm_fp4(const uint8_t* A, int64_t lda, const uint8_t* a_scales, const 
 
 int samq_linear_fp4(const void* x, int dtype, int64_t ldx, const uint8_t* W, int64_t ldw, const uint8_t* w_scales,
                     int64_t M, int64_t N, int64_t K, int format, float alpha, const void* bias, const void* residual, int64_t ldr,
-                    int activation, void* out, int64_t ldo, int32_t* status, void* stream)
+                    int activation, void* out, int out_dtype, int64_t ldo, void* workspace, size_t workspace_bytes,
+                    int32_t* status, void* stream)
 {
     return samq::linear_fp4_dispatch(x, dtype, ldx, W, ldw, w_scales, M, N, K, format, alpha, bias, residual, ldr, activation,
-                                     out, ldo, status, stream);
+                                     out, out_dtype, ldo, workspace, workspace_bytes, status, stream);
+}
+
+size_t samq_linear_fp4_workspace_bytes(int format, int64_t M, int64_t K)
+{
+    return samq::fp4::known_format(format) && M > 0 && K > 0 ? samq::linear_fp4_workspace(format, M, K) : 0;
 }
 
 int samq_gemm_set_pair_mode(int mode)

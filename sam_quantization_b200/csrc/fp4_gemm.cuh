@@ -110,6 +110,19 @@ struct EpiWarp {
             tma_load_2d(smem_u32(staging), map_res, res_bar, col, row0);
         }
     }
+    // rows that no tensor map describes: element loads, a row's columns side by side in the warp
+    __device__ __forceinline__ void fetch_residual(int row0, int col) {
+        if (lane == 0) bulk_wait_read0();
+        __syncwarp();
+        const OutT* res = static_cast<const OutT*>(p.residual) + (int64_t)row0 * p.ldr + col + lane;
+#pragma unroll 8
+        for (int i = 0; i < 32; ++i)
+#pragma unroll
+            for (int j = 0; j < PASS_COLS; j += 32)
+                if (row0 + i < p.M && col + j + lane < p.N)
+                    *reinterpret_cast<OutT*>(staging + staged(i, (j + lane) * sizeof(OutT))) = res[(int64_t)i * p.ldr + j];
+        __syncwarp();
+    }
     // What does not depend on the accumulator: the bias of the columns, and the residual's first box under way.
     __device__ __forceinline__ void before(int row0, int col0) {
 #pragma unroll
@@ -119,7 +132,10 @@ struct EpiWarp {
         }
         __syncwarp();
         if constexpr (RES) {
-            if (p.tma_res && col0 < p.N && row0 < p.M) load_residual(row0, col0);
+            if (col0 < p.N && row0 < p.M) {
+                if (p.tma_res) load_residual(row0, col0);
+                else fetch_residual(row0, col0);
+            }
         }
     }
     // acc: the 64 accumulator columns of this lane's row
@@ -154,18 +170,8 @@ struct EpiWarp {
                     const bool ok = mbar_wait(res_bar, res_phase, abort_flag);
                     res_phase ^= 1u;
                     if (!ok) return false;
-                } else {
-                    // rows that no tensor map describes: element loads, a row's columns side by side in the warp
-                    if (lane == 0) bulk_wait_read0();
-                    __syncwarp();
-                    const OutT* res = static_cast<const OutT*>(p.residual) + (int64_t)row0 * p.ldr + col;
-#pragma unroll 8
-                    for (int i = 0; i < 32; ++i)
-#pragma unroll
-                        for (int j = 0; j < PASS_COLS; j += 32)
-                            if (row0 + i < p.M && col + j + lane < p.N)
-                                *reinterpret_cast<OutT*>(staging + staged(i, (j + lane) * sizeof(OutT))) = res[(int64_t)i * p.ldr + j + lane];
-                    __syncwarp();
+                } else if (ps > 0) {
+                    fetch_residual(row0, col);
                 }
                 staging_free = true;
 #pragma unroll

@@ -29,7 +29,7 @@ constexpr int W_BYTES = BW * BK;
 constexpr int EPI_WARPS = 8;                     // two for each quarter of the 128 columns, taking turns by 16 rows
 constexpr int EPI_THREADS = EPI_WARPS * 32;
 constexpr int THREADS = 64 + EPI_THREADS;
-constexpr int FUSED_MAX_ROWS = SAMQ_LINEAR_FP4_MAX_ROWS;
+constexpr int FUSED_MAX_ROWS = SAMQ_LINEAR_FP4_ONE_KERNEL_ROWS;
 
 struct __align__(8) Control {
     uint64_t full[MAX_STAGES];
@@ -396,16 +396,22 @@ int launch_small(const Fp4Call& c, SmallParams& p, const CUtensorMap& ma, const 
     if (n_tiles * split > 2147483647LL || m_tiles > 65535) return fail(SAMQ_ERR_TOO_LARGE, "product of %lld x %lld outputs is too large", (long long)c.M, (long long)c.N);
     const int cols = p.T + 2 * Shape<FMT>::SF_COLS;
     p.tmem_cols = cols <= 64 ? 64 : cols <= 128 ? 128 : 256;
+    const dim3 grid((unsigned)(n_tiles * split), (unsigned)m_tiles);
+    const size_t smem = smem_bytes<FMT>(p.T, p.stages, split);
+    static_assert(1024 + MIN_STAGES * (stage_bytes<FMT>(MAX_T) + 2 * Shape<FMT>::SF_BYTES) + (MAX_T + MAX_SPLIT) * BW * 4 + sizeof(Control) <= SMEM_MOST &&
+                  HALF_SM + (MAX_T + MAX_SPLIT) * BW * 4 + sizeof(Control) <= SMEM_MOST, "the largest tiles and their joined rows");
+    if (split == 1) {
+        kernel<<<grid, THREADS, smem, c.stream>>>(ma, mw, p);
+        SAMQ_CUDA_TRY(cudaGetLastError());
+        return SAMQ_OK;
+    }
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)(n_tiles * split), (unsigned)m_tiles);
-    cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = smem_bytes<FMT>(p.T, p.stages, split); cfg.stream = c.stream;
+    cfg.gridDim = grid; cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = c.stream;
     cfg.attrs = attr; cfg.numAttrs = 1;
-    static_assert(1024 + MIN_STAGES * (stage_bytes<FMT>(MAX_T) + 2 * Shape<FMT>::SF_BYTES) + (MAX_T + MAX_SPLIT) * BW * 4 + sizeof(Control) <= SMEM_MOST &&
-                  HALF_SM + (MAX_T + MAX_SPLIT) * BW * 4 + sizeof(Control) <= SMEM_MOST, "the largest tiles and their joined rows");
     SAMQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, ma, mw, p));
     return SAMQ_OK;
 }
@@ -469,7 +475,22 @@ int check_call(Fp4Call& c, int64_t M, int64_t N, int64_t K, int fmt, const uint8
     return SAMQ_OK;
 }
 
+// the product of a checked call whose activation is set
+int run_gemm(Fp4Call& c) {
+    if (c.M <= MAX_T || (c.M + 255) / 256 * ((c.N + 191) / 192) < PAIR_MIN_TILES) return gemm_fp4_small(c, nullptr, 0);
+    const int esz = c.out_dtype == SAMQ_F32 ? 4 : 2;
+    int rc = SAMQ_OK;
+    memset(&c.map_out, 0, sizeof(c.map_out));
+    memset(&c.map_res, 0, sizeof(c.map_res));
+    if (c.epi.tma_out) rc = make_row_map(&c.map_out, c.epi.out, c.M, c.N, c.epi.ldo, esz);
+    if (rc == SAMQ_OK && c.epi.tma_res) rc = make_row_map(&c.map_res, c.epi.residual, c.M, c.N, c.epi.ldr, esz);
+    return rc != SAMQ_OK ? rc : gemm_fp4_pair(c);
+}
+
 }  // namespace
+
+int quant_fp4_dispatch(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, int fmt, float global_scale,
+                       uint8_t* codes, int64_t ldq, uint8_t* scales, void* fq, void* stream);
 
 int gemm_fp4_dispatch(const uint8_t* A, int64_t lda, const uint8_t* a_scales, const uint8_t* W, int64_t ldw, const uint8_t* w_scales,
                       int64_t M, int64_t N, int64_t K, int fmt, float alpha, const void* bias, const void* residual, int64_t ldr,
@@ -483,28 +504,38 @@ int gemm_fp4_dispatch(const uint8_t* A, int64_t lda, const uint8_t* a_scales, co
     if ((lda & 15) || ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(a_scales)) & 15))
         return fail(SAMQ_ERR_ALIGNMENT, "4-bit operands need 16-byte aligned bases and row strides (lda=%lld)", (long long)lda);
     c.A = A; c.lda = lda; c.a_scales = a_scales;
-    if (M <= MAX_T || (M + 255) / 256 * ((N + 191) / 192) < PAIR_MIN_TILES) return gemm_fp4_small(c, nullptr, 0);
-    const int esz = out_dtype == SAMQ_F32 ? 4 : 2;
-    memset(&c.map_out, 0, sizeof(c.map_out));
-    memset(&c.map_res, 0, sizeof(c.map_res));
-    if (c.epi.tma_out) rc = make_row_map(&c.map_out, out, M, N, ldo, esz);
-    if (rc == SAMQ_OK && c.epi.tma_res) rc = make_row_map(&c.map_res, residual, M, N, ldr, esz);
-    return rc != SAMQ_OK ? rc : gemm_fp4_pair(c);
+    return run_gemm(c);
+}
+
+// codes of whole 16-byte rows, then the scales
+size_t linear_fp4_workspace(int fmt, int64_t M, int64_t K) {
+    return (size_t)M * ((K + 31) / 32 * 16) + (size_t)((M + TILE_ROWS - 1) / TILE_ROWS * groups_of(fmt, K)) * TILE_BYTES;
 }
 
 int linear_fp4_dispatch(const void* x, int dtype, int64_t ldx, const uint8_t* W, int64_t ldw, const uint8_t* w_scales,
                         int64_t M, int64_t N, int64_t K, int fmt, float alpha, const void* bias, const void* residual, int64_t ldr,
-                        int activation, void* out, int64_t ldo, int32_t* status, void* stream)
+                        int activation, void* out, int out_dtype, int64_t ldo, void* workspace, size_t workspace_bytes,
+                        int32_t* status, void* stream)
 {
     Fp4Call c;
-    int rc = check_call(c, M, N, K, fmt, W, ldw, w_scales, alpha, bias, residual, ldr, activation, out, dtype, ldo, status, stream);
+    int rc = check_call(c, M, N, K, fmt, W, ldw, w_scales, alpha, bias, residual, ldr, activation, out, out_dtype, ldo, status, stream);
     if (rc != SAMQ_OK) return rc;
-    if (M > FUSED_MAX_ROWS) return fail(SAMQ_ERR_TOO_LARGE, "the one-kernel 4-bit linear takes at most %d rows, got %lld", FUSED_MAX_ROWS, (long long)M);
+    if (dtype != SAMQ_F16 && dtype != SAMQ_BF16 && dtype != SAMQ_F32) return fail(SAMQ_ERR_BAD_ARG, "unknown dtype %d", dtype);
     if (M == 0) return SAMQ_OK;
     if (x == nullptr) return fail(SAMQ_ERR_BAD_ARG, "x must not be null");
     if (ldx < K) return fail(SAMQ_ERR_BAD_ARG, "ldx smaller than K");
     if (reinterpret_cast<uintptr_t>(x) & (dtype == SAMQ_F32 ? 3 : 1)) return fail(SAMQ_ERR_ALIGNMENT, "x must be aligned to its elements");
-    return gemm_fp4_small(c, x, ldx);
+    if (M <= FUSED_MAX_ROWS && dtype == out_dtype) return gemm_fp4_small(c, x, ldx);
+    const int64_t pitch = (K + 31) / 32 * 16;
+    const size_t need = linear_fp4_workspace(fmt, M, K);
+    if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))
+        return fail(SAMQ_ERR_WORKSPACE, "the 4-bit linear needs %zu bytes of 16-byte aligned workspace", need);
+    uint8_t* codes = static_cast<uint8_t*>(workspace);
+    uint8_t* scales = codes + (size_t)M * pitch;
+    rc = quant_fp4_dispatch(x, dtype, M, K, ldx, fmt, 1.0f, codes, pitch, scales, nullptr, stream);
+    if (rc != SAMQ_OK) return rc;
+    c.A = codes; c.lda = pitch; c.a_scales = scales;
+    return run_gemm(c);
 }
 
 }  // namespace samq

@@ -429,14 +429,14 @@ def _data_ptr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def _call(dev: torch.device, kind: str, work: float, fn, *args) -> None:
+def _call(dev: torch.device, kind: str, work: float, fn, *args, kernels: int = 1) -> None:
     """``fn(*args, stream)`` on the current stream of ``dev``, counted (and timed) like every launch."""
     if _timing_on or torch.cuda.current_device() != dev.index:
-        with torch.cuda.device(dev), _Timed(kind, work):
+        with torch.cuda.device(dev), _Timed(kind, work, kernels):
             _lib.check(fn(*args, torch.cuda.current_stream().cuda_stream))
         return
     global _launches
-    _launches += 1
+    _launches += kernels
     code = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
     if code:
         _lib.check(code)
@@ -492,7 +492,8 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, 
         out["fq"] = fq = torch.empty_like(x, memory_format=torch.contiguous_format)
     if h is not None:
         out["residual"] = h
-    nbytes = M * K * (dtype.itemsize * (1 + (2 if h is not None else 0) + (1 if fake_quant else 0)) + (1 if codes else 0)) + 4 * M
+    nbytes = 0 if not _timing_on else \
+        M * K * (dtype.itemsize * (1 + (2 if h is not None else 0) + (1 if fake_quant else 0)) + (1 if codes else 0)) + 4 * M
     _call(dev, "rms_norm_quant", nbytes, _lib.load().samq_rms_norm_quant_i8, x2.data_ptr(), _data_ptr(res2), weight.data_ptr(), code, M, K,
           ldx, ldr, eps, n_bits, _data_ptr(h2), ldo, _data_ptr(q), out["scale"].data_ptr(), _data_ptr(fq))
     return out
@@ -575,7 +576,7 @@ def quantize_fp4(x: torch.Tensor, fmt: str = "nvfp4", global_scale: float = 1.0,
     codes = x.new_empty((M, pitch), dtype=torch.uint8)
     scales = x.new_empty(fp4_scale_shape(fmt, M, K), dtype=torch.uint8)
     fq = torch.empty_like(x, memory_format=torch.contiguous_format) if fake_quant else None
-    nbytes = M * K * x.dtype.itemsize * (2 if fake_quant else 1) + codes.numel() + scales.numel()
+    nbytes = 0 if not _timing_on else M * K * x.dtype.itemsize * (2 if fake_quant else 1) + codes.numel() + scales.numel()
     _call(dev, "quant_fp4", nbytes, _lib.load().samq_quant_fp4, x2.data_ptr(), code, M, K, ldx, fcode, global_scale, codes.data_ptr(), pitch,
           scales.data_ptr(), _data_ptr(fq))
     out = {"q": Fp4Tensor(codes, scales, M, K, fmt, global_scale)}
@@ -635,20 +636,26 @@ def linear_fp4(x: torch.Tensor, w: Fp4Tensor, bias: Optional[torch.Tensor] = Non
         raise ValueError(f"x must be [..., {w.K}]")
     if not x.is_cuda:
         _require_cuda(x, "x")
-    N, K, dev = w.rows, w.K, x.device
-    if x.numel() <= _lib.LINEAR_FP4_MAX_ROWS * K and (out_dtype is None or out_dtype == x.dtype):
-        # a few rows: one kernel quantizes and multiplies
-        if dev != w.codes.device:
-            raise ValueError("x must be on the device of w")
-        x2, M, _, ldx = _as_rows(x)
-        code, bias, residual, ldr = _linear_args(N, M, bias, residual, x.dtype, dev)
-        out = x.new_empty((*x.shape[:-1], N))
-        _call(dev, "linear_fp4", 2.0 * M * N * K, _lib.load().samq_linear_fp4, x2.data_ptr(), code, ldx, w.codes.data_ptr(), w.codes.stride(0),
-              w.scales.data_ptr(), M, N, K, FP4_FORMATS[w.fmt], w.global_scale, _data_ptr(bias), _data_ptr(residual), ldr, activation,
-              out.data_ptr(), N, _status_ptr(dev))
-        return out
-    y = gemm_fp4(quantize_fp4(x, w.fmt)["q"], w, bias=bias, residual=residual, activation=activation, out_dtype=out_dtype or x.dtype)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
+    N, K, dev, dtype, wc = w.rows, w.K, x.device, x.dtype, w.codes
+    xcode, fcode = _DTYPE_CODE.get(dtype), FP4_FORMATS[w.fmt]
+    if xcode is None:
+        raise TypeError(f"unsupported dtype {dtype}")
+    if dev != wc.device:
+        raise ValueError("x must be on the device of w")
+    lib = _lib.load()
+    x2, M, _, ldx = _as_rows(x)
+    if out_dtype is None:
+        out_dtype = dtype
+    code, bias, residual, ldr = _linear_args(N, M, bias, residual, out_dtype, dev)
+    out = x.new_empty((*x.shape[:-1], N), dtype=out_dtype)
+    ws, ws_bytes, kernels = None, 0, 1
+    if M > _lib.LINEAR_FP4_ONE_KERNEL_ROWS or code != xcode:
+        ws_bytes = lib.samq_linear_fp4_workspace_bytes(fcode, M, K)
+        ws, kernels = x.new_empty((ws_bytes,), dtype=torch.uint8), 2
+    _call(dev, "linear_fp4", 2.0 * M * N * K, lib.samq_linear_fp4, x2.data_ptr(), xcode, ldx, wc.data_ptr(), wc.stride(0), w.scales.data_ptr(),
+          M, N, K, fcode, w.global_scale, _data_ptr(bias), _data_ptr(residual), ldr, activation, out.data_ptr(), code, N,
+          _data_ptr(ws), ws_bytes, _status_ptr(dev), kernels=kernels)
+    return out
 
 
 def gemm_stall_selftest(a_q: torch.Tensor, w_q: torch.Tensor, skip_kblock: int = 0, wait_limit_cycles: int = 2_000_000) -> torch.Tensor:

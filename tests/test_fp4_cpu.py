@@ -48,6 +48,8 @@ def test_scale_bytes_match_the_shape():
     for fmt in ops.FP4_FORMATS:
         for rows, K in ((1, 1), (128, 256), (129, 257), (5, 5120)):
             assert lib.samq_fp4_scale_bytes(ops.FP4_FORMATS[fmt], rows, K) == math.prod(ops.fp4_scale_shape(fmt, rows, K))
+    assert lib.samq_linear_fp4_workspace_bytes(_lib.FP4_NV, 33, 64) == 33 * 32 + 4 * 512
+    assert lib.samq_linear_fp4_workspace_bytes(_lib.FP4_MX, 129, 257) == 129 * 144 + 2 * 4 * 512 and lib.samq_linear_fp4_workspace_bytes(9, 1, 1) == 0
     assert lib.samq_fp4_scale_bytes(7, 1, 1) == 0 and lib.samq_fp4_scale_bytes(0, 0, 16) == 0
 
 
@@ -77,7 +79,7 @@ def _calls(lib):
     gemm = dict(A=one, lda=32, sa=one, W=one, ldw=32, sw=one, M=4, N=8, K=64, fmt=_lib.FP4_NV, alpha=1.0, bias=None, res=None, ldr=0,
                 act=0, out=one, odt=_lib.F16, ldo=8, status=None, stream=None)
     lin = dict(x=one, dtype=_lib.F16, ldx=64, W=one, ldw=32, sw=one, M=4, N=8, K=64, fmt=_lib.FP4_NV, alpha=1.0, bias=None, res=None, ldr=0,
-               act=0, out=one, ldo=8, status=None, stream=None)
+               act=0, out=one, odt=_lib.F16, ldo=8, ws=None, ws_bytes=0, status=None, stream=None)
     return {"linear": (lib.samq_linear_fp4, lin), "quant": (lib.samq_quant_fp4, quant), "norm": (lib.samq_rms_norm_quant_i8, norm), "gemm": (lib.samq_gemm_fp4, gemm)}
 
 
@@ -93,7 +95,8 @@ def _calls(lib):
     ("gemm", {"A": None}, -1), ("gemm", {"sw": None}, -1), ("gemm", {"out": None}, -1), ("gemm", {"N": 0}, -1), ("gemm", {"K": -1}, -1),
     ("gemm", {"fmt": 5}, -1), ("gemm", {"act": 4}, -1), ("gemm", {"odt": _lib.I32}, -1), ("gemm", {"lda": 16}, -1), ("gemm", {"ldo": 7}, -1),
     ("gemm", {"res": 1 << 20, "ldr": 7}, -1), ("gemm", {"lda": 40}, -3), ("gemm", {"W": (1 << 20) + 8}, -3), ("gemm", {"sa": (1 << 20) + 4}, -3),
-    ("linear", {"x": None}, -1), ("linear", {"M": 33}, -6), ("linear", {"ldx": 63}, -1), ("linear", {"x": (1 << 20) + 1}, -3), ("linear", {"W": None}, -1),
+    ("linear", {"x": None}, -1), ("linear", {"M": 33}, -5), ("linear", {"M": 33, "ws": 1 << 20, "ws_bytes": 33 * 32 + 2047}, -5),
+    ("linear", {"M": 33, "ws": (1 << 20) + 8, "ws_bytes": 1 << 20}, -5), ("linear", {"odt": _lib.F32}, -5), ("linear", {"odt": _lib.I32}, -1), ("linear", {"ldx": 63}, -1), ("linear", {"x": (1 << 20) + 1}, -3), ("linear", {"W": None}, -1),
     ("linear", {"sw": (1 << 20) + 8}, -3), ("linear", {"dtype": _lib.I32}, -1), ("linear", {"K": 0}, -1), ("linear", {"fmt": -1}, -1),
     ("gemm", {"out": (1 << 20) + 1}, -3), ("gemm", {"M": 1 << 31}, -6),
 ])
