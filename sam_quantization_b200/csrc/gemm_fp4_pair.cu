@@ -88,6 +88,9 @@ struct TileWalk {
         m = begin / n_blocks; n = begin % n_blocks;
         step_m = RESIDENT ? 0 : num_pairs / n_blocks; step_n = RESIDENT ? 1 : num_pairs % n_blocks;
     }
+    // Columns of the tile's MMA: the last tile of a row is only as wide as it has to be (1280 columns are six tiles of 192
+    // and one of 128), in steps of 32 of which each CTA holds half.
+    __device__ __forceinline__ int width(int N) const { return min(BN, (N - n * BN + 31) / 32 * 32); }
     __device__ __forceinline__ bool more() const { return left > 0; }
     __device__ __forceinline__ void next() {
         --left; first = false;
@@ -154,6 +157,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             const int mt = walk.m * 2 + (int)rank;                         // this CTA's 128-row tile of A
             const int n0 = walk.n * BN;
             const int nt = n0 / TILE_ROWS;                                 // first of W's two scale tiles
+            const int w_rows = walk.width(p.epi.N) / 2;                    // of W in this CTA (a whole box is loaded)
             const bool load_a = RESIDENT && walk.new_rows();
             for (int kb = 0; kb < k_blocks; ++kb) {
                 if (load_a) ok = mbar_wait(smem_u32(&ctl->a_empty[kb]), a_phase, abort_flag);
@@ -172,7 +176,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                     }
                     if (RESIDENT && rank == 0) mbar_expect_tx(bar, 2 * S::W_BLOCK_BYTES);
                     const uint32_t ss = smem_u32(sfw_s + (size_t)stage * S::SFB_BYTES);
-                    tma_load_2d_pair(smem_u32(w_tiles + (size_t)stage * B_BYTES), &map_w, leader_bar, kb * BK, n0 + (int)rank * BNH);
+                    tma_load_2d_pair(smem_u32(w_tiles + (size_t)stage * B_BYTES), &map_w, leader_bar, kb * BK, n0 + (int)rank * w_rows);
                     tma_load_2d_pair(ss, &map_sfw, leader_bar, 0, nt * p.groups + kb * S::GROUPS);
                     tma_load_2d_pair(ss + S::SFB_BYTES / 2, &map_sfw, leader_bar, 0, (nt + 1) * p.groups + kb * S::GROUPS);
                 }
@@ -204,6 +208,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 if (!mbar_wait(smem_u32(&ctl->acc_empty[acc]), acc_phase ^ 1u, abort_flag)) break;
                 const uint32_t tmem_d = tmem + (uint32_t)(acc * BN);
                 // an odd tile's 192 rows begin in the middle of a scale tile: skip its first 64 rows, two columns
+                const uint32_t idesc_n = (uint32_t)(walk.width(p.epi.N) >> 3) << 17;
                 const uint32_t sf_shift = (uint32_t)(walk.n & 1) * 2u;
                 for (int kb = 0; kb < k_blocks; ++kb) {
                     ok = mbar_wait(smem_u32(&ctl->full[stage]), phase, abort_flag) &&
@@ -222,7 +227,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                             const int g = FMT == SAMQ_FP4_MX ? k / 2 : k;
                             const uint32_t id = FMT == SAMQ_FP4_MX ? 2u * (k & 1) : 0u;
                             mma_fp4<FMT, 2>(tmem_d, adesc + (uint64_t)(k * (UKB >> 4)), bdesc + (uint64_t)(k * (UKB >> 4)),
-                                            instr_desc(FMT, 2 * BM, BN, id), sfa + 4 * g, sfb + 8 * g, (kb | k) != 0 ? 1u : 0u);
+                                            instr_desc(FMT, 2 * BM, 0, id) | idesc_n, sfa + 4 * g, sfb + 8 * g, (kb | k) != 0 ? 1u : 0u);
                         }
                         if (free_a) tcgen05_commit_both(smem_u32(&ctl->a_empty[kb]));
                         tcgen05_commit_both(smem_u32(&ctl->empty[stage]));
