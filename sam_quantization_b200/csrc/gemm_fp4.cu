@@ -444,9 +444,6 @@ int gemm_fp4_small(const Fp4Call& c, const void* x, int64_t ldx) {
 #undef SAMQ_SMALL
 }
 
-// 256 x 192 tiles from which the pair kernel has enough to do
-constexpr int PAIR_MIN_TILES = 32;
-
 // What both entry points check: everything but the activation.
 int check_call(Fp4Call& c, int64_t M, int64_t N, int64_t K, int fmt, const uint8_t* W, int64_t ldw, const uint8_t* w_scales, float alpha,
                const void* bias, const void* residual, int64_t ldr, int activation, void* out, int out_dtype, int64_t ldo,
@@ -477,7 +474,11 @@ int check_call(Fp4Call& c, int64_t M, int64_t N, int64_t K, int fmt, const uint8
 
 // the product of a checked call whose activation is set
 int run_gemm(Fp4Call& c) {
-    if (c.M <= MAX_T || (c.M + 255) / 256 * ((c.N + 191) / 192) < PAIR_MIN_TILES) return gemm_fp4_small(c, nullptr, 0);
+    // The small kernel while all of its CTAs are on the device at once (two an SM), and for a single tile of rows, of
+    // which the pair kernel would compute two.  us, small / pair: 2048 x 2304 x 768 (288 CTAs) 8.6 / 10.3, 512 x 5120 x
+    // 1280 (160) 9.1 / 10.3, 1000 x 5120 x 1280 (320) 14.3 / 12.3, 200 x 20000 x 768 (314) 11.8 / 10.3, 2048 x 5120 x 5120
+    // (640) 40.8 / 33.8, 100 x 20000 x 5120 (157) 16.6 / 23.9
+    if (c.M <= MAX_T || (c.M + MAX_T - 1) / MAX_T * ((c.N + BW - 1) / BW) <= 2 * sm_count()) return gemm_fp4_small(c, nullptr, 0);
     const int esz = c.out_dtype == SAMQ_F32 ? 4 : 2;
     int rc = SAMQ_OK;
     memset(&c.map_out, 0, sizeof(c.map_out));
