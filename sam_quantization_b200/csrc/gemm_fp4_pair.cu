@@ -1,22 +1,23 @@
 // The 4-bit product for many rows: a persistent kernel on CTA pairs (tcgen05 cta_group::2).
 //
-// A pair owns a 256 x 192 output tile.  Each CTA loads its own 128 rows of A with their scales, half of the W tile (96
-// of 192 rows) and the scales of the whole W tile: 34 KiB (nvfp4) or 31 KiB (mxfp4) a stage of 256 columns, five stages.
-// Per stage the leader issues four MMAs (M = 256, N = 192, K = 64).
+// A pair owns a 256-row tile of 256 or 192 columns.  Each CTA loads its own 128 rows of A with their scales, half of the
+// W tile's rows and the scales of the whole W tile, a stage of 256 columns of K at a time.  The leader issues a stage's four
+// MMAs (M = 256, N = the tile's columns, K = 64).
 //
-// The scales reach tensor memory by tcgen05.cp, 12 copies of 512 bytes a stage for nvfp4 and 6 for mxfp4, each about 40
-// clocks.  Issued by the MMA thread they run in order with its MMAs and their time adds up; a thread of its own issues
-// them, so that they run beside the MMAs, half a stage (two MMAs) at a time into a ring of four buffers.  Measured at
-// 32768 x 5120 x 5120 with 256-column tiles: 516 us in the MMA thread, 384 beside it (nvfp4), 405 and 301 (mxfp4).
+// The scales reach tensor memory by tcgen05.cp, 12 copies of 512 bytes a stage for nvfp4 and 6 for mxfp4.  In the MMA thread
+// their issue would add to the MMAs'; a warp of its own issues them, into a ring of two to four stages behind the
+// accumulators.  (Every issuing loop runs in a whole warp with one elected lane: from divergent code each of these
+// instructions takes about 50 clocks.  32768 x 5120 x 5120 nvfp4 / mxfp4: copies in the MMA thread 530 / 420 us, beside it
+// 685 / 502 from divergent loops, 371 / 326 from warp-uniform ones.)
 //
-// Two accumulators of 192 columns and the ring fill tensor memory.  256-column tiles would have to share columns between
-// the two accumulators; the hand-over across the pair that this needs took 1.5 us a tile.
+// What bounds the kernel beside the power limit is the traffic between L2 and the SMs, about 45 bytes a clock and SM.
+//   K <= 1280 (RESIDENT): the A tile of a pair stays in shared memory, the pair walks along consecutive N tiles of its
+//     rows, and a stage is W's part only: 192 columns, two whole accumulators.  1280 -> 5120: 153 -> 134 us (sustained).
+//   else: 256 columns, 14 % less traffic a product than 192.  The two accumulators and the scale ring do not fit tensor memory
+//     side by side: the second accumulator shares its first columns with the first one's last, and its MMAs start when the
+//     epilogue warps that hold those columns have read them.  5120 -> 1280 nvfp4 111 -> 98 us, mxfp4 96 -> 94.
 //
-// What bounds the kernel is the traffic between L2 and the SMs, about 43 bytes a clock and SM.  So where the A tile of
-// a pair fits shared memory whole (K <= 1280) it stays there (RESIDENT): a pair walks along consecutive N tiles of its
-// rows, and a stage is W's part only, 16 instead of 34 KiB.
-//
-// Twelve epilogue warps (32 rows x 64 columns each) read their columns at once and hand them back before they compute.
+// The epilogue warps (32 rows x 64 columns each) read their columns at once and hand them back before they compute.
 // The residual comes in by TMA into the warp's staging buffer while the tile is computed, the result leaves from there
 // by TMA.  Every wait is bounded.
 #include "fp4_gemm.cuh"
@@ -27,47 +28,55 @@ namespace fp4 {
 namespace {
 
 constexpr int BM = 128;                          // rows of A of a CTA
-constexpr int BN = 192;                          // columns of the pair's tile
-constexpr int BNH = BN / 2;                      // rows of W of a CTA
-constexpr int STAGES = 5;
 constexpr int A_BYTES = BM * BK;
-constexpr int B_BYTES = BNH * BK;
-constexpr int EPI_WARPS = 4 * (BN / EPI_COLS);
 constexpr int FIRST_EPI_WARP = 4;                // TMA, MMA, scale copies, one idle
-constexpr int THREADS = (FIRST_EPI_WARP + EPI_WARPS) * 32;
 constexpr int RESIDENT_BLOCKS = 5;               // blocks of 256 columns of a resident A tile
 constexpr int TMEM_COLS = 512;
-constexpr int SF_COL = 2 * BN;                   // the ring of scale columns behind the accumulators
+constexpr int MAX_STAGES = 5, MAX_UNITS = 4, MAX_EPI_WARPS = 16;
 
-template <int FMT> struct Shape {
+// The two shapes: RESIDENT with 192-column tiles, else 256.
+template <int FMT, bool RESIDENT> struct Shape {
+    static constexpr int BN = RESIDENT ? 192 : 256;                // columns of the pair's tile
+    static constexpr int BNH = BN / 2;                             // rows of W of a CTA
+    static constexpr int STAGES = RESIDENT ? 5 : 4;
+    static constexpr int EPI_WARPS = 4 * (BN / EPI_COLS);
+    static constexpr int THREADS = (FIRST_EPI_WARP + EPI_WARPS) * 32;
     static constexpr int GROUPS = groups_per_kpad(FMT);            // scale tiles of 128 rows a stage
     static constexpr int UNIT_COLS = 12 * GROUPS;                  // a buffer of the ring: per group 4 columns for A, 8 for W
-    static constexpr int UNITS = FMT == SAMQ_FP4_MX ? 4 : 2;
-    static_assert(SF_COL + UNITS * UNIT_COLS <= TMEM_COLS, "accumulators and scales fit tensor memory");
+    static constexpr int UNITS = !RESIDENT ? 3 : FMT == SAMQ_FP4_MX ? 4 : 2;
+    static constexpr int SF_COL = TMEM_COLS - UNITS * UNIT_COLS;   // the ring of scale columns behind the accumulators
+    static constexpr int ACC1_COL = SF_COL - BN;                   // the second accumulator ends there
+    static constexpr int SHARED_COLS = BN > ACC1_COL ? BN - ACC1_COL : 0;      // columns that both accumulators use
+    static constexpr int SHARED_GROUPS = (SHARED_COLS + EPI_COLS - 1) / EPI_COLS;
+    static constexpr int B_BYTES = BNH * BK;
     static constexpr int SFA_BYTES = GROUPS * TILE_BYTES;
-    static constexpr int SFB_BYTES = 2 * GROUPS * TILE_BYTES;      // 192 rows of W lie in two tiles of 128
+    static constexpr int SFB_BYTES = 2 * GROUPS * TILE_BYTES;      // W's rows lie in two tiles of 128
     static constexpr int A_BLOCK_BYTES = A_BYTES + SFA_BYTES;
     static constexpr int W_BLOCK_BYTES = B_BYTES + SFB_BYTES;
+    static_assert(UNITS <= STAGES && UNITS <= MAX_UNITS, "a buffer's last stage is waited for by its place in the ring of stages");
+    static_assert(SFB_BYTES % 128 == 0 && ACC1_COL >= 0, "layout");
+    static constexpr int A_BLOCKS = RESIDENT ? RESIDENT_BLOCKS : STAGES;       // one a stage, or all of a resident tile
 };
 
 struct __align__(8) Control {
-    uint64_t full[STAGES];
-    uint64_t empty[STAGES];
+    uint64_t full[MAX_STAGES];
+    uint64_t empty[MAX_STAGES];
     uint64_t acc_full[2];
     uint64_t acc_empty[2];
-    uint64_t sf_ready[4];                         // scale columns written (the leader's only)
-    uint64_t res[EPI_WARPS];
+    uint64_t shared_empty;                        // the columns that the two accumulators share
+    uint64_t sf_ready[MAX_UNITS];                         // scale columns written (the leader's only)
+    uint64_t res[MAX_EPI_WARPS];
     uint64_t a_full[RESIDENT_BLOCKS];             // RESIDENT: blocks of A loaded / no longer read
     uint64_t a_empty[RESIDENT_BLOCKS];
     uint32_t tmem_base;
     uint32_t abort_flag;
 };
 
-// A blocks: one a stage, or all of a resident tile
-constexpr int a_blocks(bool resident) { return resident ? RESIDENT_BLOCKS : STAGES; }
 template <int FMT, bool RESIDENT>
 constexpr size_t smem_bytes() {
-    return 1024 + (size_t)a_blocks(RESIDENT) * Shape<FMT>::A_BLOCK_BYTES + (size_t)STAGES * Shape<FMT>::W_BLOCK_BYTES + (size_t)EPI_WARPS * (STAGING_BYTES + EPI_COLS * sizeof(float)) + sizeof(Control);
+    using S = Shape<FMT, RESIDENT>;
+    return 1024 + (size_t)S::A_BLOCKS * S::A_BLOCK_BYTES + (size_t)S::STAGES * S::W_BLOCK_BYTES +
+           (size_t)S::EPI_WARPS * (STAGING_BYTES + EPI_COLS * sizeof(float)) + sizeof(Control);
 }
 
 struct PairParams {
@@ -78,7 +87,7 @@ struct PairParams {
 
 // The tiles of a pair in order, without a division per tile.  RESIDENT: consecutive tiles, so that A changes seldom; else
 // the pairs work side by side.
-template <bool RESIDENT>
+template <bool RESIDENT, int BN>
 struct TileWalk {
     int n_blocks, left, m, n, step_m, step_n;
     bool first = true;                            // nothing of the pair's rows has been done before
@@ -102,20 +111,21 @@ struct TileWalk {
 };
 
 template <typename OutT, int FMT, bool GELU, bool RES, bool RESIDENT>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(Shape<FMT, RESIDENT>::THREADS, 1)
 gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                      const __grid_constant__ CUtensorMap map_sfa, const __grid_constant__ CUtensorMap map_sfw,
                      const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_res,
                      const __grid_constant__ PairParams p)
 {
-    using S = Shape<FMT>;
+    using S = Shape<FMT, RESIDENT>;
+    constexpr int BN = S::BN, STAGES = S::STAGES, EPI_WARPS = S::EPI_WARPS, B_BYTES = S::B_BYTES;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = smem_u32(smem_raw);
     uint8_t* tiles = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);              // 1024-byte aligned
-    uint8_t* w_tiles = tiles + (size_t)a_blocks(RESIDENT) * A_BYTES;                     // all of these 1024-byte aligned
+    uint8_t* w_tiles = tiles + (size_t)S::A_BLOCKS * A_BYTES;                     // all of these 1024-byte aligned
     uint8_t* staging = w_tiles + (size_t)STAGES * B_BYTES;
     uint8_t* sfa_s = staging + (size_t)EPI_WARPS * STAGING_BYTES;
-    uint8_t* sfw_s = sfa_s + (size_t)a_blocks(RESIDENT) * S::SFA_BYTES;
+    uint8_t* sfw_s = sfa_s + (size_t)S::A_BLOCKS * S::SFA_BYTES;
     float* bias_s = reinterpret_cast<float*>(sfw_s + (size_t)STAGES * S::SFB_BYTES);
     Control* ctl = reinterpret_cast<Control*>(bias_s + EPI_WARPS * EPI_COLS);
     volatile uint32_t* abort_flag = &ctl->abort_flag;
@@ -127,12 +137,13 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     const int n_blocks = (p.epi.N + BN - 1) / BN;
     const int k_blocks = (p.K + KPAD - 1) / KPAD;
     const int num_tiles = m_blocks * n_blocks;
-    TileWalk<RESIDENT> walk(num_tiles, n_blocks, pair, num_pairs);
+    TileWalk<RESIDENT, BN> walk(num_tiles, n_blocks, pair, num_pairs);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(smem_u32(&ctl->full[s]), 1); mbar_init(smem_u32(&ctl->empty[s]), 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(smem_u32(&ctl->acc_full[b]), 1); mbar_init(smem_u32(&ctl->acc_empty[b]), 2 * EPI_WARPS); }
-        for (int u = 0; u < 4; ++u) mbar_init(smem_u32(&ctl->sf_ready[u]), 1);
+        mbar_init(smem_u32(&ctl->shared_empty), 2 * 4 * (S::SHARED_GROUPS > 0 ? S::SHARED_GROUPS : 1));
+        for (int u = 0; u < S::UNITS; ++u) mbar_init(smem_u32(&ctl->sf_ready[u]), 1);
         for (int w = 0; w < EPI_WARPS; ++w) mbar_init(smem_u32(&ctl->res[w]), 1);
         for (int b = 0; b < RESIDENT_BLOCKS; ++b) { mbar_init(smem_u32(&ctl->a_full[b]), 1); mbar_init(smem_u32(&ctl->a_empty[b]), 1); }
         ctl->abort_flag = 0;
@@ -200,16 +211,19 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         if (rank == 0) {
             int stage = 0; uint32_t phase = 0;
             int acc = 0; uint32_t acc_phase = 0;
-            int unit = 0; uint32_t unit_phase = 0, a_phase = 1;
+            int unit = 0; uint32_t unit_phase = 0, a_phase = 1, shared_phase = 1;
             bool ok = true;
             for (; walk.more() && ok; walk.next()) {
                 const bool wait_a = RESIDENT && walk.new_rows(), free_a = RESIDENT && walk.rows_done();
                 if (wait_a) a_phase ^= 1u;
+                // the buffer itself (two tiles ago) and the columns that the previous tile's buffer shares with it
                 if (!mbar_wait(smem_u32(&ctl->acc_empty[acc]), acc_phase ^ 1u, abort_flag)) break;
-                const uint32_t tmem_d = tmem + (uint32_t)(acc * BN);
-                // an odd tile's 192 rows begin in the middle of a scale tile: skip its first 64 rows, two columns
+                if (S::SHARED_COLS > 0 && !mbar_wait(smem_u32(&ctl->shared_empty), shared_phase, abort_flag)) break;
+                shared_phase ^= 1u;
+                const uint32_t tmem_d = tmem + (uint32_t)(acc * S::ACC1_COL);
+                // an odd tile of 192 rows begins in the middle of a scale tile: skip its first 64 rows, two columns
                 const uint32_t idesc_n = (uint32_t)(walk.width(p.epi.N) >> 3) << 17;
-                const uint32_t sf_shift = (uint32_t)(walk.n & 1) * 2u;
+                const uint32_t sf_shift = BN % TILE_ROWS != 0 ? (uint32_t)(walk.n & 1) * 2u : 0u;
                 for (int kb = 0; kb < k_blocks; ++kb) {
                     ok = mbar_wait(smem_u32(&ctl->full[stage]), phase, abort_flag) &&
                          (!wait_a || mbar_wait(smem_u32(&ctl->a_full[kb]), a_phase, abort_flag)) &&
@@ -218,7 +232,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                     tcgen05_fence_after();
                     const uint64_t adesc = make_smem_desc(smem_u32(tiles + (size_t)(RESIDENT ? kb : stage) * A_BYTES));
                     const uint64_t bdesc = make_smem_desc(smem_u32(w_tiles + (size_t)stage * B_BYTES));
-                    const uint32_t sfa = tmem + SF_COL + (uint32_t)(unit * S::UNIT_COLS);
+                    const uint32_t sfa = tmem + S::SF_COL + (uint32_t)(unit * S::UNIT_COLS);
                     const uint32_t sfb = sfa + 4 * S::GROUPS + sf_shift;
                     if (elect_one()) {
 #pragma unroll
@@ -265,7 +279,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                     tcgen05_fence_after();
                     const uint32_t sa = smem_u32(sfa_s + (size_t)(RESIDENT ? kb : stage) * S::SFA_BYTES);
                     const uint32_t sw = smem_u32(sfw_s + (size_t)stage * S::SFB_BYTES);
-                    const uint32_t sfa = tmem + SF_COL + (uint32_t)(unit * S::UNIT_COLS);
+                    const uint32_t sfa = tmem + S::SF_COL + (uint32_t)(unit * S::UNIT_COLS);
                     const uint32_t sfb = sfa + 4 * S::GROUPS;
                     if (elect_one()) {
 #pragma unroll
@@ -297,10 +311,15 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             if (!mbar_wait(smem_u32(&ctl->acc_full[acc]), acc_phase, abort_flag)) break;
             tcgen05_fence_after();
             uint32_t r[EPI_COLS];
-            tmem_ld64(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN + cg * EPI_COLS), r);
+            tmem_ld64(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * S::ACC1_COL + cg * EPI_COLS), r);
             tcgen05_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_remote(map_to_cta(smem_u32(&ctl->acc_empty[acc]), 0));
+            if (lane == 0) {
+                // the last groups of the first buffer and the first ones of the second hold the shared columns
+                if (S::SHARED_GROUPS > 0 && (acc == 0 ? cg >= BN / EPI_COLS - S::SHARED_GROUPS : cg < S::SHARED_GROUPS))
+                    mbar_arrive_remote(map_to_cta(smem_u32(&ctl->shared_empty), 0));
+                mbar_arrive_remote(map_to_cta(smem_u32(&ctl->acc_empty[acc]), 0));
+            }
             if (!epi.finish(row0, col0, r)) break;
             if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
         }
@@ -322,14 +341,16 @@ int launch(const Fp4Call& c, const CUtensorMap& ma, const CUtensorMap& mw, const
     auto kernel = gemm_fp4_pair_kernel<OutT, FMT, GELU, RES, RESIDENT>;
     constexpr size_t SMEM = smem_bytes<FMT, RESIDENT>();
     SAMQ_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
-    const int64_t tiles = ((c.M + 2 * BM - 1) / (2 * BM)) * ((c.N + BN - 1) / BN);
+    using S = Shape<FMT, RESIDENT>;
+    static_assert(SMEM <= 227 * 1024, "shared memory");
+    const int64_t tiles = ((c.M + 2 * BM - 1) / (2 * BM)) * ((c.N + S::BN - 1) / S::BN);
     if (tiles > 2147483647LL - 256) return fail(SAMQ_ERR_TOO_LARGE, "product of %lld x %lld outputs is too large", (long long)c.M, (long long)c.N);
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM; cfg.stream = c.stream;
+    cfg.blockDim = dim3(S::THREADS); cfg.dynamicSmemBytes = SMEM; cfg.stream = c.stream;
     cfg.attrs = attr; cfg.numAttrs = 1;
     // how many pairs the device can hold at once (GPCs with an odd number of SMs leave one out)
     static thread_local int pairs_cached[64] = {0};
@@ -354,10 +375,10 @@ int launch(const Fp4Call& c) {
     CUtensorMap ma, mw, msa, msw;
     const int64_t row_bytes = (c.K + 1) / 2;
     int rc = make_operand_map(&ma, reinterpret_cast<const int8_t*>(c.A), c.M, row_bytes, c.lda, BM);
-    if (rc == SAMQ_OK) rc = make_operand_map(&mw, reinterpret_cast<const int8_t*>(c.W), c.N, row_bytes, c.ldw, BNH);
+    if (rc == SAMQ_OK) rc = make_operand_map(&mw, reinterpret_cast<const int8_t*>(c.W), c.N, row_bytes, c.ldw, Shape<FMT, RESIDENT>::BNH);
     const int64_t groups = groups_of(FMT, c.K);
-    if (rc == SAMQ_OK) rc = make_scale_map(&msa, c.a_scales, (c.M + TILE_ROWS - 1) / TILE_ROWS * groups, Shape<FMT>::GROUPS);
-    if (rc == SAMQ_OK) rc = make_scale_map(&msw, c.w_scales, (c.N + TILE_ROWS - 1) / TILE_ROWS * groups, Shape<FMT>::GROUPS);
+    if (rc == SAMQ_OK) rc = make_scale_map(&msa, c.a_scales, (c.M + TILE_ROWS - 1) / TILE_ROWS * groups, Shape<FMT, RESIDENT>::GROUPS);
+    if (rc == SAMQ_OK) rc = make_scale_map(&msw, c.w_scales, (c.N + TILE_ROWS - 1) / TILE_ROWS * groups, Shape<FMT, RESIDENT>::GROUPS);
     if (rc != SAMQ_OK) return rc;
     PairParams p;
     p.epi = c.epi; p.K = (int)c.K; p.groups = (int)groups; p.status = c.status;
