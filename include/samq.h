@@ -303,7 +303,8 @@ int samq_rms_norm_quant_i8(const void* x, const void* residual, const void* weig
  * border between codes depends on a rounding.
  *
  * Storage of [rows, K]:
- *   codes  : uint8 [rows, ldq], column 2j in the low nibble of byte j; ldq a multiple of 16 for the product
+ *   codes  : uint8 [rows, ldq], column 2j in the low nibble of byte j, the last high nibble of an odd K zero (what lies
+ *            behind a row's (K + 1) / 2 bytes is not read); ldq a multiple of 16 for the product
  *   scales : samq_fp4_scale_bytes() bytes, 16-byte aligned: [ceil(rows/128)][G][32][4][4], the byte of (row, block) at
  *            [row / 128][block / 4][row % 32][row % 128 / 32][block % 4]; G = ceil(K / 256) * (2 for MX, 4 for NV).
  *            Scales of blocks behind K are zero (the product multiplies them with zero codes).

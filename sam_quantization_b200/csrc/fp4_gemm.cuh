@@ -72,8 +72,14 @@ __device__ __forceinline__ uint32_t staged(int row, uint32_t byte) {
     return (uint32_t)row * 128u + (byte ^ ((uint32_t)(row & 7) << 4));
 }
 
+__device__ __forceinline__ float max0_nan(float x) {
+    float r;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(x));
+    return r;
+}
 // gelu_erf of two values in the fewest operations a result: with v = max(-|x|, -6.08), 2^Q(v) = Phi(v) and
-// gelu(x) = max(x, 0) + v * Phi(v).  Q is gelu_erf's polynomial with the odd coefficients' signs turned.
+// gelu(x) = max(x, 0) + v * Phi(v).  Q is gelu_erf's polynomial with the odd coefficients' signs turned.  v loses a NaN, the
+// other maximum keeps it.
 __device__ __forceinline__ float2 gelu_pair(float2 x) {
     const float2 v = make_float2(fmaxf(-fabsf(x.x), -6.08f), fmaxf(-fabsf(x.y), -6.08f));
     float2 q = make_float2(3.586083039e-05f, 3.586083039e-05f);
@@ -86,7 +92,7 @@ __device__ __forceinline__ float2 gelu_pair(float2 x) {
     float2 h;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h.x) : "f"(q.x));
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h.y) : "f"(q.y));
-    return __ffma2_rn(v, h, make_float2(fmaxf(x.x, 0.f), fmaxf(x.y, 0.f)));
+    return __ffma2_rn(v, h, make_float2(max0_nan(x.x), max0_nan(x.y)));
 }
 
 template <typename OutT, bool GELU, bool RES>
@@ -106,6 +112,7 @@ struct EpiWarp {
         // the staging buffer is free once the previous tile's store has read it
         if (lane == 0) {
             bulk_wait_read0();
+            fence_async_smem();
             mbar_expect_tx(res_bar, STAGING_BYTES);
             tma_load_2d(smem_u32(staging), map_res, res_bar, col, row0);
         }

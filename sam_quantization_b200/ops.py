@@ -591,7 +591,8 @@ def _linear_args(N: int, M: int, bias, residual, out_dtype, dev):
     if code is None:
         raise TypeError(f"unsupported out_dtype {out_dtype}")
     if bias is not None:
-        bias = _bias_as(bias, out_dtype, dev)
+        if bias.dtype != out_dtype or bias.device != dev or not bias.is_contiguous():
+            bias = bias.detach().to(device=dev, dtype=out_dtype).contiguous()
         if bias.numel() != N:
             raise ValueError("bias must have N elements")
     ldr = 0

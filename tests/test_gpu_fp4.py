@@ -118,7 +118,9 @@ def _exact_operand(rows, K, fmt, dev, seed):
 
 
 SHAPES = [(1, 1, 1), (1, 8, 64), (3, 130, 31), (1, 5120, 1280), (128, 128, 256), (129, 257, 300), (200, 40, 1283), (64, 1001, 512), (16, 300, 2048),
-          (17, 65, 96), (40, 200, 4100), (260, 520, 768), (1000, 384, 200), (300, 1280, 5120), (1, 20000, 300), (200, 7000, 256), (24, 2304, 768), (2600, 1300, 600), (8200, 257, 1283), (290, 8210, 300), (4096, 2304, 768)]
+          (17, 65, 96), (40, 200, 4100), (260, 520, 768), (1000, 384, 200), (300, 1280, 5120), (1, 20000, 300), (200, 7000, 256), (24, 2304, 768), (2600, 1300, 600), (8200, 257, 1283), (290, 8210, 300), (4096, 2304, 768),
+          # enough tiles for the pair kernel, A resident and not
+          (40000, 20, 100), (39990, 130, 1300), (5000, 1301, 1280), (5001, 1300, 1281), (300, 20000, 520), (20000, 384, 2600), (700, 9000, 3)]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -134,7 +136,7 @@ def test_product_is_exact_where_its_sums_are(cuda_device, fmt, M, N, K):
 
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("M,N,K", [(1, 300, 1280), (5, 72, 100), (40, 1001, 2000), (130, 257, 1283), (600, 640, 512), (2050, 1096, 300), (2050, 1101, 300)])
+@pytest.mark.parametrize("M,N,K", [(1, 300, 1280), (5, 72, 100), (40, 1001, 2000), (130, 257, 1283), (600, 640, 512), (2050, 1096, 300), (5050, 1096, 300), (5050, 1101, 1400)])
 @pytest.mark.parametrize("bias,gelu,residual", [(True, False, False), (True, True, False), (False, False, True), (True, True, True)])
 def test_epilogue(cuda_device, fmt, dtype, M, N, K, bias, gelu, residual):
     """Exact sums, so only the epilogue rounds: alpha and bias in one fused step (u), GELU (3e-7 absolute and 2e-5
@@ -221,18 +223,37 @@ def _same_bytes(a, b):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("M", [1, 33, 200, 9000])
+@pytest.mark.parametrize("M", [1, 33, 200, 40001])
 def test_rows_that_are_not_finite_stay_apart(cuda_device, fmt, M):
     x = _values(M, 300, torch.float16)
     x[M // 2, 299] = float("nan")
     w, wv = _exact_operand(50, 300, fmt, cuda_device, 3)
-    y = ops.linear_fp4(x.to(cuda_device), w)
+    for act in (ops.ACT_NONE, ops.ACT_GELU):
+        y = ops.linear_fp4(x.to(cuda_device), w, activation=act)
+        ops.check_status()
+        bad = ~x.isfinite().all(1).to(cuda_device)                       # (a value of the others can be an fp16 infinity too)
+        assert bad[M // 2] and torch.equal(y.isnan().all(1), bad) and torch.equal(y.isnan().any(1), bad)
+
+
+@pytest.mark.parametrize("K", [200, 1500])
+@pytest.mark.parametrize("N,res_pitch", [(1096, 1101), (1101, 1112), (1101, 1101), (1096, 1104)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_outputs_and_residuals_with_and_without_a_tensor_map(cuda_device, dtype, N, res_pitch, K):
+    """Rows of 16 bytes go by TMA, others element by element, the two of a call independently of one another."""
+    M = 5050
+    a, av = _exact_operand(M, K, "nvfp4", cuda_device, 1)
+    w, wv = _exact_operand(N, K, "nvfp4", cuda_device, 2)
+    w.global_scale = 2.0 ** -8
+    res = torch.randn(M, res_pitch, generator=torch.Generator().manual_seed(3)).to(dtype).to(cuda_device)[:, :N]
+    y = ops.gemm_fp4(a, w, residual=res, out_dtype=dtype)
     ops.check_status()
-    rows = [m for m in range(M) if m != M // 2]
-    assert y[M // 2].isnan().all() and not y[rows].isnan().any()
+    z = av @ wv.T * 2.0 ** -8 + res.double().cpu().numpy()
+    tol = 2.0 ** -24 * np.abs(z)
+    tol = tol + HALF[dtype] * (np.abs(z) + tol) + (2.0 ** -25 if dtype == torch.float16 else 0)
+    assert np.all(np.abs(y.double().cpu().numpy() - z) <= tol)
 
 
-@pytest.mark.parametrize("M", [3, 200, 700, 9000])
+@pytest.mark.parametrize("M", [3, 200, 700, 20001])
 def test_strided_outputs_and_operands(cuda_device, M):
     a, av = _exact_operand(M, 320, "nvfp4", cuda_device, 1)
     w, wv = _exact_operand(130, 320, "nvfp4", cuda_device, 2)
@@ -276,7 +297,7 @@ def _same(a, b):
     return torch.equal(a.view(torch.int16), b.view(torch.int16))
 
 
-@pytest.mark.parametrize("M", [2, 150])
+@pytest.mark.parametrize("M", [2, 150, 20000])
 def test_captured_replayed_and_on_two_streams(cuda_device, M):
     x = _values(M, 640, torch.float16).to(cuda_device)
     x2 = _values(M, 640, torch.float16, seed=4).to(cuda_device)
