@@ -22,7 +22,6 @@ struct RmsNormParams {
     int8_t* q; float* scale; void* fq;
     int64_t M; int K;
     float eps, inv_k, qmax;
-    int vec;                                       // every row of every tensor starts on 16 bytes and K fills vectors
 };
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -37,23 +36,29 @@ __device__ __forceinline__ float max_abs_nan(float a, float b) {
     return r;
 }
 
-// E elements of a row in the tensor type (a 16-byte vector, or one element), widened to fp32 pairs where they are used
-// (E = 1: the second of the pair is 0)
+template <int BYTES> struct RawOf;
+template <> struct RawOf<16> { using type = uint4; };
+template <> struct RawOf<8>  { using type = uint2; };
+template <> struct RawOf<4>  { using type = uint32_t; };
+template <> struct RawOf<2>  { using type = uint16_t; };
+template <> struct RawOf<1>  { using type = uint8_t; };
+
+// E elements of a row in the tensor type, loaded and stored at once, widened to fp32 pairs where they are used (E = 1: the
+// second of the pair is 0)
 template <typename T, int E> struct Vec {
     static constexpr int P = E == 1 ? 1 : E / 2;
-    union { uint4 raw; T t[E]; };
+    using Raw = typename RawOf<E * (int)sizeof(T)>::type;
+    union { Raw raw; T t[E]; };
     __device__ __forceinline__ Vec() {}
     __device__ __forceinline__ void zero() {
-        if constexpr (E == 1) t[0] = Elem<T>::down(0.0f);
-        else raw = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < E; ++j) t[j] = Elem<T>::down(0.0f);
     }
     __device__ __forceinline__ void load(const T* p) {
-        if constexpr (E == 1) t[0] = *p;
-        else raw = *reinterpret_cast<const uint4*>(p);
+        raw = *reinterpret_cast<const Raw*>(p);
     }
     __device__ __forceinline__ void store(T* p) const {
-        if constexpr (E == 1) *p = t[0];
-        else *reinterpret_cast<uint4*>(p) = raw;
+        *reinterpret_cast<Raw*>(p) = raw;
     }
     __device__ __forceinline__ float2 pair(int i) const {
         if constexpr (E == 1) return make_float2(Elem<T>::up(t[0]), 0.0f);
@@ -67,7 +72,7 @@ template <typename T, int E> struct Vec {
     }
 };
 
-// E elements a load (a 16-byte vector, or one where rows are not aligned), NV loads a thread, RW warps a row.
+// E elements a load (the widest that every row of every tensor starts on), NV loads a thread, RW warps a row.
 template <typename T, int E, int NV, int RW, bool RES>
 __global__ void __launch_bounds__(RW >= 4 ? RW * 32 : 128, 1)
 rms_norm_quant_kernel(const RmsNormParams p)
@@ -180,6 +185,8 @@ rms_norm_quant_kernel(const RmsNormParams p)
         if (q_out != nullptr) {
             if constexpr (E == 1) {
                 q_out[c] = (int8_t)(code[0] & 0xFFu);
+            } else if constexpr (E == 2) {
+                *reinterpret_cast<uint16_t*>(q_out + c) = (uint16_t)__byte_perm(code[0], code[1], 0x0040);
             } else {
                 uint32_t word[E / 4];
 #pragma unroll
@@ -216,13 +223,16 @@ int launch_warps(int64_t loads, const RmsNormParams& p, cudaStream_t st) {
     return launch<T, E, NV, 32>(p, st);
 }
 
+// `e` elements: the widest access for all rows, see the caller
 template <typename T>
-int launch_rms_norm(const RmsNormParams& p, cudaStream_t st) {
+int launch_rms_norm(const RmsNormParams& p, int e, cudaStream_t st) {
     constexpr int E = Elem<T>::kPerVec;
     // 5 vectors: 1280 columns of a 16-bit type are one warp's, with no lane idle
-    if (p.vec) return launch_warps<T, E, 5>(p.K / E, p, st);
-    // single elements: more warps and fewer elements each, while a block can hold the row so
-    if (p.K <= 8192) return launch_warps<T, 1, 8>(p.K, p, st);
+    if (e == E && p.K <= 1024 * 5 * E) return launch_warps<T, E, 5>(p.K / E, p, st);
+    // narrower accesses: more warps a row and fewer elements each
+    if (E == 8 && e == 4) return launch_warps<T, 4, 8>(p.K / 4, p, st);
+    if (e >= 2 && p.K <= 1024 * 8 * 2) return launch_warps<T, 2, 8>(p.K / 2, p, st);
+    if (p.K <= 1024 * 8) return launch_warps<T, 1, 8>(p.K, p, st);
     return launch<T, 1, 32, 32>(p, st);
 }
 
@@ -249,14 +259,15 @@ int rms_norm_quant_dispatch(const void* x, const void* residual, const void* wei
     p.x = x; p.ldx = ldx; p.residual = residual; p.ldr = residual ? ldr : 0; p.weight = weight;
     p.residual_out = residual_out; p.ldo = residual ? ldo : 0; p.q = q; p.scale = scale; p.fq = fq;
     p.M = M; p.K = (int)K; p.eps = eps; p.inv_k = 1.0f / (float)K; p.qmax = (float)((1 << (n_bits - 1)) - 1);
-    const int64_t vec = 16 / (int64_t)esz;
-    p.vec = (all & 15) == 0 && K % vec == 0 && ldx % vec == 0 && p.ldr % vec == 0 && p.ldo % vec == 0 &&
-            (reinterpret_cast<uintptr_t>(q) & (vec - 1)) == 0 && K <= 1024 * 5 * vec;
+    // Every address and pitch that a row starts by, in bytes of the tensor type (the codes' scaled to it): the largest power of
+    // two that divides them all is the widest access, up to 16 bytes.
+    const uintptr_t starts = all | reinterpret_cast<uintptr_t>(q) * esz | (uintptr_t)((K | ldx | p.ldr | p.ldo) * (int64_t)esz) | 16;
+    const int e = (int)((starts & (~starts + 1)) / esz);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (dtype) {
-    case SAMQ_F16:  return launch_rms_norm<__half>(p, st);
-    case SAMQ_BF16: return launch_rms_norm<__nv_bfloat16>(p, st);
-    default:        return launch_rms_norm<float>(p, st);
+    case SAMQ_F16:  return launch_rms_norm<__half>(p, e, st);
+    case SAMQ_BF16: return launch_rms_norm<__nv_bfloat16>(p, e, st);
+    default:        return launch_rms_norm<float>(p, e, st);
     }
 }
 
