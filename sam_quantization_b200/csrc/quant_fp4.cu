@@ -24,16 +24,19 @@ struct QuantFp4Params {
     void* fq;
     int col_blocks;
     int access_x, access_fq;                     // see Access
+    int pairs;                                   // STAGED 16-bit rows start on 4 bytes: two elements an access
     int vec_q;                                   // rows of codes start on 8 bytes
 };
 
 // A warp takes the rows that share 32 (nvfp4) or 16 (mxfp4) bytes of a scale tile, so that its scales leave as
 // whole pieces: nvfp4 8 rows (r, r + 1, each + 0, 32, 64, 96) x 4 chunks, mxfp4 4 rows (r + 0, 32, 64, 96) x 8 chunks.
+// the warp's rows in a tile: `sub` rows behind the unit's first one
 template <int FMT>
-__device__ __forceinline__ int unit_row(int unit, int sub) {
-    return FMT == SAMQ_FP4_MX ? unit + 32 * sub : 2 * unit + (sub >> 2) + 32 * (sub & 3);
-}
-constexpr int STAGED_PITCH = CHUNK + 1;
+__device__ __forceinline__ int first_row(int unit) { return FMT == SAMQ_FP4_MX ? unit : 2 * unit; }
+template <int FMT>
+__device__ __forceinline__ constexpr int row_offset(int sub) { return FMT == SAMQ_FP4_MX ? 32 * sub : (sub >> 2) + 32 * (sub & 3); }
+// elements between the chunks of two lanes in shared memory: an odd number of words, so that no two lanes meet in a bank
+template <typename T> constexpr int staged_pitch() { return sizeof(T) == 2 ? CHUNK + 2 : CHUNK + 1; }
 
 // STAGED: rows of x or fq that do not start on 16 bytes pass through shared memory
 template <typename T, int FMT, bool FQ, bool STAGED>
@@ -49,33 +52,46 @@ quant_fp4_kernel(const QuantFp4Params p)
     constexpr int UNITS = 128 / ROWS;                              // row units of a tile
     const int64_t tile = row_unit / UNITS;
     const int sub = lane / LANES;
-    const int r = unit_row<FMT>((int)(row_unit % UNITS), sub);
+    const int r0 = first_row<FMT>((int)(row_unit % UNITS)), r = r0 + row_offset<FMT>(sub);
     const int64_t row = tile * TILE_ROWS + r;
     const int64_t col = (group * LANES + lane % LANES) * CHUNK;
     const bool row_ok = row < p.M;
 
     const int left = row_ok ? (int)min((int64_t)CHUNK, p.K - col) : 0;          // columns of the chunk (0 or less: none)
     Chunk<T> x;
-    __shared__ T staged[STAGED ? WARPS * 32 * STAGED_PITCH : 1];
+    constexpr int STAGED_PITCH = staged_pitch<T>();
+    __shared__ __align__(16) T staged[STAGED ? WARPS * 32 * STAGED_PITCH : 1];
     T* const mine = staged + (STAGED ? warp * 32 * STAGED_PITCH : 0);
     constexpr int SPAN = LANES * CHUNK;                            // columns of a row in the warp
-    const int64_t first_col = group * SPAN;
+    const int64_t first_col = group * SPAN, row0 = tile * TILE_ROWS + r0;
+    const int cols = (int)max((int64_t)0, min((int64_t)SPAN, p.K - first_col));       // STAGED: the warp's columns and rows
+    const int rows_left = (int)min((int64_t)TILE_ROWS, p.M - row0);
     if constexpr (STAGED) {
         // rows that no vector may start at: the warp reads 32 neighbouring elements an instruction and turns them into
         // its lanes' chunks in shared memory
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
-            const int64_t rr = tile * TILE_ROWS + unit_row<FMT>((int)(row_unit % UNITS), i);
+            const T* src = static_cast<const T*>(p.x) + row0 * p.ldx + first_col + row_offset<FMT>(i) * p.ldx;
+            const int in = row_offset<FMT>(i) < rows_left ? cols : 0;
+            if (sizeof(T) == 2 && p.pairs) {
 #pragma unroll
-            for (int j = 0; j < SPAN; j += 32) {
-                const int c = j + lane;
-                const bool in = rr < p.M && first_col + c < p.K;
-                mine[(i * LANES + c / CHUNK) * STAGED_PITCH + c % CHUNK] = in ? static_cast<const T*>(p.x)[rr * p.ldx + first_col + c] : Elem<T>::down(0.0f);
+                for (int j = 0; j < SPAN; j += 64) {
+                    const int c = j + 2 * lane;
+                    *reinterpret_cast<uint32_t*>(mine + (i * LANES + c / CHUNK) * STAGED_PITCH + c % CHUNK) =
+                        c < in ? *reinterpret_cast<const uint32_t*>(src + c) : 0u;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < SPAN; j += 32) {
+                    const int c = j + lane;
+                    mine[(i * LANES + c / CHUNK) * STAGED_PITCH + c % CHUNK] = c < in ? src[c] : Elem<T>::down(0.0f);
+                }
             }
         }
         __syncwarp();
+        uint32_t* words = reinterpret_cast<uint32_t*>(&x);
 #pragma unroll
-        for (int i = 0; i < CHUNK; ++i) x.set(i, mine[lane * STAGED_PITCH + i]);
+        for (int i = 0; i < CHUNK * (int)sizeof(T) / 4; ++i) words[i] = reinterpret_cast<const uint32_t*>(mine + lane * STAGED_PITCH)[i];
         __syncwarp();
     } else {
         load_chunk(x, static_cast<const T*>(p.x) + row * p.ldx + col, left, p.access_x);
@@ -127,16 +143,26 @@ quant_fp4_kernel(const QuantFp4Params p)
         constexpr int WORDS = CHUNK * (int)sizeof(T) / 4;
         if constexpr (STAGED) {
 #pragma unroll
-            for (int i = 0; i < CHUNK; ++i) mine[lane * STAGED_PITCH + i] = t[i];
+            for (int i = 0; i < WORDS; ++i) reinterpret_cast<uint32_t*>(mine + lane * STAGED_PITCH)[i] = w[i];
             __syncwarp();
 #pragma unroll
             for (int i = 0; i < ROWS; ++i) {
-                const int64_t rr = tile * TILE_ROWS + unit_row<FMT>((int)(row_unit % UNITS), i);
+                T* dst = static_cast<T*>(p.fq) + row0 * p.K + first_col + row_offset<FMT>(i) * p.K;
+                const int in = row_offset<FMT>(i) < rows_left ? cols : 0;
+                if (sizeof(T) == 2 && p.pairs) {
 #pragma unroll
-                for (int j = 0; j < SPAN; j += 32) {
-                    const int c = j + lane;
-                    if (rr < p.M && first_col + c < p.K)
-                        static_cast<T*>(p.fq)[rr * p.K + first_col + c] = mine[(i * LANES + c / CHUNK) * STAGED_PITCH + c % CHUNK];
+                    for (int j = 0; j < SPAN; j += 64) {
+                        const int c = j + 2 * lane;
+                        if (c < in)
+                            *reinterpret_cast<uint32_t*>(dst + c) =
+                                *reinterpret_cast<const uint32_t*>(mine + (i * LANES + c / CHUNK) * STAGED_PITCH + c % CHUNK);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < SPAN; j += 32) {
+                        const int c = j + lane;
+                        if (c < in) dst[c] = mine[(i * LANES + c / CHUNK) * STAGED_PITCH + c % CHUNK];
+                    }
                 }
             }
         } else if (left >= CHUNK && p.access_fq == BY_32) {
@@ -201,6 +227,7 @@ int quant_fp4_dispatch(const void* x, int dtype, int64_t M, int64_t K, int64_t l
     p.col_blocks = (int)((p.groups + WARPS - 1) / WARPS);
     p.access_x = row_access(x, ldx * (int64_t)esz);
     p.access_fq = row_access(fq, K * (int64_t)esz);
+    p.pairs = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(fq) | (uintptr_t)((ldx | K) * (int64_t)esz)) & 3) == 0;
     p.vec_q = (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && ldq % 8 == 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (dtype) {
