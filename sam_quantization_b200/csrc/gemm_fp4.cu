@@ -133,38 +133,43 @@ __device__ __forceinline__ void finish_rows(const SmallParams& p, int n, float b
     }
 }
 
-// Quantization of `blocks` k-blocks of the activation from kb on, into the operand layout (128-byte swizzle) and scale
-// tiles of as many stages of the ring from `stage` on; rows behind M are zero.  A thread takes every EPI_THREADS-th chunk
-// of 16 columns, BATCH of them at a time: the loads of a batch are under way together, and may be while a stage is waited
-// for.  (A block has T * 16 chunks, a multiple of 128: whole warps leave the loops together.)
+// Quantization of `blocks` k-blocks of the activation's `rows` rows from kb on, into the operand layout (128-byte swizzle) and
+// scale tiles of as many stages of the ring from `stage` on.  (What the tile's other rows hold only meets output rows that do
+// not exist.)  Sixteen threads take the chunks of 16 columns of one row and block; 16 rows at a time, BATCH times: the loads
+// of a batch are under way together, and may be while a stage is waited for.
 constexpr int BATCH = 4;
-constexpr int CHUNKS = KPAD / 16;                // of a row and block
+constexpr int BATCH_ROWS = EPI_THREADS / 16;
+struct RowOf {                                   // idx = block * rows + row, for idx < 2048 and rows <= 32
+    int rows, inv;
+    __device__ __forceinline__ explicit RowOf(int rows_) : rows(rows_), inv((65536 + rows_ - 1) / rows_) {}
+    __device__ __forceinline__ int block(int idx) const { return (idx * inv) >> 16; }
+};
 
 template <typename T>
-__device__ __forceinline__ void load_batch(const SmallParams& p, int m0, int kb, int blocks, int first, Chunk<T> (&x)[BATCH]) {
-    const int per_block = p.T * CHUNKS;
+__device__ __forceinline__ void load_batch(const SmallParams& p, const RowOf& of, int m0, int kb, int blocks, int first, int tid, Chunk<T> (&x)[BATCH]) {
+    const int total = blocks * of.rows;
 #pragma unroll
     for (int u = 0; u < BATCH; ++u) {
-        const int c = first + u * EPI_THREADS;
-        if (c >= per_block * blocks) break;
-        const int b = c / per_block, r = c % per_block / CHUNKS, col = (kb + b) * KPAD + c % CHUNKS * 16;
-        load_chunk(x[u], static_cast<const T*>(p.x) + (int64_t)(m0 + r) * p.ldx + col, m0 + r < p.M ? min(16, p.K - col) : 0, p.access_x);
+        if (first + u * BATCH_ROWS >= total) break;                // the same in all threads; those behind the end repeat the last row
+        const int idx = min(first + u * BATCH_ROWS + (tid >> 4), total - 1), b = of.block(idx), r = idx - b * of.rows;
+        const int col = (kb + b) * KPAD + (tid & 15) * 16;
+        load_chunk(x[u], static_cast<const T*>(p.x) + (int64_t)(m0 + r) * p.ldx + col, min(16, p.K - col), p.access_x);
     }
 }
 template <typename T, int FMT>
-__device__ __forceinline__ void quantize_batch(const SmallParams& p, int kb, int blocks, int first, int stage, const Chunk<T> (&x)[BATCH],
-                                               uint8_t* tiles, int st_bytes, uint8_t* sf) {
-    const int per_block = p.T * CHUNKS;
+__device__ __forceinline__ void quantize_batch(const SmallParams& p, const RowOf& of, int kb, int blocks, int first, int tid, int stage,
+                                               const Chunk<T> (&x)[BATCH], uint8_t* tiles, int st_bytes, uint8_t* sf) {
+    const int total = blocks * of.rows, j = tid & 15, block = j * 16 / block_of(FMT);
 #pragma unroll
     for (int u = 0; u < BATCH; ++u) {
-        const int c = first + u * EPI_THREADS;
-        if (c >= per_block * blocks) break;
-        const int b = c / per_block, r = c % per_block / CHUNKS, j = c % CHUNKS, s = (stage + b) % p.stages;
+        if (first + u * BATCH_ROWS >= total) break;
+        const int idx = min(first + u * BATCH_ROWS + (tid >> 4), total - 1), b = of.block(idx), r = idx - b * of.rows;
+        const int s = stage + b < p.stages ? stage + b : stage + b - p.stages;
         uint32_t amax = x[u].amax_bits();
         if constexpr (FMT == SAMQ_FP4_MX) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         const Scale sc = block_scale<FMT>(amax, 1.0f, 1.0f);
-        *reinterpret_cast<uint2*>(tiles + (size_t)s * st_bytes + W_BYTES + staged(r, j * 8)) = encode_chunk<FMT>(x[u], sc, amax < 0x7F800000u);
-        const int block = j * 16 / block_of(FMT);
+        *reinterpret_cast<uint2*>(tiles + (size_t)s * st_bytes + W_BYTES + r * BK + ((uint32_t)(j * 8) ^ ((uint32_t)(r & 7) << 4))) =
+            encode_chunk<FMT>(x[u], sc, amax < 0x7F800000u);
         if (FMT == SAMQ_FP4_NV || (j & 1) == 0)
             sf[(size_t)(2 * s + 1) * Shape<FMT>::SF_BYTES + (block / 4) * TILE_BYTES + r * 16 + (block & 3)] =
                 (uint8_t)((kb + b) * KPAD + block * block_of(FMT) < p.K ? sc.byte : 0u);
@@ -210,8 +215,8 @@ gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     const int own_max = owned_rows(rows, split);
     const int owned = max(0, min(own_max, rows - rank * own_max));  // rows of this CTA, from rank * own_max on
 
-    // The set-up of the roles runs side by side: the first warp makes the barriers and sends the first loads off, the
-    // second allocates tensor memory, the others quantize as many blocks as there are stages.
+    // The set-up of the roles runs side by side: the first warp makes the barriers, lets the others pass and sends the first
+    // loads off, the second allocates tensor memory, the others quantize as many blocks as there are stages.
     if (warp == 0) {
         if (elect_one()) {
             for (int s = 0; s < stages; ++s) { mbar_init(smem_u32(&ctl->full[s]), QUANT ? 1 + EPI_THREADS : 1); mbar_init(smem_u32(&ctl->empty[s]), 1); }
@@ -220,6 +225,10 @@ gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
             ctl->abort_flag = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             if (split > 1) mbar_expect_tx(smem_u32(&ctl->joined), (uint32_t)(split * owned * BW) * 4u);
+        }
+        __syncwarp();
+        asm volatile("bar.arrive 1, %0;" ::"r"(THREADS) : "memory");
+        if (elect_one()) {
             for (int i = 0; i < min(kb_count, stages); ++i) load_stage(i);
         }
         __syncwarp();
@@ -229,18 +238,21 @@ gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     } else if constexpr (QUANT) {
         const int tid = threadIdx.x - 64, blocks = min(kb_count, stages);
-        for (int c = tid; c < blocks * p.T * CHUNKS; c += BATCH * EPI_THREADS) {
+        const RowOf of(rows);
+        for (int first = 0; first < blocks * rows; first += BATCH * BATCH_ROWS) {
             Chunk<OutT> x[BATCH];
-            load_batch(p, m0, kb_first, blocks, c, x);
-            quantize_batch<OutT, FMT>(p, kb_first, blocks, c, 0, x, tiles, st_bytes, sf);
+            load_batch(p, of, m0, kb_first, blocks, first, tid, x);
+            quantize_batch<OutT, FMT>(p, of, kb_first, blocks, first, tid, 0, x, tiles, st_bytes, sf);
         }
         fence_async_smem();
     }
-    tcgen05_fence_before();
-    __syncthreads();
-    tcgen05_fence_after();
+    if (warp > 0) {
+        tcgen05_fence_before();
+        asm volatile("bar.sync 1, %0;" ::"r"(THREADS) : "memory");
+        tcgen05_fence_after();
+    }
     if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");    // this CTA's barriers exist
-    const uint32_t tmem = ctl->tmem_base;
+    const uint32_t tmem = warp > 0 ? ctl->tmem_base : 0u;          // (the first warp has not waited for it, and does not need it)
 
     if (warp == 0) {
         bool ok = true;
@@ -291,15 +303,16 @@ gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
             const int tid = threadIdx.x - 64;
             for (int i = 0; i < min(kb_count, stages); ++i) mbar_arrive(smem_u32(&ctl->full[i]));
             // the others a few blocks at a time: half of the ring, and no more than one batch
-            const int group = max(1, min(stages / 2, BATCH * EPI_THREADS / (p.T * CHUNKS)));
+            const int group = max(1, min(stages / 2, BATCH * BATCH_ROWS / rows));
+            const RowOf of(rows);
             bool ok = true;
             for (int i = stages; i < kb_count && ok; i += group) {
                 const int blocks = min(group, kb_count - i);
                 Chunk<OutT> x[BATCH];
-                load_batch(p, m0, kb_first + i, blocks, tid, x);
+                load_batch(p, of, m0, kb_first + i, blocks, 0, tid, x);
                 for (int k = i; k < i + blocks && ok; ++k) ok = mbar_wait(smem_u32(&ctl->empty[k % stages]), ((k / stages) & 1) ^ 1u, abort_flag);
                 if (!ok) break;
-                quantize_batch<OutT, FMT>(p, kb_first + i, blocks, tid, i % stages, x, tiles, st_bytes, sf);
+                quantize_batch<OutT, FMT>(p, of, kb_first + i, blocks, 0, tid, i % stages, x, tiles, st_bytes, sf);
                 fence_async_smem();
                 for (int k = i; k < i + blocks; ++k) mbar_arrive(smem_u32(&ctl->full[k % stages]));
             }
