@@ -323,10 +323,13 @@ int samq_gemm_fp4(const uint8_t* A, int64_t lda, const uint8_t* a_scales, const 
                   int activation, void* out, int out_dtype, int64_t ldo, int32_t* status, void* stream);
 
 /* A 4-bit linear layer: x [M, K] of `dtype`, row stride ldx, is quantized as samq_quant_fp4 does with global_scale 1 and
- * multiplied as in samq_gemm_fp4.  Up to SAMQ_LINEAR_FP4_ONE_KERNEL_ROWS rows with dtype == out_dtype it is one kernel and
- * takes no workspace (it may be NULL); otherwise the quantized activation lives in `workspace`, 16-byte aligned and of
- * samq_linear_fp4_workspace_bytes() at least, until the call's work on the stream is done. */
+ * multiplied as in samq_gemm_fp4.  Up to SAMQ_LINEAR_FP4_ONE_KERNEL_ROWS rows with dtype == out_dtype it can be one kernel,
+ * and `workspace` may be NULL; otherwise the quantized activation lives in `workspace`, 16-byte aligned and of
+ * samq_linear_fp4_workspace_bytes() at least, until the call's work on the stream is done.  Few rows with
+ * (M + 8) * ceil(K / 256) > SAMQ_LINEAR_FP4_ONE_KERNEL_WORK take a workspace too if they are given one, where two kernels are
+ * faster; both ways give the same output. */
 #define SAMQ_LINEAR_FP4_ONE_KERNEL_ROWS 32
+#define SAMQ_LINEAR_FP4_ONE_KERNEL_WORK 256
 size_t samq_linear_fp4_workspace_bytes(int format, int64_t M, int64_t K);
 int samq_linear_fp4(const void* x, int dtype, int64_t ldx, const uint8_t* W, int64_t ldw, const uint8_t* w_scales,
                     int64_t M, int64_t N, int64_t K, int format, float alpha, const void* bias, const void* residual, int64_t ldr,

@@ -18,7 +18,7 @@ GRAN_ROW, GRAN_TENSOR, GRAN_GROUP = 0, 1, 2
 ACT_NONE, ACT_GELU = 0, 1
 HAD_NONE, HAD_FULL, HAD_PARTIAL = 0, 1, 2
 FP4_MX, FP4_NV = 0, 1
-LINEAR_FP4_ONE_KERNEL_ROWS = 32
+LINEAR_FP4_ONE_KERNEL_ROWS, LINEAR_FP4_ONE_KERNEL_WORK = 32, 256
 
 EXPORTED_SYMBOLS = (
     "samq_version",

@@ -29,7 +29,7 @@ constexpr int W_BYTES = BW * BK;
 constexpr int EPI_WARPS = 8;                     // two for each quarter of the 128 columns, taking turns by 16 rows
 constexpr int EPI_THREADS = EPI_WARPS * 32;
 constexpr int THREADS = 64 + EPI_THREADS;
-constexpr int FUSED_MAX_ROWS = SAMQ_LINEAR_FP4_ONE_KERNEL_ROWS;
+constexpr int FUSED_MAX_ROWS = SAMQ_LINEAR_FP4_ONE_KERNEL_ROWS, FUSED_MOST = SAMQ_LINEAR_FP4_ONE_KERNEL_WORK;
 
 struct __align__(8) Control {
     uint64_t full[MAX_STAGES];
@@ -64,18 +64,19 @@ template <int FMT> struct Shape {
 };
 template <int FMT>
 __host__ __device__ constexpr int stage_bytes(int T) { return W_BYTES + T * BK; }
+inline int tile_rows(int64_t M) { return M >= MAX_T ? MAX_T : (int)((M + 7) / 8 * 8); }
 // rows of a tile that one of `split` CTAs owns, at most
 __host__ __device__ inline int owned_rows(int rows, int split) { return (rows + split - 1) / split; }
 constexpr size_t HALF_SM = 112 * 1024;           // shared memory of one of two CTAs on an SM
+inline size_t joined_bytes(int T, int split) { return split > 1 ? (size_t)split * owned_rows(T, split) * BW * sizeof(float) : 0; }
 template <int FMT>
-int stages_of(int T) {
-    const int n = (int)((HALF_SM - 2048) / (stage_bytes<FMT>(T) + 2 * Shape<FMT>::SF_BYTES));
+int stages_of(int T, int split) {
+    const int n = (int)((HALF_SM - 2048 - (T <= 32 ? joined_bytes(T, split) : 0)) / (stage_bytes<FMT>(T) + 2 * Shape<FMT>::SF_BYTES));
     return n < MIN_STAGES ? MIN_STAGES : n > MAX_STAGES ? MAX_STAGES : n;
 }
 template <int FMT>
 size_t smem_bytes(int T, int stages, int split) {
-    return 1024 + (size_t)stages * (stage_bytes<FMT>(T) + 2 * Shape<FMT>::SF_BYTES) +
-           (split > 1 ? (size_t)split * owned_rows(T, split) * BW * sizeof(float) : 0) + sizeof(Control);
+    return 1024 + (size_t)stages * (stage_bytes<FMT>(T) + 2 * Shape<FMT>::SF_BYTES) + joined_bytes(T, split) + sizeof(Control);
 }
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -386,11 +387,48 @@ gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     if (split > 1 && *abort_flag != 0) cluster_sync();
 }
 
+// as much shared memory as the largest tile takes
+constexpr size_t SMEM_MOST = 227 * 1024;
+
+// How many clusters of `split` CTAs, two an SM, are on the device at once: fewer than its CTAs divided by `split`, since a
+// cluster stays within one of the device's groups of SMs.  The runtime answers for one CTA an SM (15 clusters of eight, 22 of
+// six, 33 of four), the same for every form of the kernel; a property of the device, asked for once.
+int active_clusters(int split) {
+    static thread_local int known[64][MAX_SPLIT + 1] = {};
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return 2 * (sm_count() / split); }
+    if (known[dev][split] > 0) return known[dev][split];
+    auto kernel = gemm_fp4_small_kernel<__half, SAMQ_FP4_NV, true>;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((unsigned)split); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = HALF_SM + HALF_SM / 2;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_MOST) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        return 2 * (sm_count() / split);
+    }
+    return known[dev][split] = 2 * n;
+}
+
+// Split K while SMs are idle, but leave a CTA four blocks of 256 columns at least: joining two halves costs about as much as
+// two more blocks (one token, 1280 -> 3840: 6.2 us whole, 6.6 us in two; 5120 -> 1280: 16.4 and 8.2 in five).  All clusters
+// are on the device at once: one token, 10240 -> 5120 takes 11.6 us in six and 20 in seven, 36 of whose 40 clusters fit.
+int split_of(const Fp4Call& c, int T) {
+    const int64_t tiles = (c.N + BW - 1) / BW * ((c.M + MAX_T - 1) / MAX_T), k_blocks = (c.K + KPAD - 1) / KPAD;
+    const int64_t room = (T <= 32 ? 2 : 1) * (int64_t)sm_count() / tiles;
+    const int64_t most = k_blocks / 4 < room ? k_blocks / 4 : room;
+    int split = (int)(most < 1 ? 1 : most > MAX_SPLIT ? MAX_SPLIT : most);
+    while (split > 1 && tiles > active_clusters(split) / (T <= 32 ? 1 : 2)) --split;
+    return split;
+}
+
 template <typename OutT, int FMT, bool QUANT>
 int launch_small(const Fp4Call& c, SmallParams& p, const CUtensorMap& ma, const CUtensorMap& mw) {
     auto kernel = gemm_fp4_small_kernel<OutT, FMT, QUANT>;
-    // as much shared memory as the largest tile takes, set once per device
-    constexpr size_t SMEM_MOST = 227 * 1024;
     static thread_local bool ready[64] = {false};
     int dev = 0;
     SAMQ_CUDA_TRY(cudaGetDevice(&dev));
@@ -399,13 +437,8 @@ int launch_small(const Fp4Call& c, SmallParams& p, const CUtensorMap& ma, const 
         if (dev >= 0 && dev < 64) ready[dev] = true;
     }
     const int64_t n_tiles = (c.N + BW - 1) / BW, m_tiles = (c.M + MAX_T - 1) / MAX_T;
-    const int64_t k_blocks = (c.K + KPAD - 1) / KPAD;
-    // Split K while SMs are idle, but leave a CTA four blocks of 256 columns at least: joining two halves costs about as
-    // much as two more blocks (one token, 1280 -> 3840: 6.2 us whole, 6.6 us in two; 5120 -> 1280: 16.4 and 8.2 in five).
-    const int64_t room = (p.T <= 32 ? 2 : 1) * sm_count() / (n_tiles * m_tiles);
-    int64_t most = k_blocks / 4 < room ? k_blocks / 4 : room;
-    const int split = (int)(most < 1 ? 1 : most > MAX_SPLIT ? MAX_SPLIT : most);
-    p.stages = stages_of<FMT>(p.T);
+    const int split = split_of(c, p.T);
+    p.stages = stages_of<FMT>(p.T, split);
     if (n_tiles * split > 2147483647LL || m_tiles > 65535) return fail(SAMQ_ERR_TOO_LARGE, "product of %lld x %lld outputs is too large", (long long)c.M, (long long)c.N);
     const int cols = p.T + 2 * Shape<FMT>::SF_COLS;
     p.tmem_cols = cols <= 64 ? 64 : cols <= 128 ? 128 : 256;
@@ -433,7 +466,7 @@ int launch_small(const Fp4Call& c, SmallParams& p, const CUtensorMap& ma, const 
 int gemm_fp4_small(const Fp4Call& c, const void* x, int64_t ldx) {
     SmallParams p;
     p.M = (int)c.M; p.N = (int)c.N; p.K = (int)c.K;
-    p.T = c.M >= MAX_T ? MAX_T : (int)((c.M + 7) / 8 * 8);
+    p.T = tile_rows(c.M);
     p.groups = (int)groups_of(c.fmt, c.K); p.a_scales = c.a_scales; p.w_scales = c.w_scales;
     const size_t esz = c.out_dtype == SAMQ_F32 ? 4 : 2;
     p.x = x; p.ldx = ldx; p.access_x = row_access(x, ldx * (int64_t)esz);
@@ -539,9 +572,18 @@ int linear_fp4_dispatch(const void* x, int dtype, int64_t ldx, const uint8_t* W,
     if (x == nullptr) return fail(SAMQ_ERR_BAD_ARG, "x must not be null");
     if (ldx < K) return fail(SAMQ_ERR_BAD_ARG, "ldx smaller than K");
     if (reinterpret_cast<uintptr_t>(x) & (dtype == SAMQ_F32 ? 3 : 1)) return fail(SAMQ_ERR_ALIGNMENT, "x must be aligned to its elements");
-    if (M <= FUSED_MAX_ROWS && dtype == out_dtype) return gemm_fp4_small(c, x, ldx);
     const int64_t pitch = (K + 31) / 32 * 16;
     const size_t need = linear_fp4_workspace(fmt, M, K);
+    if (M <= FUSED_MAX_ROWS && dtype == out_dtype) {
+        // Every CTA quantizes all rows of its share of K: where that is much, and there is a workspace, the quantizer runs
+        // first.  us, one kernel / two: 32 rows, 1280 -> 5120 (a share of 5 blocks) 8.1 / 7.6, but the second launch costs
+        // the host 3 us; 32, 5120 -> 10240 (7) 17.5 / 13.8; 8, 10240 -> 10240 (14) 17.4 / 18.2, 16 20.9 / 18.2; 8, 5120 ->
+        // 20000 (20) 19.0 / 17.3; 1, 10240 -> 20000 (40) 32.5 / 26.3.
+        const int64_t k_blocks = (K + KPAD - 1) / KPAD;
+        if (workspace == nullptr || workspace_bytes < need || (M + 8) * k_blocks <= FUSED_MOST) return gemm_fp4_small(c, x, ldx);
+        const int split = split_of(c, tile_rows(M));
+        if ((M + 8) * ((k_blocks + split - 1) / split) <= FUSED_MOST) return gemm_fp4_small(c, x, ldx);
+    }
     if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))
         return fail(SAMQ_ERR_WORKSPACE, "the 4-bit linear needs %zu bytes of 16-byte aligned workspace", need);
     uint8_t* codes = static_cast<uint8_t*>(workspace);

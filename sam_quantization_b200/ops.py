@@ -650,9 +650,10 @@ def linear_fp4(x: torch.Tensor, w: Fp4Tensor, bias: Optional[torch.Tensor] = Non
     code, bias, residual, ldr = _linear_args(N, M, bias, residual, out_dtype, dev)
     out = x.new_empty((*x.shape[:-1], N), dtype=out_dtype)
     ws, ws_bytes, kernels = None, 0, 1
-    if M > _lib.LINEAR_FP4_ONE_KERNEL_ROWS or code != xcode:
+    two = M > _lib.LINEAR_FP4_ONE_KERNEL_ROWS or code != xcode
+    if two or (M + 8) * ((K + 255) // 256) > _lib.LINEAR_FP4_ONE_KERNEL_WORK:      # (the latter may use it)
         ws_bytes = lib.samq_linear_fp4_workspace_bytes(fcode, M, K)
-        ws, kernels = x.new_empty((ws_bytes,), dtype=torch.uint8), 2
+        ws, kernels = x.new_empty((ws_bytes,), dtype=torch.uint8), 1 + two
     _call(dev, "linear_fp4", 2.0 * M * N * K, lib.samq_linear_fp4, x2.data_ptr(), xcode, ldx, wc.data_ptr(), wc.stride(0), w.scales.data_ptr(),
           M, N, K, fcode, w.global_scale, _data_ptr(bias), _data_ptr(residual), ldr, activation, out.data_ptr(), code, N,
           _data_ptr(ws), ws_bytes, _status_ptr(dev), kernels=kernels)

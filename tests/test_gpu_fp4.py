@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from oracle import fp4 as F
-from sam_quantization_b200 import ops
+from sam_quantization_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 FORMATS = ["mxfp4", "nvfp4"]
@@ -216,6 +216,23 @@ def test_one_kernel_layer_equals_its_two_halves(cuda_device, fmt, dtype, M, N, K
     wide[:, 3:K + 3] = x
     assert _same_bytes(ops.linear_fp4(wide[:, 3:K + 3], w, bias=bias.to(cuda_device), residual=res.to(cuda_device)), y)
     assert ops.linear_fp4(x.view(M, 1, K), w).shape == (M, 1, N)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N,K", [(1, 700, 10240), (9, 5003, 5130), (16, 20000, 5120), (24, 2700, 4099), (32, 10240, 5120), (32, 640, 1290)])
+def test_layer_of_few_rows_is_the_same_with_and_without_a_workspace(cuda_device, fmt, M, N, K):
+    """Given a workspace, the library may quantize first; the sums are the same, in the same order.  Clusters of every size."""
+    lib, g = _lib.load(), torch.Generator().manual_seed(M + N)
+    x = torch.randn(M, K, generator=g).to(torch.bfloat16).to(cuda_device)
+    w = ops.quantize_fp4(torch.randn(N, K, generator=g).to(torch.bfloat16).to(cuda_device), fmt)["q"]
+    y = ops.linear_fp4(x, w)
+    two = ops.gemm_fp4(ops.quantize_fp4(x, fmt)["q"], w, out_dtype=torch.bfloat16)
+    one = torch.empty_like(y)
+    rc = lib.samq_linear_fp4(x.data_ptr(), _lib.BF16, K, w.codes.data_ptr(), w.codes.stride(0), w.scales.data_ptr(), M, N, K, ops.FP4_FORMATS[fmt],
+                             w.global_scale, None, None, 0, 0, one.data_ptr(), _lib.BF16, N, None, 0, None, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    ops.check_status()
+    assert _same_bytes(y, two) and _same_bytes(one, two)
 
 
 def _same_bytes(a, b):
