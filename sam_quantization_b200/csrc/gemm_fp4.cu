@@ -100,11 +100,20 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
     tmem_ld_wait();
 }
 
-// 16 neighbouring rows of output column n from row m on, `count` of them: the sums in y
-template <typename OutT>
-__device__ __forceinline__ void finish_rows(const SmallParams& p, int n, float bias, int64_t m, int count, float (&y)[16]) {
-    OutT* out = static_cast<OutT*>(p.out) + m * p.ldo + n;
+// The residual under up to 16 neighbouring rows of output column n from row m on, asked for before the sums are there: its
+// way from memory is a good part of a small call (2777 x 1001 x 1283, 176 CTAs of 4 x 16 rows a warp: 14.3 -> 12.0 us).
+template <typename OutT, bool RES>
+__device__ __forceinline__ void load_residual(const SmallParams& p, int n, int64_t m, int count, OutT (&r)[16]) {
+    if (!RES || n >= p.N) return;
     const OutT* res = static_cast<const OutT*>(p.residual) + m * p.ldr + n;
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+        if (j < count) { r[j] = *res; res += p.ldr; }
+}
+// those rows' outputs: the sums in y
+template <typename OutT, bool RES>
+__device__ __forceinline__ void finish_rows(const SmallParams& p, int n, float bias, int64_t m, int count, float (&y)[16], const OutT (&r)[16]) {
+    OutT* out = static_cast<OutT*>(p.out) + m * p.ldo + n;
     const bool all = count >= 16;                                   // the same in all threads, as the other branches here
 #pragma unroll
     for (int j = 0; j < 16; ++j) y[j] = fmaf(y[j], p.alpha, bias);
@@ -115,11 +124,7 @@ __device__ __forceinline__ void finish_rows(const SmallParams& p, int n, float b
             y[j] = g.x; y[j + 1] = g.y;
         }
     }
-    if (p.residual != nullptr) {
-        OutT r[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-            if (all || j < count) { r[j] = *res; res += p.ldr; }
+    if (RES) {
 #pragma unroll
         for (int j = 0; j < 16; ++j)
             if (all || j < count) y[j] += OutOps<OutT>::up(r[j]);
@@ -177,8 +182,9 @@ __device__ __forceinline__ void quantize_batch(const SmallParams& p, const RowOf
     }
 }
 
-// QUANT: the activation is `x` of type OutT, quantized here; otherwise codes and scales are loaded.
-template <typename OutT, int FMT, bool QUANT>
+// QUANT: the activation is `x` of type OutT, quantized here; otherwise codes and scales are loaded.  RES: with a residual
+// (whose registers cost a call without one 0.3 us).
+template <typename OutT, int FMT, bool QUANT, bool RES>
 __global__ void __launch_bounds__(THREADS, 2)
 gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const SmallParams p)
 {
@@ -326,17 +332,27 @@ gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         const int col = (warp & 3) * 32 + lane, n = n0 + col;
         const uint32_t acc = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const float bias = (p.bias != nullptr && n < p.N) ? OutOps<OutT>::up(static_cast<const OutT*>(p.bias)[n]) : 0.0f;
+        const int turn = 16 * ((warp - 2) >> 2);                    // this warp's rows: every second sixteen
+        const int first_row = split == 1 ? m0 : m0 + rank * own_max, mine = split == 1 ? rows : owned;
+        OutT res[2][16] = {};                                       // of this turn and the next
+        load_residual<OutT, RES>(p, n, first_row + turn, mine - turn, res[0]);
+        load_residual<OutT, RES>(p, n, first_row + turn + 32, mine - turn - 32, res[1]);
         if (mbar_wait(smem_u32(&ctl->acc_full), 0, abort_flag)) {
             tcgen05_fence_after();
-            const int turn = 16 * ((warp - 2) >> 2);                // this warp's rows: every second sixteen
             if (split == 1) {
-                for (int c = turn; c < rows; c += 32) {
-                    uint32_t r[16];
-                    tmem_ld16(acc + (uint32_t)c, r);
-                    float y[16];
+                for (int c = turn; c < rows; c += 64) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) y[j] = __uint_as_float(r[j]);
-                    if (n < p.N) finish_rows<OutT>(p, n, bias, m0 + c, rows - c, y);
+                    for (int h = 0; h < 2; ++h) {
+                        const int at = c + 32 * h;
+                        if (at >= rows) break;
+                        uint32_t r[16];
+                        tmem_ld16(acc + (uint32_t)at, r);
+                        float y[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) y[j] = __uint_as_float(r[j]);
+                        if (n < p.N) finish_rows<OutT, RES>(p, n, bias, m0 + at, rows - at, y, res[h]);
+                        load_residual<OutT, RES>(p, n, m0 + at + 64, rows - at - 64, res[h]);
+                    }
                 }
             } else {
                 const uint32_t bar = smem_u32(&ctl->joined);
@@ -358,7 +374,10 @@ gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                     }
                 }
                 if (turn < owned && mbar_wait_cluster(bar, 0, abort_flag) && n < p.N) {
-                    for (int k = turn; k < owned; k += 32) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {                   // two turns at most: half of 128 rows
+                        const int k = turn + 32 * h;
+                        if (k >= owned) break;
                         const float* from = joined + k * BW + col;
                         float y[16];
 #pragma unroll
@@ -367,9 +386,10 @@ gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
 #pragma unroll
                             for (int j = 0; j < 16; ++j) if (k + j < owned) y[j] += from[j * BW];
                         }
-                        finish_rows<OutT>(p, n, bias, m0 + rank * own_max + k, owned - k, y);
+                        finish_rows<OutT, RES>(p, n, bias, first_row + k, owned - k, y, res[h]);
                     }
                 }
+                static_assert(MAX_T / 2 <= 64, "rows of one of two CTAs in two turns");
             }
         }
         tcgen05_fence_before();
@@ -398,7 +418,7 @@ int active_clusters(int split) {
     int dev = 0, n = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return 2 * (sm_count() / split); }
     if (known[dev][split] > 0) return known[dev][split];
-    auto kernel = gemm_fp4_small_kernel<__half, SAMQ_FP4_NV, true>;
+    auto kernel = gemm_fp4_small_kernel<__half, SAMQ_FP4_NV, true, false>;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
@@ -426,9 +446,9 @@ int split_of(const Fp4Call& c, int T) {
     return split;
 }
 
-template <typename OutT, int FMT, bool QUANT>
+template <typename OutT, int FMT, bool QUANT, bool RES>
 int launch_small(const Fp4Call& c, SmallParams& p, const CUtensorMap& ma, const CUtensorMap& mw) {
-    auto kernel = gemm_fp4_small_kernel<OutT, FMT, QUANT>;
+    auto kernel = gemm_fp4_small_kernel<OutT, FMT, QUANT, RES>;
     static thread_local bool ready[64] = {false};
     int dev = 0;
     SAMQ_CUDA_TRY(cudaGetDevice(&dev));
@@ -462,6 +482,20 @@ int launch_small(const Fp4Call& c, SmallParams& p, const CUtensorMap& ma, const 
     return SAMQ_OK;
 }
 
+template <typename OutT>
+int launch_form(int form, const Fp4Call& c, SmallParams& p, const CUtensorMap& ma, const CUtensorMap& mw) {
+    switch (form) {
+    case 0:  return launch_small<OutT, SAMQ_FP4_NV, false, false>(c, p, ma, mw);
+    case 1:  return launch_small<OutT, SAMQ_FP4_NV, false, true>(c, p, ma, mw);
+    case 2:  return launch_small<OutT, SAMQ_FP4_MX, false, false>(c, p, ma, mw);
+    case 3:  return launch_small<OutT, SAMQ_FP4_MX, false, true>(c, p, ma, mw);
+    case 4:  return launch_small<OutT, SAMQ_FP4_NV, true, false>(c, p, ma, mw);
+    case 5:  return launch_small<OutT, SAMQ_FP4_NV, true, true>(c, p, ma, mw);
+    case 6:  return launch_small<OutT, SAMQ_FP4_MX, true, false>(c, p, ma, mw);
+    default: return launch_small<OutT, SAMQ_FP4_MX, true, true>(c, p, ma, mw);
+    }
+}
+
 // x != nullptr: quantize it in the kernel
 int gemm_fp4_small(const Fp4Call& c, const void* x, int64_t ldx) {
     SmallParams p;
@@ -478,16 +512,12 @@ int gemm_fp4_small(const Fp4Call& c, const void* x, int64_t ldx) {
     if (rc == SAMQ_OK && x == nullptr) rc = make_operand_map(&ma, reinterpret_cast<const int8_t*>(c.A), c.M, row_bytes, c.lda, p.T);
     if (rc != SAMQ_OK) return rc;
     if (x != nullptr) ma = mw;                                      // not used
-    const bool mx = c.fmt == SAMQ_FP4_MX;
-#define SAMQ_SMALL(T)                                                                                                        \
-    (x != nullptr ? (mx ? launch_small<T, SAMQ_FP4_MX, true>(c, p, ma, mw) : launch_small<T, SAMQ_FP4_NV, true>(c, p, ma, mw)) \
-                  : (mx ? launch_small<T, SAMQ_FP4_MX, false>(c, p, ma, mw) : launch_small<T, SAMQ_FP4_NV, false>(c, p, ma, mw)))
+    const int form = (x != nullptr ? 4 : 0) + (c.fmt == SAMQ_FP4_MX ? 2 : 0) + (p.residual != nullptr ? 1 : 0);
     switch (c.out_dtype) {
-    case SAMQ_F16:  return SAMQ_SMALL(__half);
-    case SAMQ_BF16: return SAMQ_SMALL(__nv_bfloat16);
-    default:        return SAMQ_SMALL(float);
+    case SAMQ_F16:  return launch_form<__half>(form, c, p, ma, mw);
+    case SAMQ_BF16: return launch_form<__nv_bfloat16>(form, c, p, ma, mw);
+    default:        return launch_form<float>(form, c, p, ma, mw);
     }
-#undef SAMQ_SMALL
 }
 
 // What both entry points check: everything but the activation.
