@@ -1,4 +1,4 @@
-"""CPU checker of the RMS norm with an 8-bit output and of the microscaled 4-bit format, in 64 bits (numpy).
+"""CPU oracle of the RMS norm with an 8-bit output and of the microscaled 4-bit format, in 64 bits (numpy).
 
 Written from the definitions in include/samq.h; shares nothing with the CUDA path.  Test-only."""
 import numpy as np

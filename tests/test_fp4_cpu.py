@@ -1,4 +1,4 @@
-"""The 4-bit format and the RMS norm without a GPU: the checker against known values, host helpers, and every refusal
+"""The 4-bit format and the RMS norm without a GPU: the oracle against known values, host helpers, and every refusal
 (argument checks answer before any device work)."""
 import math
 
@@ -11,7 +11,7 @@ from sam_quantization_b200 import _lib, ops
 from tests.test_abi_cpu import built_library
 
 
-def test_checker_rounds_to_nearest_even_codes():
+def test_oracle_rounds_to_nearest_even_codes():
     x = np.zeros((1, 32))
     x[0, :16] = [0.25, 0.26, 0.75, 0.74, 1.25, 1.75, 2.5, 3.5, 5.0, 5.1, 7.9, -0.75, -0.0, 0.5, -6.0, 4.0]
     code, byte, value = F.quantize(x, "mxfp4")                          # largest 7.9 -> scale 2^0
@@ -23,7 +23,7 @@ def test_checker_rounds_to_nearest_even_codes():
     assert len(F.E4M3) == 127 and F.E4M3[0x7E] == 448 and F.E4M3[1] == 2.0 ** -9
 
 
-def test_checker_layout_places_every_scale_once():
+def test_oracle_layout_places_every_scale_once():
     byte = np.arange(200 * 20).reshape(200, 20).astype(np.uint8)
     t = F.tile_scales(byte, "nvfp4", 20 * 16)
     assert t.shape == (2, 8, 32, 4, 4) == ops.fp4_scale_shape("nvfp4", 200, 320)

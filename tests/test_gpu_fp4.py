@@ -1,4 +1,4 @@
-"""Microscaled 4-bit floating point on the GPU: the quantizer bit for bit against the 64-bit checker, the product
+"""Microscaled 4-bit floating point on the GPU: the quantizer bit for bit against the 64-bit oracle, the product
 exactly where its sums are exact, and within derived bounds elsewhere."""
 import numpy as np
 import pytest
@@ -34,7 +34,7 @@ def _check_quantized(x, out, fmt, g=1.0):
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("M,K", [(1, 1), (1, 16), (3, 31), (5, 33), (128, 256), (129, 257), (130, 1282), (131, 1283), (40, 70), (7, 5120), (300, 64), (33, 1023)])
-def test_quantizer_equals_the_checker(cuda_device, fmt, dtype, M, K):
+def test_quantizer_equals_the_oracle(cuda_device, fmt, dtype, M, K):
     x = _values(M, K, dtype)
     _check_quantized(x, ops.quantize_fp4(x.to(cuda_device), fmt, fake_quant=True), fmt)
 
