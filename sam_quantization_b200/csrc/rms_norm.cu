@@ -8,7 +8,7 @@
 // One pass: a row stays in registers between the two reductions (sum of squares, largest magnitude).  Bound: HBM,
 // 2 + 2 + 2 + 1 bytes an element of a 16-bit type (x, residual, h, q), 2 more for the dequantized values.  A row is kept
 // in its own type (60 registers instead of 110 of fp32: 66.3 -> 61.5 us).  Measured, 32768 x 1280 fp16 with residual and
-// values: 61.5 us, 6.1 TB/s; without a residual 28.3; widths that only 4 bytes divide 74, odd ones 130.
+// values: 61.5 us, 6.1 TB/s; without a residual 28.3; 1278 columns (4-byte accesses) 76, 1279 82.
 #include "common.cuh"
 #include <type_traits>
 
@@ -59,6 +59,10 @@ template <typename T, int E> struct Vec {
     __device__ __forceinline__ void load(const T* p) {
         raw = *reinterpret_cast<const Raw*>(p);
     }
+    __device__ __forceinline__ void load_each(const T* p) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) t[j] = p[j];
+    }
     __device__ __forceinline__ void store(T* p) const {
         *reinterpret_cast<Raw*>(p) = raw;
     }
@@ -75,7 +79,10 @@ template <typename T, int E> struct Vec {
 };
 
 // E elements a load (the widest that every row of every tensor starts on), NV loads a thread, RW warps a row.
-template <typename T, int E, int NV, int RW, bool RES>
+// ODD (E = 2): an odd number of columns side by side.  Even rows start on a pair, odd rows one element before one; so the
+// pairs of an odd row begin at its second element, and each row has one element left, its first or its last, which its last
+// thread takes.
+template <typename T, int E, int NV, int RW, bool RES, bool ODD>
 __global__ void __launch_bounds__(RW >= 4 ? RW * 32 : 128, 1)
 rms_norm_quant_kernel(const RmsNormParams p)
 {
@@ -89,23 +96,33 @@ rms_norm_quant_kernel(const RmsNormParams p)
     const int64_t row = (int64_t)blockIdx.x * ROWS + sub;
     // loads of this thread; rows behind the last one only keep the barriers company
     const int nv = row < p.M ? (p.K / E - t + T_ROW - 1) / T_ROW : 0;
+    const int start = t * E + (ODD ? (int)(row & 1) : 0);          // column of the first load
+    const bool extra = ODD && t == T_ROW - 1 && row < p.M;         // this thread has the row's single element
+    const int alone = (row & 1) ? 0 : p.K - 1;
 
     V h[NV];
     {
-        const T* x = static_cast<const T*>(p.x) + row * p.ldx + t * E;
+        const T* x = static_cast<const T*>(p.x) + row * p.ldx + start;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             h[v].zero();
             if (v < nv) h[v].load(x + v * T_ROW * E);
         }
     }
+    float h1 = 0.0f, y1 = 0.0f;                                    // of the single element
+    if (extra) h1 = Elem<T>::up(static_cast<const T*>(p.x)[row * p.ldx + alone]);
     if constexpr (RES) {
-        const T* res = static_cast<const T*>(p.residual) + row * p.ldr + t * E;
-        T* h_out = static_cast<T*>(p.residual_out) + row * p.ldo + t * E;
+        const T* res = static_cast<const T*>(p.residual) + row * p.ldr + start;
+        T* h_out = static_cast<T*>(p.residual_out) + row * p.ldo + start;
         V r[NV];
 #pragma unroll
         for (int v = 0; v < NV; ++v)
             if (v < nv) r[v].load(res + v * T_ROW * E);
+        if (extra) {
+            const T sum1 = Elem<T>::down(h1 + Elem<T>::up(static_cast<const T*>(p.residual)[row * p.ldr + alone]));
+            static_cast<T*>(p.residual_out)[row * p.ldo + alone] = sum1;
+            h1 = Elem<T>::up(sum1);
+        }
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             if (v >= nv) continue;
@@ -114,7 +131,7 @@ rms_norm_quant_kernel(const RmsNormParams p)
             h[v].store(h_out + v * T_ROW * E);
         }
     }
-    float2 sum2 = make_float2(0.0f, 0.0f);
+    float2 sum2 = make_float2(ODD ? h1 * h1 : 0.0f, 0.0f);
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
@@ -134,13 +151,18 @@ rms_norm_quant_kernel(const RmsNormParams p)
     const float2 u2 = make_float2(u, u);
 
     float amax = 0.0f;
+    if (extra) {
+        y1 = h1 * u * Elem<T>::up(static_cast<const T*>(p.weight)[alone]);
+        amax = max_abs_nan(amax, y1);
+    }
     float2 y[NV][P];
-    const T* w = static_cast<const T*>(p.weight) + t * E;
+    const T* w = static_cast<const T*>(p.weight) + start;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         if (v >= nv) continue;
         V wv;
-        wv.load(w + v * T_ROW * E);
+        if constexpr (ODD) wv.load_each(w + v * T_ROW * E);
+        else wv.load(w + v * T_ROW * E);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             y[v][i] = __fmul2_rn(__fmul2_rn(h[v].pair(i), u2), wv.pair(i));
@@ -167,8 +189,8 @@ rms_norm_quant_kernel(const RmsNormParams p)
     const float inv = finite ? __frcp_rn(s) : 0.0f;
     const float2 inv2 = make_float2(inv, inv), ns2 = make_float2(-s, -s), magic2 = make_float2(kRoundMagic, kRoundMagic);
     const float2 s2 = make_float2(s, s), nmagic2 = make_float2(-kRoundMagic, -kRoundMagic);
-    int8_t* q_out = p.q == nullptr ? nullptr : p.q + row * (int64_t)p.K + t * E;
-    T* fq = p.fq == nullptr ? nullptr : static_cast<T*>(p.fq) + row * (int64_t)p.K + t * E;
+    int8_t* q_out = p.q == nullptr ? nullptr : p.q + row * (int64_t)p.K + start;
+    T* fq = p.fq == nullptr ? nullptr : static_cast<T*>(p.fq) + row * (int64_t)p.K + start;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         if (v >= nv) continue;
@@ -200,40 +222,48 @@ rms_norm_quant_kernel(const RmsNormParams p)
         }
         if (fq != nullptr) o.store(fq + c);
     }
+    if (extra) {
+        const float y0 = y1 * inv, m = fmaf(fmaf(y0, -s, y1), inv, y0) + kRoundMagic;
+        if (p.q != nullptr) p.q[row * (int64_t)p.K + alone] = (int8_t)(finite ? __float_as_uint(m) & 0xFFu : 0u);
+        if (p.fq != nullptr) static_cast<T*>(p.fq)[row * (int64_t)p.K + alone] = Elem<T>::down((m - kRoundMagic) * s);
+    }
 }
 
-template <typename T, int E, int NV, int RW>
+template <typename T, int E, int NV, int RW, bool ODD = false>
 int launch(const RmsNormParams& p, cudaStream_t st) {
     constexpr int ROWS = RW >= 4 ? 1 : 4 / RW;
     const int64_t blocks = (p.M + ROWS - 1) / ROWS;
     if (blocks > 2147483647LL) return fail(SAMQ_ERR_TOO_LARGE, "RMS norm of %lld rows is too large", (long long)p.M);
     const int threads = RW >= 4 ? RW * 32 : 128;
-    if (p.residual != nullptr) rms_norm_quant_kernel<T, E, NV, RW, true><<<(unsigned)blocks, threads, 0, st>>>(p);
-    else rms_norm_quant_kernel<T, E, NV, RW, false><<<(unsigned)blocks, threads, 0, st>>>(p);
+    if (p.residual != nullptr) rms_norm_quant_kernel<T, E, NV, RW, true, ODD><<<(unsigned)blocks, threads, 0, st>>>(p);
+    else rms_norm_quant_kernel<T, E, NV, RW, false, ODD><<<(unsigned)blocks, threads, 0, st>>>(p);
     SAMQ_CUDA_TRY(cudaGetLastError());
     return SAMQ_OK;
 }
 
 // The fewest warps whose threads hold the row in NV loads each, 1 to 32.
-template <typename T, int E, int NV>
+template <typename T, int E, int NV, bool ODD = false>
 int launch_warps(int64_t loads, const RmsNormParams& p, cudaStream_t st) {
-    if (loads <= 32 * NV) return launch<T, E, NV, 1>(p, st);
-    if (loads <= 64 * NV) return launch<T, E, NV, 2>(p, st);
-    if (loads <= 128 * NV) return launch<T, E, NV, 4>(p, st);
-    if (loads <= 256 * NV) return launch<T, E, NV, 8>(p, st);
-    if (loads <= 512 * NV) return launch<T, E, NV, 16>(p, st);
-    return launch<T, E, NV, 32>(p, st);
+    if (loads <= 32 * NV) return launch<T, E, NV, 1, ODD>(p, st);
+    if (loads <= 64 * NV) return launch<T, E, NV, 2, ODD>(p, st);
+    if (loads <= 128 * NV) return launch<T, E, NV, 4, ODD>(p, st);
+    if (loads <= 256 * NV) return launch<T, E, NV, 8, ODD>(p, st);
+    if (loads <= 512 * NV) return launch<T, E, NV, 16, ODD>(p, st);
+    return launch<T, E, NV, 32, ODD>(p, st);
 }
 
-// `e` elements: the widest access for all rows, see the caller
+// `e` elements: the widest access for all rows; odd: all rows as ODD needs them (see the caller)
 template <typename T>
-int launch_rms_norm(const RmsNormParams& p, int e, cudaStream_t st) {
+int launch_rms_norm(const RmsNormParams& p, int e, bool odd, cudaStream_t st) {
     constexpr int E = Elem<T>::kPerVec;
     // 5 vectors: 1280 columns of a 16-bit type are one warp's, with no lane idle
     if (e == E && p.K <= 1024 * 5 * E) return launch_warps<T, E, 5>(p.K / E, p, st);
     // narrower accesses: more warps a row and fewer elements each
     if (E == 8 && e == 4) return launch_warps<T, 4, 8>(p.K / 4, p, st);
     if (e >= 2 && p.K <= 1024 * 8 * 2) return launch_warps<T, 2, 8>(p.K / 2, p, st);
+    // odd widths: pairs once single elements take more than a warp a row.  us, elements / pairs, fp16: 65536 x 255 38.9 / 45.0,
+    // 32768 x 301 34.8 / 26.6, 32768 x 1279 131 / 82, 8192 x 8191 250 / 182
+    if constexpr (sizeof(T) == 2) { if (odd && p.K > 256 && p.K < 1024 * 8 * 2) return launch_warps<T, 2, 8, true>(p.K / 2, p, st); }
     if (p.K <= 1024 * 8) return launch_warps<T, 1, 8>(p.K, p, st);
     return launch<T, 1, 32, 32>(p, st);
 }
@@ -265,11 +295,14 @@ int rms_norm_quant_dispatch(const void* x, const void* residual, const void* wei
     // two that divides them all is the widest access, up to 16 bytes.
     const uintptr_t starts = all | reinterpret_cast<uintptr_t>(q) * esz | (uintptr_t)((K | ldx | p.ldr | p.ldo) * (int64_t)esz) | 16;
     const int e = (int)((starts & (~starts + 1)) / esz);
+    const uintptr_t bases = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) | reinterpret_cast<uintptr_t>(residual_out) |
+                            reinterpret_cast<uintptr_t>(fq) | reinterpret_cast<uintptr_t>(q) * 2;
+    const bool odd = (bases & 3) == 0 && (K & ldx & (residual ? ldr & ldo : 1) & 1) != 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (dtype) {
-    case SAMQ_F16:  return launch_rms_norm<__half>(p, e, st);
-    case SAMQ_BF16: return launch_rms_norm<__nv_bfloat16>(p, e, st);
-    default:        return launch_rms_norm<float>(p, e, st);
+    case SAMQ_F16:  return launch_rms_norm<__half>(p, e, odd, st);
+    case SAMQ_BF16: return launch_rms_norm<__nv_bfloat16>(p, e, odd, st);
+    default:        return launch_rms_norm<float>(p, e, odd, st);
     }
 }
 

@@ -38,7 +38,7 @@ def _check(out, h, w, n_bits=8, eps=EPS):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("M,K", [(1, 1), (1, 1280), (3, 7), (5, 1023), (33, 1280), (17, 2048), (9, 4096), (3, 5120), (70, 96), (2, 8200), (65, 1281), (67, 1282), (130, 85), (40, 20), (19, 5119), (9, 8191), (2, 20481), (3, 31), (11, 12), (10, 3),
+@pytest.mark.parametrize("M,K", [(1, 1), (1, 1280), (3, 7), (5, 1023), (33, 1280), (17, 2048), (9, 4096), (3, 5120), (70, 96), (2, 8200), (65, 1281), (67, 1282), (130, 85), (40, 20), (19, 5119), (9, 8191), (2, 20481), (3, 31), (11, 12), (10, 3), (6, 257), (7, 515), (5, 4099), (3, 16383),
                                  (2, 20488), (1, 32767), (2, 32768)])
 def test_matches_the_definition(cuda_device, dtype, M, K):
     x, r, w = _inputs(M, K, dtype, cuda_device)
