@@ -101,6 +101,25 @@ def test_rows_of_zeros_and_rows_that_are_not_finite(cuda_device):
     assert out["scale"][2:4].isnan().all() and int(out["q"][2:4].abs().max()) == 0 and out["fq"][2:4].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("K", [257, 1279])
+def test_odd_widths_first_and_last_elements(cuda_device, dtype, K):
+    """Of an odd number of columns one a row stands apart from the pairs: the first or the last, by turns."""
+    x, r, w = _inputs(8, K, dtype, cuda_device)
+    x[0, K - 1], x[1, 0], x[2, 0], x[3, K - 1] = 40.0, -40.0, 40.0, -40.0         # the row's scale comes from there
+    x[4, K - 1] = float("nan")
+    x[5, 0] = float("inf")
+    out = ops.rms_norm_quantize(x, w, EPS, residual=r, fake_quant=True)
+    h = (x.float() + r.float()).to(dtype)
+    assert torch.equal(out["residual"][:4], h[:4]) and torch.equal(out["residual"][6:], h[6:])
+    fine = [0, 1, 2, 3, 6, 7]
+    _check({k: v[fine] for k, v in out.items()}, h[fine], w)
+    assert out["scale"][4:6].isnan().all() and int(out["q"][4:6].abs().max()) == 0 and out["fq"][4:6].isnan().all()
+    stream = r.clone()
+    again = ops.rms_norm_quantize(x, w, EPS, residual=stream, residual_out=stream, fake_quant=True)
+    assert torch.equal(again["q"], out["q"]) and torch.equal(stream[fine], h[fine])
+
+
 def test_large_rows_of_fp32_do_not_overflow_early(cuda_device):
     """Squares of 1e18 sum to 1e39 only behind fp32's range: the row is reported as not finite, others stand."""
     x, _, w = _inputs(2, 512, torch.float32, cuda_device)
