@@ -76,6 +76,8 @@ template <typename T> struct Chunk {
             else return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
         }
     }
+    // values that bfloat16 holds exactly
+    __device__ __forceinline__ void set_pair(int i, float2 v) { w[i] = (__float_as_uint(v.x) >> 16) | (__float_as_uint(v.y) & 0xFFFF0000u); }
     // the largest |x| as fp32 bits; a NaN or an infinity counts as larger than every number
     __device__ __forceinline__ uint32_t amax_bits() const {
         uint32_t m = 0;
@@ -98,6 +100,7 @@ template <> struct Chunk<float> {
     }
     __device__ __forceinline__ void set(int i, float v) { f[i] = v; }
     __device__ __forceinline__ float2 pair(int i) const { return make_float2(f[2 * i], f[2 * i + 1]); }
+    __device__ __forceinline__ void set_pair(int i, float2 v) { f[2 * i] = v.x; f[2 * i + 1] = v.y; }
     __device__ __forceinline__ uint32_t amax_bits() const {
         uint32_t m = 0;
 #pragma unroll
@@ -160,8 +163,9 @@ __device__ __forceinline__ Scale block_scale(uint32_t amax_bits, float global_sc
         // amax / (6 g) to e4m3, at most 448, and at least its smallest value 2^-9 (the block's own values are
         // then still resolved below the point where the scale alone would round to zero).  6 has few
         // significant bits, so the correctly rounded quotient never reaches a tie that amax itself missed.
-        // g is a power of two: amax / g is exact, and a sixth of it is one correctly rounded quotient by a constant
-        const float a = __uint_as_float(amax_bits) * inv_global_scale;
+        // g is a power of two: amax / g is exact, and a sixth of it is one correctly rounded quotient by a constant.  Beyond
+        // 6 * 448 the scale saturates; a is held there, since the correction of an infinite a would be a NaN.
+        const float a = fminf(__uint_as_float(amax_bits) * inv_global_scale, 2688.0f);
         const float sixth = 1.0f / 6.0f;
         const float q0 = a * sixth;
         const float q = fmaf(fmaf(-q0, 6.0f, a), sixth, q0);
@@ -179,7 +183,8 @@ __device__ __forceinline__ Scale block_scale(uint32_t amax_bits, float global_sc
 // x / scale for a finite block, two values at a time.  mxfp4: a product with the exact reciprocal.  nvfp4: Markstein's
 // correction of an approximate quotient, y = y0 + (x - y0 s) / s: exact where x / s is a number of few bits, so on every
 // border between codes, and a correct rounding elsewhere up to 2^-45; a scale has four significant bits and a border
-// three, so a value beside a border stays beside it.  The correction loses the sign of -0, which is put back.
+// three, so a value beside a border stays beside it.  The correction loses the sign of -0, which is put back; and it needs
+// a quotient within fp32 (see hold_far).
 template <int FMT>
 struct ToCode {
     float2 s2, inv2;
@@ -210,6 +215,23 @@ __device__ __forceinline__ uint2 encode_chunk(const Chunk<T>& c, const Scale& s,
     }
     const uint2 q = make_uint2(pack_e2m1x8(v), pack_e2m1x8(v + 8));
     return finite ? q : make_uint2(0u, 0u);
+}
+
+// An nvfp4 block far beyond the largest scale: x / s may leave fp32.  Magnitudes from 6 s on have the same code, so they are
+// held at 8 s.  Only where the largest scale 448 g is below 1, since |x| < 2^128, and not in fp16, whose values end at 2^16:
+// the branch is the same in the whole grid (a bound on every element would cost 32768 x 5120 bf16 a seventh of its time).
+template <int FMT, typename T>
+__device__ __forceinline__ void hold_far(Chunk<T>& c, const Scale& s, float global_scale) {
+    if constexpr (FMT == SAMQ_FP4_NV && !std::is_same<T, __half>::value) {
+        if (global_scale < 0x1p-8f) {
+            const float most = 8.0f * s.value;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float2 x = c.pair(i);
+                c.set_pair(i, make_float2(fminf(fmaxf(x.x, -most), most), fminf(fmaxf(x.y, -most), most)));
+            }
+        }
+    }
 }
 
 }  // namespace fp4

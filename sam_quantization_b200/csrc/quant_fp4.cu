@@ -101,6 +101,7 @@ quant_fp4_kernel(const QuantFp4Params p)
     uint32_t amax = x.amax_bits();
     if constexpr (FMT == SAMQ_FP4_MX) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     const Scale s = block_scale<FMT>(amax, p.global_scale, p.inv_global_scale);
+    hold_far<FMT>(x, s, p.global_scale);
     const uint2 q = encode_chunk<FMT>(x, s, amax < 0x7F800000u);
 
     // the word of four scales is put together by the group's first lane; blocks behind K and rows behind M are zero

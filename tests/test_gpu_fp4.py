@@ -339,3 +339,21 @@ def test_captured_replayed_and_on_two_streams(cuda_device, M):
             graph.replay()
     assert _same(graphs[0][1], want) and _same(graphs[1][1], want2)
     ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("g", [2.0 ** -64, 2.0 ** -40, 2.0 ** -14, 0.5, 2.0 ** 20, 2.0 ** 64])
+def test_extreme_values_under_a_global_scale(cuda_device, dtype, g):
+    """Blocks far beyond the largest scale saturate (and stay finite), blocks far below the smallest round to zero."""
+    top = float(torch.finfo(dtype).max)
+    x = torch.zeros(12, 70)
+    for i, size in enumerate((top, 3e38, 3e34, 1e30, 1e20, 1e-20, 1e-38, 1e-44)):
+        x[i] = min(size, top) * torch.linspace(-1, 1, 70)
+    x[8] = min(3e38, top) * torch.logspace(0, -70, 70) * (1 - 2 * (torch.arange(70) % 2))      # every magnitude beside the largest
+    x[9] = g * torch.linspace(-3000, 3000, 70)
+    x[10, 3], x[10, 60] = float("nan"), 1e30
+    x[11, 40], x[11, 3] = -float("inf"), -1e30
+    x = x.clamp(-top, top) if dtype == torch.float16 else x
+    x[10, 3], x[11, 40] = float("nan"), -float("inf")
+    x = x.to(dtype)
+    _check_quantized(x, ops.quantize_fp4(x.to(cuda_device), "nvfp4", global_scale=g, fake_quant=True), "nvfp4", g)
