@@ -287,7 +287,8 @@ int samq_sym_dequant_i32(const int32_t* q, const void* scale_row, const void* sc
  * weight    : [K] of `dtype`
  * q_out     : [M, K] int8 codes or NULL;  scale_out : [M] fp32 or NULL (what samq_gemm_i8 takes as ROW scales)
  * fq_out    : [M, K] of `dtype`, the values q * s, or NULL
- * A row with a NaN or an infinity gets a NaN scale and zero codes.  K <= 32768. */
+ * A row with a NaN or an infinity gets a NaN scale and zero codes; finite rows may have any magnitude (their squares need
+ * not fit fp32), and a row of zeros has zero codes with eps = 0 too.  K <= 32768. */
 int samq_rms_norm_quant_i8(const void* x, const void* residual, const void* weight, int dtype, int64_t M, int64_t K,
                            int64_t ldx, int64_t ldr, float eps, int n_bits, void* residual_out, int64_t ldo,
                            int8_t* q_out, float* scale_out, void* fq_out, void* stream);

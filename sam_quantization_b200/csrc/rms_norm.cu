@@ -10,6 +10,7 @@
 // in its own type (60 registers instead of 110 of fp32: 66.3 -> 61.5 us).  Measured, 32768 x 1280 fp16 with residual and
 // values: 61.5 us, 6.1 TB/s; without a residual 28.3; 1278 columns (4-byte accesses) 76, 1279 82.
 #include "common.cuh"
+#include <float.h>
 #include <type_traits>
 
 namespace samq {
@@ -77,6 +78,65 @@ template <typename T, int E> struct Vec {
         else { t[2 * i] = v.x; t[2 * i + 1] = v.y; }
     }
 };
+
+// a barrier of the RW warps of a block's `sub`-th row, and of what they have stored (numbers known when compiled: a block whose
+// barriers go by a register reserves all sixteen, and only four such fit an SM)
+template <int RW>
+__device__ __forceinline__ void row_sync(int sub) {
+    if constexpr (RW == 1) __syncwarp();
+    else if (RW > 2 || sub == 0) asm volatile("bar.sync 1, %0;" ::"n"(RW * 32) : "memory");
+    else asm volatile("bar.sync 2, %0;" ::"n"(RW * 32) : "memory");
+}
+// the sum (or the largest, of values that are not negative) over the threads of a row; `red`: RW floats of the row
+template <int RW, bool MAX>
+__device__ __forceinline__ float row_reduce(float v, int sub, int t, float* red) {
+    v = MAX ? __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v))) : warp_sum(v);
+    if constexpr (RW > 1) {
+        row_sync<RW>(sub);                                         // `red` has been read
+        if ((t & 31) == 0) red[t >> 5] = v;
+        row_sync<RW>(sub);
+        v = red[0];
+#pragma unroll 1
+        for (int w = 1; w < RW; ++w) v = MAX ? max_abs_nan(v, red[w]) : v + red[w];
+    }
+    return v;
+}
+
+// A row whose squares leave fp32, or lose bits below it where eps does not cover them, and a row of zeros without an eps (which
+// stays one).  y does not change when h is scaled by a power of two and eps by its square, so the row is brought to where
+// its largest element, or the root of eps, is near 1.  It is read again, element by element: kept out of the kernel's
+// registers (in line, the branch took ordinary rows of bfloat16 from 64 to 80).
+template <typename T, int RW>
+__device__ __noinline__ void scaled_row(const RmsNormParams p, int64_t row, int sub, int t, float* red) {
+    constexpr int T_ROW = RW * 32;
+    const T* h = p.residual != nullptr ? static_cast<const T*>(p.residual_out) + row * p.ldo : static_cast<const T*>(p.x) + row * p.ldx;
+    const T* w = static_cast<const T*>(p.weight);
+    row_sync<RW>(sub);                                             // the row's sums with the residual have been stored
+    float m = 0.0f;
+#pragma unroll 1
+    for (int k = t; k < p.K; k += T_ROW) m = fmaxf(m, fabsf(Elem<T>::up(h[k])));
+    m = row_reduce<RW, true>(m, sub, t, red);
+    float c = 1.0f;                                                // 2^-126 to 2^126; an infinity stays one, and its row ends as NaN
+    if (m > 0.0f && m <= FLT_MAX) c = __uint_as_float((254u - min(max(__float_as_uint(fmaxf(m, sqrtf(p.eps))) >> 23, 1u), 253u)) << 23);
+    float sum = 0.0f;
+#pragma unroll 1
+    for (int k = t; k < p.K; k += T_ROW) { const float f = Elem<T>::up(h[k]) * c; sum = fmaf(f, f, sum); }
+    const float mean = fmaf(row_reduce<RW, false>(sum, sub, t, red), p.inv_k, p.eps * c * c);
+    const float u = mean == 0.0f ? 0.0f : rsqrtf(mean);
+    float amax = 0.0f;
+#pragma unroll 1
+    for (int k = t; k < p.K; k += T_ROW) amax = max_abs_nan(amax, Elem<T>::up(h[k]) * c * u * Elem<T>::up(w[k]));
+    amax = row_reduce<RW, true>(fabsf(amax), sub, t, red);
+    const bool finite = __float_as_uint(amax) < 0x7F800000u;
+    const float s = finite ? __fdiv_rn(fmaxf(amax, 1e-5f), p.qmax) : __uint_as_float(0x7FC00000u);
+    if (t == 0 && p.scale != nullptr) p.scale[row] = s;
+#pragma unroll 1
+    for (int k = t; k < p.K; k += T_ROW) {
+        const float q = rintf(__fdiv_rn(Elem<T>::up(h[k]) * c * u * Elem<T>::up(w[k]), s));
+        if (p.q != nullptr) p.q[row * (int64_t)p.K + k] = (int8_t)(finite ? (int)q : 0);
+        if (p.fq != nullptr) static_cast<T*>(p.fq)[row * (int64_t)p.K + k] = Elem<T>::down(q * s);
+    }
+}
 
 // E elements a load (the widest that every row of every tensor starts on), NV loads a thread, RW warps a row.
 // ODD (E = 2): an odd number of columns side by side.  Even rows start on a pair, odd rows one element before one; so the
@@ -180,6 +240,12 @@ rms_norm_quant_kernel(const RmsNormParams p)
         for (int k = 1; k < RW; ++k) amax = max_abs_nan(amax, red_max[sub * RW + k]);
     }
     if (row >= p.M) return;
+    // The squares have left fp32 (u = 0), or are so small that some may have been lost and eps does not hide it.  All threads of a
+    // row take the same way; the rows of a block share no barrier from here on.
+    if (u == 0.0f || u > 0x1p35f) {
+        scaled_row<T, RW>(p, row, sub, t, red_max + sub * RW);
+        return;
+    }
     // a row with a NaN or an infinity has a NaN scale and zero codes
     const bool finite = (__float_as_uint(amax) & 0x7FFFFFFFu) < 0x7F800000u;
     const float s = finite ? __fdiv_rn(fmaxf(amax, 1e-5f), p.qmax) : __uint_as_float(0x7FC00000u);

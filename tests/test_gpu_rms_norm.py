@@ -177,3 +177,36 @@ def test_feeds_the_int8_product(cuda_device):
     # exact integer sums, then two fp32 products and a conversion: 4 u relative
     assert ((y.double() - want).abs() <= 4 * U * want.abs() + 1e-30).all()
     ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("K", [1, 96, 160, 1279, 1280, 2050, 8191, 20488])
+@pytest.mark.parametrize("eps", [1e-6, 0.0, 1e-30])
+def test_rows_whose_squares_leave_the_range(cuda_device, dtype, K, eps):
+    """Finite rows whose squares overflow fp32, or underflow it under a small eps, beside ordinary ones."""
+    x, r, w = _inputs(9, K, torch.float32, cuda_device)
+    x /= x.abs().amax(1, keepdim=True)
+    # tiny rows down to 1e-30: below, the elements of a bf16 or fp32 row lose bits of their own
+    for i, size in enumerate((3e19, 1.0, 1e30, 3e38, 1e-25, 1e-30, 5.0, 1e19, 1e-19)):
+        x[i] *= size
+    x, w = x.to(dtype), w.to(dtype)
+    out = ops.rms_norm_quantize(x, w, eps, fake_quant=True)
+    _check(out, x, w, eps=eps)
+    out = ops.rms_norm_quantize(torch.zeros_like(x), w, eps, residual=x, fake_quant=True)      # the residual stream is not scaled
+    assert torch.equal(out["residual"], x)
+    _check(out, x, w, eps=eps)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("K", [96, 257, 1280])
+def test_rows_of_zeros_without_an_eps(cuda_device, dtype, K):
+    x, r, w = _inputs(5, K, dtype, cuda_device)
+    x[1], x[4] = 0, -0.0
+    x[2, K - 1] = float("inf")
+    x[3, 0] = float("nan")
+    out = ops.rms_norm_quantize(x, w, 0.0, fake_quant=True)
+    _check({k: v[:1] for k, v in out.items()}, x[:1], w, eps=0.0)
+    for i in (1, 4):
+        assert abs(float(out["scale"][i]) - 1e-5 / 127) < 1e-5 / 127 * 4 * U
+        assert int(out["q"][i].abs().max()) == 0 and int(out["fq"][i].count_nonzero()) == 0
+    assert out["scale"][2:4].isnan().all() and int(out["q"][2:4].abs().max()) == 0 and out["fq"][2:4].isnan().all()
