@@ -174,7 +174,7 @@ struct EpiWarp {
             if constexpr (RES) {
                 if (p.tma_res) {
                     if (ps > 0) load_residual(row0, col);
-                    const bool ok = mbar_wait(res_bar, res_phase, abort_flag);
+                    const bool ok = mbar_wait_warp(res_bar, res_phase, abort_flag);
                     res_phase ^= 1u;
                     if (!ok) return false;
                 } else if (ps > 0) {

@@ -268,7 +268,7 @@ gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     if (warp == 0) {
         bool ok = true;
         for (int i = stages; i < kb_count; ++i) {
-            ok = mbar_wait(smem_u32(&ctl->empty[i % stages]), ((i / stages) & 1) ^ 1u, abort_flag);
+            ok = mbar_wait_warp(smem_u32(&ctl->empty[i % stages]), ((i / stages) & 1) ^ 1u, abort_flag);
             if (!ok) break;
             if (elect_one()) load_stage(i);
             __syncwarp();
@@ -282,7 +282,7 @@ gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         const uint32_t idesc_n = (uint32_t)p.T;
         for (int i = 0; i < kb_count; ++i) {
             const int s = i % stages;
-            ok = mbar_wait(smem_u32(&ctl->full[s]), (i / stages) & 1, abort_flag);
+            ok = mbar_wait_warp(smem_u32(&ctl->full[s]), (i / stages) & 1, abort_flag);
             if (!ok) break;
             tcgen05_fence_after();
             const uint32_t sw = smem_u32(tiles + (size_t)s * st_bytes);
@@ -321,7 +321,7 @@ gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                 const int blocks = min(group, kb_count - i);
                 Chunk<OutT> x[BATCH];
                 load_batch(p, of, m0, kb_first + i, blocks, 0, tid, x);
-                for (int k = i; k < i + blocks && ok; ++k) ok = mbar_wait(smem_u32(&ctl->empty[k % stages]), ((k / stages) & 1) ^ 1u, abort_flag);
+                for (int k = i; k < i + blocks && ok; ++k) ok = mbar_wait_warp(smem_u32(&ctl->empty[k % stages]), ((k / stages) & 1) ^ 1u, abort_flag);
                 if (!ok) break;
                 quantize_batch<OutT, FMT>(p, of, kb_first + i, blocks, 0, tid, i % stages, x, tiles, st_bytes, sf);
                 fence_async_smem();
@@ -341,7 +341,7 @@ gemm_fp4_small_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         OutT res[2][16] = {};                                       // of this turn and the next
         load_residual<OutT, RES>(p, n, first_row + turn, mine - turn, res[0]);
         load_residual<OutT, RES>(p, n, first_row + turn + 32, mine - turn - 32, res[1]);
-        if (mbar_wait(smem_u32(&ctl->acc_full), 0, abort_flag)) {
+        if (mbar_wait_warp(smem_u32(&ctl->acc_full), 0, abort_flag)) {
             tcgen05_fence_after();
             if (split == 1) {
                 for (int c = turn; c < rows; c += 64) {

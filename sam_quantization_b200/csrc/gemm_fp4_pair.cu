@@ -171,8 +171,8 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             const int w_rows = walk.width(p.epi.N) / 2;                    // of W in this CTA (a whole box is loaded)
             const bool load_a = RESIDENT && walk.new_rows();
             for (int kb = 0; kb < k_blocks; ++kb) {
-                if (load_a) ok = mbar_wait(smem_u32(&ctl->a_empty[kb]), a_phase, abort_flag);
-                ok = ok && mbar_wait(smem_u32(&ctl->empty[stage]), phase ^ 1u, abort_flag);
+                if (load_a) ok = mbar_wait_warp(smem_u32(&ctl->a_empty[kb]), a_phase, abort_flag);
+                ok = ok && mbar_wait_warp(smem_u32(&ctl->empty[stage]), phase ^ 1u, abort_flag);
                 if (!ok) break;
                 if (elect_one()) {
                     const uint32_t bar = smem_u32(&ctl->full[stage]), leader_bar = map_to_cta(bar, 0);
@@ -199,7 +199,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         // every stage has been handed back: no completion from the leader's MMAs can still be on its way to this CTA's
         // barriers when the CTA retires
         for (int s = 0; s < STAGES && ok; ++s) {
-            ok = mbar_wait(smem_u32(&ctl->empty[stage]), phase ^ 1u, abort_flag);
+            ok = mbar_wait_warp(smem_u32(&ctl->empty[stage]), phase ^ 1u, abort_flag);
             if (++stage == STAGES) { stage = 0; phase ^= 1u; }
         }
         if (!ok) {
@@ -217,17 +217,17 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 const bool wait_a = RESIDENT && walk.new_rows(), free_a = RESIDENT && walk.rows_done();
                 if (wait_a) a_phase ^= 1u;
                 // the buffer itself (two tiles ago) and the columns that the previous tile's buffer shares with it
-                if (!mbar_wait(smem_u32(&ctl->acc_empty[acc]), acc_phase ^ 1u, abort_flag)) break;
-                if (S::SHARED_COLS > 0 && !mbar_wait(smem_u32(&ctl->shared_empty), shared_phase, abort_flag)) break;
+                if (!mbar_wait_warp(smem_u32(&ctl->acc_empty[acc]), acc_phase ^ 1u, abort_flag)) break;
+                if (S::SHARED_COLS > 0 && !mbar_wait_warp(smem_u32(&ctl->shared_empty), shared_phase, abort_flag)) break;
                 shared_phase ^= 1u;
                 const uint32_t tmem_d = tmem + (uint32_t)(acc * S::ACC1_COL);
                 // an odd tile of 192 rows begins in the middle of a scale tile: skip its first 64 rows, two columns
                 const uint32_t idesc_n = (uint32_t)(walk.width(p.epi.N) >> 3) << 17;
                 const uint32_t sf_shift = BN % TILE_ROWS != 0 ? (uint32_t)(walk.n & 1) * 2u : 0u;
                 for (int kb = 0; kb < k_blocks; ++kb) {
-                    ok = mbar_wait(smem_u32(&ctl->full[stage]), phase, abort_flag) &&
-                         (!wait_a || mbar_wait(smem_u32(&ctl->a_full[kb]), a_phase, abort_flag)) &&
-                         mbar_wait(smem_u32(&ctl->sf_ready[unit]), unit_phase, abort_flag);
+                    ok = mbar_wait_warp(smem_u32(&ctl->full[stage]), phase, abort_flag) &&
+                         (!wait_a || mbar_wait_warp(smem_u32(&ctl->a_full[kb]), a_phase, abort_flag)) &&
+                         mbar_wait_warp(smem_u32(&ctl->sf_ready[unit]), unit_phase, abort_flag);
                     if (!ok) break;
                     tcgen05_fence_after();
                     const uint64_t adesc = make_smem_desc(smem_u32(tiles + (size_t)(RESIDENT ? kb : stage) * A_BYTES));
@@ -267,10 +267,10 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 const bool wait_a = RESIDENT && walk.new_rows();
                 if (wait_a) a_phase ^= 1u;
                 for (int kb = 0; kb < k_blocks; ++kb) {
-                    ok = mbar_wait(smem_u32(&ctl->full[stage]), phase, abort_flag) &&
-                         (!wait_a || mbar_wait(smem_u32(&ctl->a_full[kb]), a_phase, abort_flag));
+                    ok = mbar_wait_warp(smem_u32(&ctl->full[stage]), phase, abort_flag) &&
+                         (!wait_a || mbar_wait_warp(smem_u32(&ctl->a_full[kb]), a_phase, abort_flag));
                     if (ok && filled == S::UNITS) {
-                        ok = mbar_wait(smem_u32(&ctl->empty[old_stage]), old_phase, abort_flag);
+                        ok = mbar_wait_warp(smem_u32(&ctl->empty[old_stage]), old_phase, abort_flag);
                         if (++old_stage == STAGES) { old_stage = 0; old_phase ^= 1u; }
                     } else {
                         ++filled;
@@ -308,7 +308,7 @@ gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             const int row0 = walk.m * (2 * BM) + (int)rank * BM + quad * 32;
             const int col0 = walk.n * BN + cg * EPI_COLS;
             epi.before(row0, col0);
-            if (!mbar_wait(smem_u32(&ctl->acc_full[acc]), acc_phase, abort_flag)) break;
+            if (!mbar_wait_warp(smem_u32(&ctl->acc_full[acc]), acc_phase, abort_flag)) break;
             tcgen05_fence_after();
             uint32_t r[EPI_COLS];
             tmem_ld64(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * S::ACC1_COL + cg * EPI_COLS), r);

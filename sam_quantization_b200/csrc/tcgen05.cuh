@@ -44,6 +44,19 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
     return true;
 }
+// The same by a whole converged warp, with one answer for all lanes: a lane that polled, read the flag and the clock for itself
+// and gave up alone would be missing from the warp-wide instructions (elect, tcgen05.ld, barriers) that follow.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    const long long t0 = clock64();
+    for (uint32_t spins = 1; !__all_sync(0xffffffffu, mbar_try_wait(bar, parity)); ++spins) {
+        if ((spins & 255u) == 0 && __any_sync(0xffffffffu, *abort_flag != 0 || clock64() - t0 > WAIT_LIMIT_CYCLES)) {
+            *abort_flag = 1;
+            return false;
+        }
+    }
+    return true;
+}
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
                  " [%0], [%1, {%3, %4}], [%2];"

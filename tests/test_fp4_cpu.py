@@ -1,6 +1,8 @@
 """The 4-bit format and the RMS norm without a GPU: the oracle against known values, host helpers, and every refusal
 (argument checks answer before any device work)."""
 import math
+import os
+import re
 
 import numpy as np
 import pytest
@@ -113,3 +115,13 @@ def test_no_rows_are_no_work():
     lib = _lib.load()
     for fn, args in _calls(lib).values():
         assert fn(*dict(args, M=0).values()) == 0
+
+
+@pytest.mark.parametrize("name", ["gemm_fp4.cu", "gemm_fp4_pair.cu", "fp4_gemm.cuh"])
+def test_loops_of_whole_warps_wait_as_a_warp(name):
+    """A wait that ran out must send all lanes of a warp the same way: the loops of these kernels run warp-wide instructions
+    behind their waits, so none polls a barrier lane by lane (the last join, with no such instruction behind it, is the
+    cluster form)."""
+    with open(os.path.join(os.path.dirname(_lib.__file__), "csrc", name)) as f:
+        code = re.sub(r"//[^\n]*", "", f.read())
+    assert "mbar_wait_warp(" in code and not re.search(r"\bmbar_(try_)?wait\(", code)
