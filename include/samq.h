@@ -323,8 +323,10 @@ int samq_gemm_fp4(const uint8_t* A, int64_t lda, const uint8_t* a_scales, const 
                   int64_t M, int64_t N, int64_t K, int format, float alpha, const void* bias, const void* residual, int64_t ldr,
                   int activation, void* out, int out_dtype, int64_t ldo, int32_t* status, void* stream);
 
-/* A 4-bit linear layer: x [M, K] of `dtype`, row stride ldx, is quantized as samq_quant_fp4 does with global_scale 1 and
- * multiplied as in samq_gemm_fp4.  Up to SAMQ_LINEAR_FP4_ONE_KERNEL_ROWS rows with dtype == out_dtype it can be one kernel,
+/* A 4-bit linear layer: x [M, K] of `dtype`, row stride ldx, is quantized as samq_quant_fp4 does with global_scale 1
+ * (samq_linear_fp4_ex: x_global_scale, which multiplies alpha) and multiplied as in samq_gemm_fp4.  nvfp4 with a global
+ * scale g holds magnitudes up to 2688 g; what is larger saturates, blocks below about 2^-6 g lose resolution and elements
+ * below 2^-11 g become zero: activations outside that range need a scale of their own (mxfp4 reaches every exponent).  Up to SAMQ_LINEAR_FP4_ONE_KERNEL_ROWS rows with dtype == out_dtype it can be one kernel,
  * and `workspace` may be NULL; otherwise the quantized activation lives in `workspace`, 16-byte aligned and of
  * samq_linear_fp4_workspace_bytes() at least, until the call's work on the stream is done.  Few rows with
  * (M + 8) * ceil(K / 256) > SAMQ_LINEAR_FP4_ONE_KERNEL_WORK take a workspace too if they are given one, where two kernels are
@@ -336,6 +338,10 @@ int samq_linear_fp4(const void* x, int dtype, int64_t ldx, const uint8_t* W, int
                     int64_t M, int64_t N, int64_t K, int format, float alpha, const void* bias, const void* residual, int64_t ldr,
                     int activation, void* out, int out_dtype, int64_t ldo, void* workspace, size_t workspace_bytes,
                     int32_t* status, void* stream);
+int samq_linear_fp4_ex(const void* x, int dtype, int64_t ldx, float x_global_scale, const uint8_t* W, int64_t ldw, const uint8_t* w_scales,
+                       int64_t M, int64_t N, int64_t K, int format, float alpha, const void* bias, const void* residual, int64_t ldr,
+                       int activation, void* out, int out_dtype, int64_t ldo, void* workspace, size_t workspace_bytes,
+                       int32_t* status, void* stream);
 
 /* Process-wide choice between the two implementations of samq_gemm_i8 for row / tensor scales
  * (no reference counterpart: the reference has a single cuBLAS-style path):

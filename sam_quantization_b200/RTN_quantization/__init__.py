@@ -9,4 +9,4 @@ from .per_tensor_channel_group import (W8A8Linear, quantize_activation_codes,  #
 from .Smooth import smooth_ln_fcs  # noqa: F401
 from .utils import replace_linear_with_target_and_quantize, smooth_sam  # noqa: F401
 from .calibration import get_act_scales_sam  # noqa: F401
-from .fp4 import FP4Linear  # noqa: F401
+from .fp4 import FP4Linear, set_fp4_act_scales  # noqa: F401

@@ -16,7 +16,10 @@ from .._lib import ACT_GELU, ACT_NONE
 class FP4Linear(nn.Module):
     """``y = x @ W^T + bias`` with both operands in ``weight_quant``: "nvfp4" (16 columns a scale, e4m3) or "mxfp4" (32
     columns, powers of two).  The weight is kept as codes and scales (``qcodes``, ``qscales`` and, for nvfp4, a power of
-    two ``global_scale``) and the activation is quantized in every call."""
+    two ``global_scale``) and the activation is quantized in every call, for nvfp4 under the power of two
+    ``act_global_scale``: magnitudes beyond 2688 times it saturate and blocks below about 2^-6 times it lose resolution, so
+    a layer whose activations are far from 1 is given its own (``calibrate``, ``set_fp4_act_scales``).
+    ``output_global_scale`` is the same for the output, where ``quantize_output`` asks for it."""
 
     # callers that know this module may fuse the following GELU / residual add into the product
     supports_fused_epilogue = True
@@ -28,7 +31,7 @@ class FP4Linear(nn.Module):
         self.in_features, self.out_features = in_features, out_features
         self.weight_quant_name = self.act_quant_name = weight_quant
         self.quantize_output = bool(quantize_output)
-        self.global_scale = 1.0
+        self.global_scale = self.act_global_scale = self.output_global_scale = 1.0
         self.compute_dtype = torch.float16
         self.register_buffer("qcodes", torch.zeros(out_features, (in_features + 31) // 32 * 16, dtype=torch.uint8))
         self.register_buffer("qscales", torch.zeros(ops.fp4_scale_shape(weight_quant, out_features, in_features), dtype=torch.uint8))
@@ -62,10 +65,13 @@ class FP4Linear(nn.Module):
     def get_extra_state(self):
         return {"kind": "FP4Linear", "in_features": self.in_features, "out_features": self.out_features,
                 "weight_quant": self.weight_quant_name, "quantize_output": self.quantize_output,
-                "global_scale": self.global_scale, "compute_dtype": str(self.compute_dtype).split(".")[-1]}
+                "global_scale": self.global_scale, "act_global_scale": self.act_global_scale,
+                "output_global_scale": self.output_global_scale, "compute_dtype": str(self.compute_dtype).split(".")[-1]}
 
     def set_extra_state(self, state):
         self.quantize_output, self.global_scale = bool(state["quantize_output"]), float(state["global_scale"])
+        self.act_global_scale = float(state.get("act_global_scale", 1.0))
+        self.output_global_scale = float(state.get("output_global_scale", 1.0))
         self.compute_dtype = getattr(torch, state["compute_dtype"])
 
     def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
@@ -78,17 +84,33 @@ class FP4Linear(nn.Module):
         super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
 
     # -- the layer -----------------------------------------------------------------------------
+    def calibrate(self, act_absmax, output_absmax=None):
+        """Choose the global scales of the activation and, with ``output_absmax``, of the output from their largest
+        magnitudes in calibration.  mxfp4 has none and stays as it is.  Returns ``act_global_scale``."""
+        if self.weight_quant_name == "nvfp4":
+            self.act_global_scale = ops.fp4_global_scale(float(act_absmax))
+            if output_absmax is not None:
+                self.output_global_scale = ops.fp4_global_scale(float(output_absmax))
+        return self.act_global_scale
+
     def act_quant(self, x):
         """The fake-quantized activation."""
-        return ops.quantize_fp4(x, self.act_quant_name, fake_quant=True)["fq"]
+        return ops.quantize_fp4(x, self.act_quant_name, global_scale=self.act_global_scale, fake_quant=True)["fq"]
+
+    def output_quant(self, y):
+        """The output as ``quantize_output`` asks for it."""
+        if not self.quantize_output:
+            return y
+        return ops.quantize_fp4(y, self.act_quant_name, global_scale=self.output_global_scale, fake_quant=True)["fq"]
 
     @torch.no_grad()
     def forward(self, x, residual=None, activation=None, out_dtype=None):
         """As ``W8A8Linear.forward``: ``activation="gelu"`` and ``residual`` act in the product's epilogue, ``out_dtype``
         selects the stored type; with ``quantize_output`` the result is fake-quantized again."""
         y = ops.linear_fp4(x, self.qweight, bias=self.bias, residual=residual,
-                           activation=ACT_GELU if activation == "gelu" else ACT_NONE, out_dtype=out_dtype)
-        return self.act_quant(y) if self.quantize_output else y
+                           activation=ACT_GELU if activation == "gelu" else ACT_NONE, out_dtype=out_dtype,
+                           x_global_scale=self.act_global_scale)
+        return self.output_quant(y)
 
     @staticmethod
     def from_float(module, n_bits=4, weight_quant="nvfp4", act_quant=None, quantize_output=False, group_size=None):
@@ -114,3 +136,14 @@ class FP4Linear(nn.Module):
     def __repr__(self):
         return (f"FP4Linear({self.in_features}, {self.out_features}, bias={self.bias is not None}, "
                 f"weight_quant={self.weight_quant_name}, quantize_output={self.quantize_output})")
+
+
+def set_fp4_act_scales(model, act_scales) -> int:
+    """Give every ``FP4Linear`` of ``model`` that ``act_scales`` names the activation scale for its largest magnitude.
+    ``act_scales``: {module name: per-channel largest |x|}, what ``get_act_scales_sam`` returns for the float model before
+    it is converted.  Returns how many layers were set."""
+    layers = dict(model.named_modules())
+    named = [name for name in act_scales if isinstance(layers.get(name), FP4Linear)]
+    for name in named:
+        layers[name].calibrate(float(torch.as_tensor(act_scales[name]).max()))
+    return len(named)

@@ -41,6 +41,7 @@ EXPORTED_SYMBOLS = (
     "samq_quant_fp4",
     "samq_gemm_fp4",
     "samq_linear_fp4",
+    "samq_linear_fp4_ex",
     "samq_linear_fp4_workspace_bytes",
     "samq_attn_window_prep",
     "samq_attn_rel_bias",
@@ -184,6 +185,11 @@ def load() -> ctypes.CDLL:
         c_void_p, c_void_p, c_int64,                                  # bias, residual, ldr
         c_int, c_void_p, c_int, c_int64,                              # activation, out, out_dtype, ldo
         c_void_p, c_size_t, c_void_p, c_void_p,                       # workspace, bytes, status, stream
+    ]
+    lib.samq_linear_fp4_ex.restype = c_int
+    lib.samq_linear_fp4_ex.argtypes = [
+        c_void_p, c_int, c_int64, c_float, c_void_p, c_int64, c_void_p,   # x, dtype, ldx, x_global_scale, W, ldw, w_scales
+        *lib.samq_linear_fp4.argtypes[6:],
     ]
     lib.samq_linear_fp4_workspace_bytes.restype = c_size_t
     lib.samq_linear_fp4_workspace_bytes.argtypes = [c_int, c_int64, c_int64]

@@ -72,7 +72,7 @@ int quant_fp4_dispatch(const void* x, int dtype, int64_t M, int64_t K, int64_t l
 int gemm_fp4_dispatch(const uint8_t* A, int64_t lda, const uint8_t* a_scales, const uint8_t* W, int64_t ldw, const uint8_t* w_scales,
                       int64_t M, int64_t N, int64_t K, int fmt, float alpha, const void* bias, const void* residual, int64_t ldr,
                       int activation, void* out, int out_dtype, int64_t ldo, int32_t* status, void* stream);
-int linear_fp4_dispatch(const void* x, int dtype, int64_t ldx, const uint8_t* W, int64_t ldw, const uint8_t* w_scales,
+int linear_fp4_dispatch(const void* x, int dtype, int64_t ldx, float x_global_scale, const uint8_t* W, int64_t ldw, const uint8_t* w_scales,
                         int64_t M, int64_t N, int64_t K, int fmt, float alpha, const void* bias, const void* residual, int64_t ldr,
                         int activation, void* out, int out_dtype, int64_t ldo, void* workspace, size_t workspace_bytes,
                         int32_t* status, void* stream);
@@ -276,7 +276,16 @@ int samq_linear_fp4(const void* x, int dtype, int64_t ldx, const uint8_t* W, int
                     int activation, void* out, int out_dtype, int64_t ldo, void* workspace, size_t workspace_bytes,
                     int32_t* status, void* stream)
 {
-    return samq::linear_fp4_dispatch(x, dtype, ldx, W, ldw, w_scales, M, N, K, format, alpha, bias, residual, ldr, activation,
+    return samq::linear_fp4_dispatch(x, dtype, ldx, 1.0f, W, ldw, w_scales, M, N, K, format, alpha, bias, residual, ldr, activation,
+                                     out, out_dtype, ldo, workspace, workspace_bytes, status, stream);
+}
+
+int samq_linear_fp4_ex(const void* x, int dtype, int64_t ldx, float x_global_scale, const uint8_t* W, int64_t ldw, const uint8_t* w_scales,
+                       int64_t M, int64_t N, int64_t K, int format, float alpha, const void* bias, const void* residual, int64_t ldr,
+                       int activation, void* out, int out_dtype, int64_t ldo, void* workspace, size_t workspace_bytes,
+                       int32_t* status, void* stream)
+{
+    return samq::linear_fp4_dispatch(x, dtype, ldx, x_global_scale, W, ldw, w_scales, M, N, K, format, alpha, bias, residual, ldr, activation,
                                      out, out_dtype, ldo, workspace, workspace_bytes, status, stream);
 }
 

@@ -31,6 +31,11 @@ inline bool known_format(int fmt) { return fmt == SAMQ_FP4_MX || fmt == SAMQ_FP4
 inline bool good_global_scale(float g) {
     return g >= 5.42101086e-20f /* 2^-64 */ && g <= 1.84467441e19f /* 2^64 */ && (__builtin_bit_cast(uint32_t, g) & 0x7FFFFFu) == 0;
 }
+inline int check_global_scale(int fmt, float g) {
+    if (!good_global_scale(g)) return fail(SAMQ_ERR_BAD_ARG, "global_scale must be a power of two between 2^-64 and 2^64");
+    if (fmt == SAMQ_FP4_MX && g != 1.0f) return fail(SAMQ_ERR_BAD_ARG, "mxfp4 has no global scale: its block scales reach every exponent");
+    return SAMQ_OK;
+}
 
 // Eight values to eight e2m1 codes, v[0] in the low nibble: round to nearest, ties to the even code,
 // magnitudes beyond 6 become 6 (the conversion instruction's definition).

@@ -52,6 +52,7 @@ struct SmallParams {
     const uint8_t* a_scales;                      // unless the kernel quantizes
     const uint8_t* w_scales;
     const void* x; int64_t ldx; int access_x;     // the activation, if the kernel quantizes it
+    float x_global_scale, inv_x_global_scale;
     int tmem_cols;
     float alpha;
     const void* bias;
@@ -177,9 +178,11 @@ __device__ __forceinline__ void quantize_batch(const SmallParams& p, const RowOf
         const int s = stage + b < p.stages ? stage + b : stage + b - p.stages;
         uint32_t amax = x[u].amax_bits();
         if constexpr (FMT == SAMQ_FP4_MX) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        const Scale sc = block_scale<FMT>(amax, 1.0f, 1.0f);
+        const Scale sc = block_scale<FMT>(amax, p.x_global_scale, p.inv_x_global_scale);
+        Chunk<T> held = x[u];
+        hold_far<FMT>(held, sc, p.x_global_scale);
         *reinterpret_cast<uint2*>(tiles + (size_t)s * st_bytes + W_BYTES + r * BK + ((uint32_t)(j * 8) ^ ((uint32_t)(r & 7) << 4))) =
-            encode_chunk<FMT>(x[u], sc, amax < 0x7F800000u);
+            encode_chunk<FMT>(held, sc, amax < 0x7F800000u);
         if (FMT == SAMQ_FP4_NV || (j & 1) == 0)
             sf[(size_t)(2 * s + 1) * Shape<FMT>::SF_BYTES + (block / 4) * TILE_BYTES + r * 16 + (block & 3)] =
                 (uint8_t)((kb + b) * KPAD + block * block_of(FMT) < p.K ? sc.byte : 0u);
@@ -500,14 +503,15 @@ int launch_form(int form, const Fp4Call& c, SmallParams& p, const CUtensorMap& m
     }
 }
 
-// x != nullptr: quantize it in the kernel
-int gemm_fp4_small(const Fp4Call& c, const void* x, int64_t ldx) {
+// x != nullptr: quantize it in the kernel, under x_global_scale
+int gemm_fp4_small(const Fp4Call& c, const void* x, int64_t ldx, float x_global_scale) {
     SmallParams p;
     p.M = (int)c.M; p.N = (int)c.N; p.K = (int)c.K;
     p.T = tile_rows(c.M);
     p.groups = (int)groups_of(c.fmt, c.K); p.a_scales = c.a_scales; p.w_scales = c.w_scales;
     const size_t esz = c.out_dtype == SAMQ_F32 ? 4 : 2;
     p.x = x; p.ldx = ldx; p.access_x = row_access(x, ldx * (int64_t)esz);
+    p.x_global_scale = x_global_scale; p.inv_x_global_scale = 1.0f / x_global_scale;
     p.alpha = c.epi.alpha; p.bias = c.epi.bias; p.residual = c.epi.residual; p.ldr = c.epi.ldr; p.out = c.epi.out; p.ldo = c.epi.ldo;
     p.gelu = c.gelu; p.status = c.status;
     CUtensorMap ma, mw;
@@ -558,7 +562,7 @@ int run_gemm(Fp4Call& c) {
     // which the pair kernel would compute two.  us, small / pair: 2048 x 2304 x 768 (288 CTAs) 8.6 / 10.3, 512 x 5120 x
     // 1280 (160) 9.1 / 10.3, 1000 x 5120 x 1280 (320) 14.3 / 12.3, 200 x 20000 x 768 (314) 11.8 / 10.3, 2048 x 5120 x 5120
     // (640) 40.8 / 33.8, 100 x 20000 x 5120 (157) 16.6 / 23.9
-    if (c.M <= MAX_T || (c.M + MAX_T - 1) / MAX_T * ((c.N + BW - 1) / BW) <= 2 * sm_count()) return gemm_fp4_small(c, nullptr, 0);
+    if (c.M <= MAX_T || (c.M + MAX_T - 1) / MAX_T * ((c.N + BW - 1) / BW) <= 2 * sm_count()) return gemm_fp4_small(c, nullptr, 0, 1.0f);
     const int esz = c.out_dtype == SAMQ_F32 ? 4 : 2;
     int rc = SAMQ_OK;
     memset(&c.map_out, 0, sizeof(c.map_out));
@@ -593,7 +597,7 @@ size_t linear_fp4_workspace(int fmt, int64_t M, int64_t K) {
     return (size_t)M * ((K + 31) / 32 * 16) + (size_t)((M + TILE_ROWS - 1) / TILE_ROWS * groups_of(fmt, K)) * TILE_BYTES;
 }
 
-int linear_fp4_dispatch(const void* x, int dtype, int64_t ldx, const uint8_t* W, int64_t ldw, const uint8_t* w_scales,
+int linear_fp4_dispatch(const void* x, int dtype, int64_t ldx, float x_global_scale, const uint8_t* W, int64_t ldw, const uint8_t* w_scales,
                         int64_t M, int64_t N, int64_t K, int fmt, float alpha, const void* bias, const void* residual, int64_t ldr,
                         int activation, void* out, int out_dtype, int64_t ldo, void* workspace, size_t workspace_bytes,
                         int32_t* status, void* stream)
@@ -602,7 +606,9 @@ int linear_fp4_dispatch(const void* x, int dtype, int64_t ldx, const uint8_t* W,
     int rc = check_call(c, M, N, K, fmt, W, ldw, w_scales, alpha, bias, residual, ldr, activation, out, out_dtype, ldo, status, stream);
     if (rc != SAMQ_OK) return rc;
     if (dtype != SAMQ_F16 && dtype != SAMQ_BF16 && dtype != SAMQ_F32) return fail(SAMQ_ERR_BAD_ARG, "unknown dtype %d", dtype);
-    if (M == 0) return SAMQ_OK;
+    rc = check_global_scale(fmt, x_global_scale);
+    if (rc != SAMQ_OK || M == 0) return rc;
+    c.epi.alpha = alpha * x_global_scale;
     if (x == nullptr) return fail(SAMQ_ERR_BAD_ARG, "x must not be null");
     if (ldx < K) return fail(SAMQ_ERR_BAD_ARG, "ldx smaller than K");
     if (reinterpret_cast<uintptr_t>(x) & (dtype == SAMQ_F32 ? 3 : 1)) return fail(SAMQ_ERR_ALIGNMENT, "x must be aligned to its elements");
@@ -614,15 +620,15 @@ int linear_fp4_dispatch(const void* x, int dtype, int64_t ldx, const uint8_t* W,
         // the host 3 us; 32, 5120 -> 10240 (7) 17.5 / 13.8; 8, 10240 -> 10240 (14) 17.4 / 18.2, 16 20.9 / 18.2; 8, 5120 ->
         // 20000 (20) 19.0 / 17.3; 1, 10240 -> 20000 (40) 32.5 / 26.3.
         const int64_t k_blocks = (K + KPAD - 1) / KPAD;
-        if (workspace == nullptr || workspace_bytes < need || (M + 8) * k_blocks <= FUSED_MOST) return gemm_fp4_small(c, x, ldx);
+        if (workspace == nullptr || workspace_bytes < need || (M + 8) * k_blocks <= FUSED_MOST) return gemm_fp4_small(c, x, ldx, x_global_scale);
         const int split = split_of(c, tile_rows(M));
-        if ((M + 8) * ((k_blocks + split - 1) / split) <= FUSED_MOST) return gemm_fp4_small(c, x, ldx);
+        if ((M + 8) * ((k_blocks + split - 1) / split) <= FUSED_MOST) return gemm_fp4_small(c, x, ldx, x_global_scale);
     }
     if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))
         return fail(SAMQ_ERR_WORKSPACE, "the 4-bit linear needs %zu bytes of 16-byte aligned workspace", need);
     uint8_t* codes = static_cast<uint8_t*>(workspace);
     uint8_t* scales = codes + (size_t)M * pitch;
-    rc = quant_fp4_dispatch(x, dtype, M, K, ldx, fmt, 1.0f, codes, pitch, scales, nullptr, stream);
+    rc = quant_fp4_dispatch(x, dtype, M, K, ldx, fmt, x_global_scale, codes, pitch, scales, nullptr, stream);
     if (rc != SAMQ_OK) return rc;
     c.A = codes; c.lda = pitch; c.a_scales = scales;
     return run_gemm(c);

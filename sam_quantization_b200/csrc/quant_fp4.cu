@@ -214,9 +214,8 @@ int quant_fp4_dispatch(const void* x, int dtype, int64_t M, int64_t K, int64_t l
     if (K > 2147483647LL - 256) return fail(SAMQ_ERR_TOO_LARGE, "K=%lld exceeds 2^31", (long long)K);
     if (dtype != SAMQ_F16 && dtype != SAMQ_BF16 && dtype != SAMQ_F32) return fail(SAMQ_ERR_BAD_ARG, "unknown dtype %d", dtype);
     if (!fp4::known_format(fmt)) return fail(SAMQ_ERR_BAD_ARG, "unknown 4-bit format %d", fmt);
-    if (!fp4::good_global_scale(global_scale)) return fail(SAMQ_ERR_BAD_ARG, "global_scale must be a power of two between 2^-64 and 2^64");
-    if (fmt == SAMQ_FP4_MX && global_scale != 1.0f) return fail(SAMQ_ERR_BAD_ARG, "mxfp4 has no global scale: its block scales reach every exponent");
-    if (M == 0) return SAMQ_OK;
+    const int rc = fp4::check_global_scale(fmt, global_scale);
+    if (rc != SAMQ_OK || M == 0) return rc;
     if (x == nullptr || codes == nullptr || scales == nullptr) return fail(SAMQ_ERR_BAD_ARG, "x, codes and scales must not be null");
     if (ldx < K) return fail(SAMQ_ERR_BAD_ARG, "ldx smaller than K");
     if (ldq < (K + 1) / 2) return fail(SAMQ_ERR_BAD_ARG, "ldq smaller than the %lld bytes of a row", (long long)((K + 1) / 2));

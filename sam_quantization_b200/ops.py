@@ -630,9 +630,13 @@ def gemm_fp4(a: Fp4Tensor, w: Fp4Tensor, bias: Optional[torch.Tensor] = None, re
 
 
 def linear_fp4(x: torch.Tensor, w: Fp4Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
-               activation: int = ACT_NONE, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """``x`` ([..., K]) quantized to the format of ``w`` (without a global scale) and multiplied with it:
-    ``act(q(x) @ w.T + bias) + residual`` -> [..., N], of ``x.dtype`` unless ``out_dtype`` says otherwise."""
+               activation: int = ACT_NONE, out_dtype: Optional[torch.dtype] = None, x_global_scale: float = 1.0) -> torch.Tensor:
+    """``x`` ([..., K]) quantized to the format of ``w`` and multiplied with it:
+    ``act(q(x) @ w.T + bias) + residual`` -> [..., N], of ``x.dtype`` unless ``out_dtype`` says otherwise.
+
+    ``x_global_scale`` (nvfp4) is the power of two under which ``x`` is quantized: magnitudes beyond 2688 times it saturate,
+    blocks below about 2^-6 times it lose resolution.  The default serves activations around 1; ``fp4_global_scale`` gives
+    the scale for a calibrated largest magnitude."""
     if x.shape[-1] != w.K:
         raise ValueError(f"x must be [..., {w.K}]")
     if not x.is_cuda:
@@ -654,7 +658,7 @@ def linear_fp4(x: torch.Tensor, w: Fp4Tensor, bias: Optional[torch.Tensor] = Non
     if two or (M + 8) * ((K + 255) // 256) > _lib.LINEAR_FP4_ONE_KERNEL_WORK:      # (the latter may use it)
         ws_bytes = lib.samq_linear_fp4_workspace_bytes(fcode, M, K)
         ws, kernels = x.new_empty((ws_bytes,), dtype=torch.uint8), 1 + two
-    _call(dev, "linear_fp4", 2.0 * M * N * K, lib.samq_linear_fp4, x2.data_ptr(), xcode, ldx, wc.data_ptr(), wc.stride(0), w.scales.data_ptr(),
+    _call(dev, "linear_fp4", 2.0 * M * N * K, lib.samq_linear_fp4_ex, x2.data_ptr(), xcode, ldx, x_global_scale, wc.data_ptr(), wc.stride(0), w.scales.data_ptr(),
           M, N, K, fcode, w.global_scale, _data_ptr(bias), _data_ptr(residual), ldr, activation, out.data_ptr(), code, N,
           _data_ptr(ws), ws_bytes, _status_ptr(dev), kernels=kernels)
     return out

@@ -10,6 +10,7 @@ import torch
 
 from oracle import fp4 as F
 from sam_quantization_b200 import _lib, ops
+from sam_quantization_b200.RTN_quantization import FP4Linear
 from tests.test_abi_cpu import built_library
 
 
@@ -125,3 +126,25 @@ def test_loops_of_whole_warps_wait_as_a_warp(name):
     with open(os.path.join(os.path.dirname(_lib.__file__), "csrc", name)) as f:
         code = re.sub(r"//[^\n]*", "", f.read())
     assert "mbar_wait_warp(" in code and not re.search(r"\bmbar_(try_)?wait\(", code)
+
+
+@pytest.mark.parametrize("change,code", [({"g": 3.0}, -1), ({"g": 0.0}, -1), ({"g": float("nan")}, -1), ({"g": 2.0 ** 65}, -1),
+                                         ({"fmt": _lib.FP4_MX, "g": 2.0}, -1), ({"x": None}, -1), ({"M": 0}, 0), ({"M": 33}, -5)])
+def test_layer_with_an_activation_scale_refuses_bad_arguments(change, code):
+    built_library()
+    lib = _lib.load()
+    args = dict(_calls(lib)["linear"][1])
+    args = dict(list(args.items())[:3] + [("g", 0.5)] + list(args.items())[3:])        # behind x, dtype and ldx
+    assert lib.samq_linear_fp4_ex(*dict(args, **change).values()) == code
+
+
+def test_layer_state_keeps_its_scales():
+    layer = FP4Linear(32, 16, True, "nvfp4")
+    assert layer.calibrate(1e-4, 5e3) == layer.act_global_scale == ops.fp4_global_scale(1e-4)
+    other = FP4Linear(32, 16, True, "nvfp4")
+    other.load_state_dict(layer.state_dict())
+    assert (other.act_global_scale, other.output_global_scale) == (layer.act_global_scale, ops.fp4_global_scale(5e3))
+    mx = FP4Linear(32, 16, True, "mxfp4")
+    assert mx.calibrate(1e-4) == 1.0
+    with pytest.raises(ValueError):
+        layer.calibrate(float("inf"))

@@ -357,3 +357,46 @@ def test_extreme_values_under_a_global_scale(cuda_device, dtype, g):
     x[10, 3], x[11, 40] = float("nan"), -float("inf")
     x = x.to(dtype)
     _check_quantized(x, ops.quantize_fp4(x.to(cuda_device), "nvfp4", global_scale=g, fake_quant=True), "nvfp4", g)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("k", [-20, -13, 9, 30])
+@pytest.mark.parametrize("M,N,K", [(1, 300, 1283), (8, 264, 300), (32, 640, 5120), (40, 200, 1280), (300, 130, 520), (4000, 1300, 300)])
+def test_layer_under_an_activation_scale(cuda_device, dtype, k, M, N, K):
+    """Activations of another power of two under a scale that follows them: the same codes, so the same output times that
+    power, bit for bit.  (K = 5120 and 32 rows quantize first, since the wrapper gives a workspace.)"""
+    x = _values(M, K, dtype).clamp(-2000, 2000).to(cuda_device)
+    w = ops.quantize_fp4((torch.randn(N, K, generator=torch.Generator().manual_seed(1)) * 0.02).to(cuda_device), global_scale=2.0 ** -14)["q"]
+    y = ops.linear_fp4(x, w, out_dtype=torch.float32)
+    z = ops.linear_fp4(x * 2.0 ** k, w, out_dtype=torch.float32, x_global_scale=2.0 ** k)
+    assert torch.equal(z, y * 2.0 ** k)
+    # output of the activation's type: one kernel up to 32 rows
+    b = (torch.randn(N, generator=torch.Generator().manual_seed(2)) * 2.0 ** k).to(dtype).to(cuda_device)
+    z = ops.linear_fp4(x * 2.0 ** k, w, bias=b, x_global_scale=2.0 ** k)
+    a = ops.quantize_fp4(x * 2.0 ** k, "nvfp4", global_scale=2.0 ** k)["q"]
+    assert _same_bytes(z, ops.gemm_fp4(a, w, bias=b, out_dtype=dtype))
+    ops.check_status()
+
+
+@pytest.mark.parametrize("M", [1, 8, 40, 200])
+@pytest.mark.parametrize("size", [1e-4, 1e4])
+def test_small_and_large_activations(cuda_device, M, size):
+    """Against the float product.  An element is off by at most half of the largest spacing (2, from 4 on) times its block's
+    scale, which is at most max / 6 * (1 + 2^-4) (and a block's largest, up to 6 / (1 - 2^-4) scales, by 0.4 of them)."""
+    K, N = 640, 96
+    x = (torch.randn(M, K, generator=torch.Generator().manual_seed(M)) * size).to(torch.bfloat16).to(cuda_device)
+    w, wv = _exact_operand(N, K, "nvfp4", cuda_device, 3)
+    g = ops.fp4_global_scale(float(x.abs().max()))
+    xv = x.double().cpu().numpy()
+    top = np.repeat(np.abs(xv).reshape(M, K // 16, 16).max(-1), 16, 1) * (1.0625 / 6)
+    for out_dtype in (torch.bfloat16, torch.float32):                      # one kernel and two, for few rows
+        y = ops.linear_fp4(x, w, out_dtype=out_dtype, x_global_scale=g).double().cpu().numpy()
+        bound = top @ np.abs(wv).T
+        want = xv @ wv.T
+        assert np.all(np.abs(y - want) <= bound + (HALF[out_dtype] + K * 2.0 ** -23) * (np.abs(xv) @ np.abs(wv).T + bound))
+        assert np.corrcoef(y.ravel(), want.ravel())[0, 1] > 0.98
+    with pytest.raises(RuntimeError, match="global_scale"):
+        ops.linear_fp4(x, w, x_global_scale=3.0)
+    m, _ = _exact_operand(N, K, "mxfp4", cuda_device, 3)
+    with pytest.raises(RuntimeError, match="mxfp4"):
+        ops.linear_fp4(x, m, x_global_scale=2.0)

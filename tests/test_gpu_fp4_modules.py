@@ -6,7 +6,8 @@ import torch
 from torch import nn
 
 from sam_quantization_b200 import checkpoint, ops, sam_encoder
-from sam_quantization_b200.RTN_quantization import FP4Linear, W8A8Linear, replace_linear_with_target_and_quantize
+from sam_quantization_b200.RTN_quantization import (FP4Linear, W8A8Linear, get_act_scales_sam, replace_linear_with_target_and_quantize,
+                                                    set_fp4_act_scales)
 
 pytestmark = pytest.mark.gpu
 FORMATS = ["mxfp4", "nvfp4"]
@@ -140,4 +141,50 @@ def test_a_block_of_a_rotated_network(cuda_device, M):
     assert s2 is stream2 and torch.equal(y2, h) and torch.equal(stream2, stream)
     with pytest.raises(ValueError):
         W8A8Linear.from_float(_linear(K, F, torch.float16, cuda_device), 8, act_quant="per_tensor").forward_rms_norm(x, w)
+    ops.check_status()
+
+
+@pytest.mark.parametrize("size", [1e-4, 1.0, 1e4])
+def test_calibrated_activation_scale(cuda_device, size, tmp_path):
+    lin = _linear(320, 264, torch.bfloat16, cuda_device)
+    model = nn.Module()
+    model.up = FP4Linear.from_float(lin, 4, weight_quant="nvfp4", act_quant="nvfp4", quantize_output=True)
+    model.other = FP4Linear.from_float(_linear(320, 264, torch.bfloat16, cuda_device), 4, weight_quant="mxfp4", act_quant="mxfp4")
+    x = (torch.randn(40, 320, generator=torch.Generator().manual_seed(1)) * size).to(torch.bfloat16).to(cuda_device)
+    assert set_fp4_act_scales(model, {"up": x.abs().amax(0).float().cpu(), "other": torch.ones(320), "head": torch.ones(3)}) == 2
+    layer = model.up
+    g = ops.fp4_global_scale(float(x.abs().max()))
+    assert layer.act_global_scale == g and model.other.act_global_scale == 1.0
+    y = ops.linear_fp4(x, layer.qweight, bias=layer.bias, x_global_scale=g)
+    layer.calibrate(x.abs().max(), y.abs().max())
+    out = ops.fp4_global_scale(float(y.abs().max()))
+    assert torch.equal(layer(x), ops.quantize_fp4(y, "nvfp4", global_scale=out, fake_quant=True)["fq"])
+    a, w = layer.act_quant(x).double(), layer.qweight.dequantize().double()
+    want = a @ w.t() + layer.bias.double()
+    bound = 320 * 2.0 ** -23 * (a.abs() @ w.abs().t())
+    assert ((y.double() - want).abs() <= bound + 2.0 ** -8 * (want.abs() + bound)).all()
+    assert ((a - x.double()).abs() <= x.abs().max().double() / 6 * 1.0625).all() and (a.count_nonzero() > 0.8 * a.numel())
+    # the scales travel with the checkpoint; one without them has scales of 1
+    torch.save(layer.state_dict(), str(tmp_path / "layer.pt"))
+    other = FP4Linear(320, 264, True, "nvfp4").to(cuda_device)
+    state = torch.load(str(tmp_path / "layer.pt"))
+    other.load_state_dict(state)
+    assert torch.equal(other(x), layer(x))
+    for key in ("act_global_scale", "output_global_scale"):
+        del state["_extra_state"][key]
+    other.load_state_dict(state)
+    assert other.act_global_scale == other.output_global_scale == 1.0
+    ops.check_status()
+
+
+def test_scales_of_a_float_encoder_reach_its_converted_layers(cuda_device):
+    model = sam_encoder.build_encoder("vit_b", seed=1, img_size=64, embed_dim=64, depth=2, num_heads=4, window_size=2, global_attn_indexes=(1,),
+                                      out_chans=32, device=cuda_device)
+    images = torch.rand(2, 3, 64, 64, generator=torch.Generator().manual_seed(0)).half().to(cuda_device)
+    scales = get_act_scales_sam(model, [images])
+    replace_linear_with_target_and_quantize(model, FP4Linear, 4, [], weight_quant="nvfp4", act_quant="nvfp4")
+    assert set_fp4_act_scales(model, scales) == len(scales) == 8
+    layer = model.image_encoder.blocks[1].mlp.lin2
+    assert layer.act_global_scale == ops.fp4_global_scale(float(scales["image_encoder.blocks.1.mlp.lin2"].max()))
+    assert model(images).isfinite().all()
     ops.check_status()
