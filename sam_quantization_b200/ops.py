@@ -544,17 +544,15 @@ class Fp4Tensor:
         return self.codes.device
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
-        """The values [rows, K], rounded once to ``dtype`` (off the hot path: plain torch)."""
+        """The values [rows, K], the global scale included, rounded once to ``dtype`` if that scale is a power of two (off the
+        hot path: plain torch)."""
         b = FP4_BLOCK[self.fmt]
         table = torch.tensor(_E2M1 + tuple(-v for v in _E2M1), device=self.device)
         v = table[torch.stack((self.codes & 15, self.codes >> 4), -1).flatten(1)[:, :self.K].long()]
         nb = (self.K + b - 1) // b
         byte = self.scales.permute(0, 3, 2, 1, 4).reshape(-1, 4 * self.scales.shape[1])[:self.rows, :nb]
-        if self.fmt == "mxfp4":
-            s = byte.contiguous().view(torch.float8_e8m0fnu).float()
-        else:
-            s = byte.contiguous().view(torch.float8_e4m3fn).float() * self.global_scale
-        return (v * s.repeat_interleave(b, 1)[:, :self.K]).to(dtype)
+        s = byte.contiguous().view(torch.float8_e8m0fnu if self.fmt == "mxfp4" else torch.float8_e4m3fn).float()
+        return (v * s.repeat_interleave(b, 1)[:, :self.K] * self.global_scale).to(dtype)
 
 
 def quantize_fp4(x: torch.Tensor, fmt: str = "nvfp4", global_scale: float = 1.0, fake_quant: bool = False) -> dict:

@@ -400,3 +400,15 @@ def test_small_and_large_activations(cuda_device, M, size):
     m, _ = _exact_operand(N, K, "mxfp4", cuda_device, 3)
     with pytest.raises(RuntimeError, match="mxfp4"):
         ops.linear_fp4(x, m, x_global_scale=2.0)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("g", [1.0, 0.25, 2.0 ** 20])
+def test_dequantized_values_are_what_the_product_multiplies(cuda_device, fmt, g):
+    a, av = _exact_operand(70, 45, fmt, cuda_device, 1)
+    a.global_scale = g
+    eye = ops.quantize_fp4(6 * torch.eye(45, device=cuda_device), fmt)["q"]              # blocks of a six: scale 1
+    y = ops.gemm_fp4(a, eye, out_dtype=torch.float32)
+    assert np.array_equal(a.dequantize().double().cpu().numpy(), av * g) and torch.equal(a.dequantize() * 6, y)
+    a.global_scale = 0.3                                                                 # any float in a product
+    assert torch.allclose(a.dequantize() * 6, ops.gemm_fp4(a, eye, out_dtype=torch.float32), rtol=4 * 2.0 ** -24, atol=0)
