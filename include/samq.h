@@ -334,6 +334,8 @@ int samq_gemm_fp4(const uint8_t* A, int64_t lda, const uint8_t* a_scales, const 
 #define SAMQ_LINEAR_FP4_ONE_KERNEL_ROWS 32
 #define SAMQ_LINEAR_FP4_ONE_KERNEL_WORK 256
 size_t samq_linear_fp4_workspace_bytes(int format, int64_t M, int64_t K);
+/* Kernels that samq_linear_fp4 launches for such a call with a workspace of that size (0: none): 1 or 2; 0 for no rows. */
+int samq_linear_fp4_kernels(int format, int dtype, int out_dtype, int64_t M, int64_t N, int64_t K, size_t workspace_bytes);
 int samq_linear_fp4(const void* x, int dtype, int64_t ldx, const uint8_t* W, int64_t ldw, const uint8_t* w_scales,
                     int64_t M, int64_t N, int64_t K, int format, float alpha, const void* bias, const void* residual, int64_t ldr,
                     int activation, void* out, int out_dtype, int64_t ldo, void* workspace, size_t workspace_bytes,

@@ -43,6 +43,7 @@ EXPORTED_SYMBOLS = (
     "samq_linear_fp4",
     "samq_linear_fp4_ex",
     "samq_linear_fp4_workspace_bytes",
+    "samq_linear_fp4_kernels",
     "samq_attn_window_prep",
     "samq_attn_rel_bias",
     "samq_attn_windowed",
@@ -193,6 +194,8 @@ def load() -> ctypes.CDLL:
     ]
     lib.samq_linear_fp4_workspace_bytes.restype = c_size_t
     lib.samq_linear_fp4_workspace_bytes.argtypes = [c_int, c_int64, c_int64]
+    lib.samq_linear_fp4_kernels.restype = c_int
+    lib.samq_linear_fp4_kernels.argtypes = [c_int, c_int, c_int, c_int64, c_int64, c_int64, c_size_t]
     lib.samq_gemm_set_pair_mode.restype = c_int
     lib.samq_gemm_set_pair_mode.argtypes = [c_int]
     lib.samq_attn_transpose_v.restype = c_int

@@ -77,6 +77,7 @@ int linear_fp4_dispatch(const void* x, int dtype, int64_t ldx, float x_global_sc
                         int activation, void* out, int out_dtype, int64_t ldo, void* workspace, size_t workspace_bytes,
                         int32_t* status, void* stream);
 size_t linear_fp4_workspace(int fmt, int64_t M, int64_t K);
+int linear_fp4_kernels(int fmt, int dtype, int out_dtype, int64_t M, int64_t N, int64_t K, size_t workspace_bytes);
 int attn_window14_dispatch(const void* qkv, const void* table, int table_rows, int dtype, int64_t windows, int heads, int head_dim,
                            float scale, void* out, int32_t* status, void* stream);
 int attn_window_dispatch(const void* qkv, int dtype, int64_t windows, int H, int W, int nh, int d,
@@ -292,6 +293,12 @@ int samq_linear_fp4_ex(const void* x, int dtype, int64_t ldx, float x_global_sca
 size_t samq_linear_fp4_workspace_bytes(int format, int64_t M, int64_t K)
 {
     return samq::fp4::known_format(format) && M > 0 && K > 0 ? samq::linear_fp4_workspace(format, M, K) : 0;
+}
+
+int samq_linear_fp4_kernels(int format, int dtype, int out_dtype, int64_t M, int64_t N, int64_t K, size_t workspace_bytes)
+{
+    if (!samq::fp4::known_format(format) || M <= 0 || N <= 0 || K <= 0) return 0;
+    return samq::linear_fp4_kernels(format, dtype, out_dtype, M, N, K, workspace_bytes);
 }
 
 int samq_gemm_set_pair_mode(int mode)

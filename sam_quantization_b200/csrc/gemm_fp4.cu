@@ -572,7 +572,27 @@ int run_gemm(Fp4Call& c) {
     return rc != SAMQ_OK ? rc : gemm_fp4_pair(c);
 }
 
+// Whether the layer quantizes its activation in the product's kernel.  Every CTA quantizes all rows of its share of K: where
+// that is much, and there is a workspace, the quantizer runs first.  us, one kernel / two: 32 rows, 1280 -> 5120 (a share of 5
+// blocks) 8.1 / 7.6, but the second launch costs the host 3 us; 32, 5120 -> 10240 (7) 17.5 / 13.8; 8, 10240 -> 10240 (14)
+// 17.4 / 18.2, 16 20.9 / 18.2; 8, 5120 -> 20000 (20) 19.0 / 17.3; 1, 10240 -> 20000 (40) 32.5 / 26.3.
+bool one_kernel(const Fp4Call& c, int dtype, bool has_workspace) {
+    if (c.M > FUSED_MAX_ROWS || dtype != c.out_dtype) return false;
+    const int64_t k_blocks = (c.K + KPAD - 1) / KPAD;
+    if (!has_workspace || (c.M + 8) * k_blocks <= FUSED_MOST) return true;
+    const int split = split_of(c, tile_rows(c.M));
+    return (c.M + 8) * ((k_blocks + split - 1) / split) <= FUSED_MOST;
+}
+
 }  // namespace
+
+size_t linear_fp4_workspace(int fmt, int64_t M, int64_t K);
+
+int linear_fp4_kernels(int fmt, int dtype, int out_dtype, int64_t M, int64_t N, int64_t K, size_t workspace_bytes) {
+    Fp4Call c;
+    c.M = M; c.N = N; c.K = K; c.fmt = fmt; c.out_dtype = out_dtype;
+    return one_kernel(c, dtype, workspace_bytes >= linear_fp4_workspace(fmt, M, K)) ? 1 : 2;
+}
 
 int quant_fp4_dispatch(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, int fmt, float global_scale,
                        uint8_t* codes, int64_t ldq, uint8_t* scales, void* fq, void* stream);
@@ -614,16 +634,7 @@ int linear_fp4_dispatch(const void* x, int dtype, int64_t ldx, float x_global_sc
     if (reinterpret_cast<uintptr_t>(x) & (dtype == SAMQ_F32 ? 3 : 1)) return fail(SAMQ_ERR_ALIGNMENT, "x must be aligned to its elements");
     const int64_t pitch = (K + 31) / 32 * 16;
     const size_t need = linear_fp4_workspace(fmt, M, K);
-    if (M <= FUSED_MAX_ROWS && dtype == out_dtype) {
-        // Every CTA quantizes all rows of its share of K: where that is much, and there is a workspace, the quantizer runs
-        // first.  us, one kernel / two: 32 rows, 1280 -> 5120 (a share of 5 blocks) 8.1 / 7.6, but the second launch costs
-        // the host 3 us; 32, 5120 -> 10240 (7) 17.5 / 13.8; 8, 10240 -> 10240 (14) 17.4 / 18.2, 16 20.9 / 18.2; 8, 5120 ->
-        // 20000 (20) 19.0 / 17.3; 1, 10240 -> 20000 (40) 32.5 / 26.3.
-        const int64_t k_blocks = (K + KPAD - 1) / KPAD;
-        if (workspace == nullptr || workspace_bytes < need || (M + 8) * k_blocks <= FUSED_MOST) return gemm_fp4_small(c, x, ldx, x_global_scale);
-        const int split = split_of(c, tile_rows(M));
-        if ((M + 8) * ((k_blocks + split - 1) / split) <= FUSED_MOST) return gemm_fp4_small(c, x, ldx, x_global_scale);
-    }
+    if (one_kernel(c, dtype, workspace != nullptr && workspace_bytes >= need)) return gemm_fp4_small(c, x, ldx, x_global_scale);
     if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))
         return fail(SAMQ_ERR_WORKSPACE, "the 4-bit linear needs %zu bytes of 16-byte aligned workspace", need);
     uint8_t* codes = static_cast<uint8_t*>(workspace);

@@ -655,7 +655,8 @@ def linear_fp4(x: torch.Tensor, w: Fp4Tensor, bias: Optional[torch.Tensor] = Non
     two = M > _lib.LINEAR_FP4_ONE_KERNEL_ROWS or code != xcode
     if two or (M + 8) * ((K + 255) // 256) > _lib.LINEAR_FP4_ONE_KERNEL_WORK:      # (the latter may use it)
         ws_bytes = lib.samq_linear_fp4_workspace_bytes(fcode, M, K)
-        ws, kernels = x.new_empty((ws_bytes,), dtype=torch.uint8), 1 + two
+        ws = x.new_empty((ws_bytes,), dtype=torch.uint8)
+        kernels = 2 if two else lib.samq_linear_fp4_kernels(fcode, xcode, code, M, N, K, ws_bytes)
     _call(dev, "linear_fp4", 2.0 * M * N * K, lib.samq_linear_fp4_ex, x2.data_ptr(), xcode, ldx, x_global_scale, wc.data_ptr(), wc.stride(0), w.scales.data_ptr(),
           M, N, K, fcode, w.global_scale, _data_ptr(bias), _data_ptr(residual), ldr, activation, out.data_ptr(), code, N,
           _data_ptr(ws), ws_bytes, _status_ptr(dev), kernels=kernels)

@@ -148,3 +148,14 @@ def test_layer_state_keeps_its_scales():
     assert mx.calibrate(1e-4) == 1.0
     with pytest.raises(ValueError):
         layer.calibrate(float("inf"))
+
+
+def test_kernels_of_a_layer():
+    built_library()
+    kernels = _lib.load().samq_linear_fp4_kernels
+    need = _lib.load().samq_linear_fp4_workspace_bytes
+    assert kernels(_lib.FP4_NV, _lib.BF16, _lib.BF16, 32, 640, 1280, 0) == 1
+    assert kernels(_lib.FP4_NV, _lib.BF16, _lib.F32, 1, 640, 1280, 1 << 20) == 2 and kernels(_lib.FP4_MX, _lib.F16, _lib.F16, 33, 640, 1280, 1 << 20) == 2
+    for ws, count in ((0, 1), (need(_lib.FP4_NV, 32, 20480) - 1, 1), (need(_lib.FP4_NV, 32, 20480), 2)):       # (a share of 10 blocks at least)
+        assert kernels(_lib.FP4_NV, _lib.BF16, _lib.BF16, 32, 40000, 20480, ws) == count
+    assert kernels(9, _lib.BF16, _lib.BF16, 1, 1, 1, 0) == 0 and kernels(_lib.FP4_NV, _lib.BF16, _lib.BF16, 0, 1, 1, 0) == 0

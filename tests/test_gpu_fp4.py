@@ -412,3 +412,15 @@ def test_dequantized_values_are_what_the_product_multiplies(cuda_device, fmt, g)
     assert np.array_equal(a.dequantize().double().cpu().numpy(), av * g) and torch.equal(a.dequantize() * 6, y)
     a.global_scale = 0.3                                                                 # any float in a product
     assert torch.allclose(a.dequantize() * 6, ops.gemm_fp4(a, eye, out_dtype=torch.float32), rtol=4 * 2.0 ** -24, atol=0)
+
+
+@pytest.mark.parametrize("M,N,K,out_dtype,kernels", [(1, 640, 1280, None, 1), (32, 640, 1280, None, 1), (32, 20000, 5120, None, 2), (1, 20000, 10240, None, 2),
+                                                     (32, 640, 5120, None, 1), (33, 640, 1280, None, 2), (1, 640, 1280, torch.float32, 2)])
+def test_launches_of_a_layer_are_counted(cuda_device, M, N, K, out_dtype, kernels):
+    """The count is the library's own choice of one or two kernels: the rule that its dispatch goes by."""
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(torch.bfloat16).to(cuda_device)
+    w = ops.quantize_fp4(torch.randn(N, K, device=cuda_device) * 0.02)["q"]
+    ops.reset_counters()
+    ops.linear_fp4(x, w, out_dtype=out_dtype)
+    assert ops.launch_count() == kernels
+    ops.check_status()
