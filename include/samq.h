@@ -318,7 +318,7 @@ int samq_quant_fp4(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, 
 
 /* y[m,n] = act(alpha * sum_k a[m,k] * w[n,k] + bias[n]) + residual[m,n]   on the tensor cores' block-scaled 4-bit kinds,
  * accumulated in fp32.  A [M, K] and W [N, K] are operands in the storage above, of one format; alpha is the product of
- * their global scales.  bias, residual, activation, out, ldo and status as in samq_gemm_i8 (out F16, BF16 or F32). */
+ * their global scales and has to be finite.  bias, residual, activation, out, ldo and status as in samq_gemm_i8 (out F16, BF16 or F32). */
 int samq_gemm_fp4(const uint8_t* A, int64_t lda, const uint8_t* a_scales, const uint8_t* W, int64_t ldw, const uint8_t* w_scales,
                   int64_t M, int64_t N, int64_t K, int format, float alpha, const void* bias, const void* residual, int64_t ldr,
                   int activation, void* out, int out_dtype, int64_t ldo, int32_t* status, void* stream);

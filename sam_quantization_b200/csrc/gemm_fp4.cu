@@ -18,6 +18,7 @@
 // 5.1: the latency of one pass (loads 1.1 us, stores 0.4, the rest launch and set-up); 1 x 40000 x 5120 from memory 30 us,
 // 4.2 TB/s.
 #include "fp4_gemm.cuh"
+#include <float.h>
 
 namespace samq {
 
@@ -537,6 +538,7 @@ int check_call(Fp4Call& c, int64_t M, int64_t N, int64_t K, int fmt, const uint8
     if (!known_format(fmt)) return fail(SAMQ_ERR_BAD_ARG, "unknown 4-bit format %d", fmt);
     if (activation != SAMQ_ACT_NONE && activation != SAMQ_ACT_GELU) return fail(SAMQ_ERR_BAD_ARG, "unknown activation %d", activation);
     if (out_dtype != SAMQ_F16 && out_dtype != SAMQ_BF16 && out_dtype != SAMQ_F32) return fail(SAMQ_ERR_BAD_ARG, "unknown out_dtype %d", out_dtype);
+    if (!(fabsf(alpha) <= FLT_MAX)) return fail(SAMQ_ERR_BAD_ARG, "alpha, the product of the global scales, must be finite");
     if (M > 2147483647LL - 256 || N > 2147483647LL - 256 || K > 2147483647LL - 256) return fail(SAMQ_ERR_TOO_LARGE, "GEMM dimension exceeds 2^31");
     if (M == 0) return SAMQ_OK;
     if (W == nullptr || w_scales == nullptr || out == nullptr) return fail(SAMQ_ERR_BAD_ARG, "operands, scales and out must not be null");
@@ -623,12 +625,12 @@ int linear_fp4_dispatch(const void* x, int dtype, int64_t ldx, float x_global_sc
                         int32_t* status, void* stream)
 {
     Fp4Call c;
-    int rc = check_call(c, M, N, K, fmt, W, ldw, w_scales, alpha, bias, residual, ldr, activation, out, out_dtype, ldo, status, stream);
+    int rc = check_global_scale(fmt, x_global_scale);
+    if (rc != SAMQ_OK) return rc;
+    rc = check_call(c, M, N, K, fmt, W, ldw, w_scales, alpha * x_global_scale, bias, residual, ldr, activation, out, out_dtype, ldo, status, stream);
     if (rc != SAMQ_OK) return rc;
     if (dtype != SAMQ_F16 && dtype != SAMQ_BF16 && dtype != SAMQ_F32) return fail(SAMQ_ERR_BAD_ARG, "unknown dtype %d", dtype);
-    rc = check_global_scale(fmt, x_global_scale);
-    if (rc != SAMQ_OK || M == 0) return rc;
-    c.epi.alpha = alpha * x_global_scale;
+    if (M == 0) return SAMQ_OK;
     if (x == nullptr) return fail(SAMQ_ERR_BAD_ARG, "x must not be null");
     if (ldx < K) return fail(SAMQ_ERR_BAD_ARG, "ldx smaller than K");
     if (reinterpret_cast<uintptr_t>(x) & (dtype == SAMQ_F32 ? 3 : 1)) return fail(SAMQ_ERR_ALIGNMENT, "x must be aligned to its elements");

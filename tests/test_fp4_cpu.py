@@ -159,3 +159,16 @@ def test_kernels_of_a_layer():
     for ws, count in ((0, 1), (need(_lib.FP4_NV, 32, 20480) - 1, 1), (need(_lib.FP4_NV, 32, 20480), 2)):       # (a share of 10 blocks at least)
         assert kernels(_lib.FP4_NV, _lib.BF16, _lib.BF16, 32, 40000, 20480, ws) == count
     assert kernels(9, _lib.BF16, _lib.BF16, 1, 1, 1, 0) == 0 and kernels(_lib.FP4_NV, _lib.BF16, _lib.BF16, 0, 1, 1, 0) == 0
+
+
+@pytest.mark.parametrize("name,change", [("gemm", {"alpha": float("inf")}), ("gemm", {"alpha": float("nan")}), ("linear", {"alpha": -float("inf")}),
+                                         ("linear", {"alpha": 2.0 ** 128})])
+def test_scales_whose_product_leaves_fp32_are_refused(name, change):
+    """An infinite alpha would turn the sums that are zero into NaN."""
+    built_library()
+    lib = _lib.load()
+    fn, args = _calls(lib)[name]
+    assert fn(*dict(args, **change).values()) == -1 and b"alpha" in lib.samq_last_error_string()
+    args = dict(_calls(lib)["linear"][1], alpha=2.0 ** 64)
+    args = dict(list(args.items())[:3] + [("g", 2.0 ** 64)] + list(args.items())[3:])
+    assert lib.samq_linear_fp4_ex(*args.values()) == -1 and b"alpha" in lib.samq_last_error_string()

@@ -424,3 +424,20 @@ def test_launches_of_a_layer_are_counted(cuda_device, M, N, K, out_dtype, kernel
     ops.linear_fp4(x, w, out_dtype=out_dtype)
     assert ops.launch_count() == kernels
     ops.check_status()
+
+
+@pytest.mark.parametrize("e", [-64, 63])
+def test_global_scales_at_their_ends(cuda_device, e):
+    """The product of two scales 2^64 is beyond fp32 and refused; 2^-64 and 2^-64 make a subnormal alpha, which is exact."""
+    a, av = _exact_operand(5, 100, "nvfp4", cuda_device, 1)
+    w, wv = _exact_operand(30, 100, "nvfp4", cuda_device, 2)
+    a.global_scale, w.global_scale = 2.0 ** e, 2.0 ** e
+    y = ops.gemm_fp4(a, w, out_dtype=torch.float32)
+    want = (av @ wv.T) * 2.0 ** (2 * e)
+    with np.errstate(over="ignore"):
+        assert np.array_equal(y.cpu().numpy(), want.astype(np.float32))
+    a.global_scale = w.global_scale = 2.0 ** 64
+    with pytest.raises(RuntimeError, match="alpha"):
+        ops.gemm_fp4(a, w, out_dtype=torch.float32)
+    with pytest.raises(RuntimeError, match="alpha"):
+        ops.linear_fp4(torch.ones(5, 100, device=cuda_device), w, x_global_scale=2.0 ** 64)
