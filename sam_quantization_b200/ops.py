@@ -519,7 +519,9 @@ def fp4_global_scale(absmax: float) -> float:
         raise ValueError("a global scale needs a finite largest magnitude")
     if absmax <= 0.0:
         return 1.0
-    return min(max(2.0 ** math.ceil(math.log2(absmax / (6.0 * 448.0))), 2.0 ** -64), 2.0 ** 64)
+    if absmax <= 6.0 * 448.0 * 2.0 ** -64:
+        return 2.0 ** -64
+    return min(2.0 ** math.ceil(math.log2(absmax / (6.0 * 448.0))), 2.0 ** 64)
 
 
 class Fp4Tensor:

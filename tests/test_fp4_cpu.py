@@ -172,3 +172,9 @@ def test_scales_whose_product_leaves_fp32_are_refused(name, change):
     args = dict(_calls(lib)["linear"][1], alpha=2.0 ** 64)
     args = dict(list(args.items())[:3] + [("g", 2.0 ** 64)] + list(args.items())[3:])
     assert lib.samq_linear_fp4_ex(*args.values()) == -1 and b"alpha" in lib.samq_last_error_string()
+
+
+@pytest.mark.parametrize("absmax,g", [(5e-324, 2.0 ** -64), (1e-320, 2.0 ** -64), (2688.0 * 2.0 ** -64, 2.0 ** -64), (2689.0 * 2.0 ** -64, 2.0 ** -63),
+                                      (2688.0 * 2.0 ** 63, 2.0 ** 63), (1e308, 2.0 ** 64)])
+def test_global_scale_at_its_ends(absmax, g):
+    assert ops.fp4_global_scale(absmax) == g
