@@ -325,7 +325,7 @@ int launch_rms_norm(const RmsNormParams& p, int e, bool odd, cudaStream_t st) {
     // 5 vectors: 1280 columns of a 16-bit type are one warp's, with no lane idle
     if (e == E && p.K <= 1024 * 5 * E) return launch_warps<T, E, 5>(p.K / E, p, st);
     // narrower accesses: more warps a row and fewer elements each
-    if (E == 8 && e == 4) return launch_warps<T, 4, 8>(p.K / 4, p, st);
+    if constexpr (E == 8) { if (e == 4) return launch_warps<T, 4, 8>(p.K / 4, p, st); }
     if (e >= 2 && p.K <= 1024 * 8 * 2) return launch_warps<T, 2, 8>(p.K / 2, p, st);
     // odd widths: pairs once single elements take more than a warp a row.  us, elements / pairs, fp16: 65536 x 255 38.9 / 45.0,
     // 32768 x 301 34.8 / 26.6, 32768 x 1279 131 / 82, 8192 x 8191 250 / 182
