@@ -62,6 +62,7 @@ _status_words = {}
 _launches = 0
 _timing_on = False
 _timing_records = []          # (kind, start_event, end_event, work, detail)
+_COUNTED_IN_OPS = ("gemm_i8", "gemm_fp4", "linear_fp4")      # kinds whose work is operations; the others' is bytes
 _valid_rows = {}              # (data_ptr, numel) of a row map -> rows that are not padding
 
 
@@ -84,7 +85,7 @@ def enable_kernel_timing(on: bool) -> None:
 
 def kernel_timing_summary() -> dict:
     """{kind: {"ms", "launches", "ops" | "bytes"}} summed over the bracketed launches
-    (synchronises).  ``ops`` = 2*M*N*K per GEMM, ``bytes`` = the algorithmic bytes of K1 (source rows
+    (synchronises).  ``ops`` = 2*M*N*K per GEMM (int8 or 4-bit, the 4-bit layer too), ``bytes`` = the algorithmic bytes of K1 (source rows
     actually read x element size + codes + scales).  The GEMM entry also carries ``bytes_alg`` (the
     algorithmic M*K + N*K + out_bytes*M*N) and ``"gemm_shapes"`` maps "KxN" to launches and total rows."""
     torch.cuda.synchronize()
@@ -95,7 +96,7 @@ def kernel_timing_summary() -> dict:
         ms = e0.elapsed_time(e1)
         d["ms"] += ms
         d["launches"] += 1
-        d["ops" if kind == "gemm_i8" else "bytes"] += work
+        d["ops" if kind in _COUNTED_IN_OPS else "bytes"] += work
         if kind == "gemm_i8" and detail is not None:
             M, N, K, out_bytes = detail
             d["bytes_alg"] = d.get("bytes_alg", 0.0) + M * K + N * K + out_bytes * M * N

@@ -441,3 +441,23 @@ def test_global_scales_at_their_ends(cuda_device, e):
         ops.gemm_fp4(a, w, out_dtype=torch.float32)
     with pytest.raises(RuntimeError, match="alpha"):
         ops.linear_fp4(torch.ones(5, 100, device=cuda_device), w, x_global_scale=2.0 ** 64)
+
+
+def test_kernel_timing_tells_operations_from_bytes(cuda_device):
+    M, N, K = 40, 64, 96
+    a, _ = _exact_operand(M, K, "nvfp4", cuda_device, 1)
+    w, _ = _exact_operand(N, K, "nvfp4", cuda_device, 2)
+    x = torch.zeros(M, K, dtype=torch.float16, device=cuda_device)
+    ops.enable_kernel_timing(True)
+    try:
+        ops.gemm_fp4(a, w)
+        ops.linear_fp4(x, w)
+        ops.quantize_fp4(x)
+        ops.rms_norm_quantize(x, x[0])
+        got = ops.kernel_timing_summary()
+    finally:
+        ops.enable_kernel_timing(False)
+    for kind in ("gemm_fp4", "linear_fp4"):
+        assert (got[kind]["ops"], got[kind]["bytes"], got[kind]["launches"]) == (2.0 * M * N * K, 0.0, 1)
+    assert got["quant_fp4"]["ops"] == got["rms_norm_quant"]["ops"] == 0.0
+    assert got["quant_fp4"]["bytes"] == M * K * 2 + M * K // 2 + 128 * 16 and got["rms_norm_quant"]["bytes"] == M * K * 3 + 4 * M
