@@ -188,3 +188,33 @@ def test_scales_of_a_float_encoder_reach_its_converted_layers(cuda_device):
     assert layer.act_global_scale == ops.fp4_global_scale(float(scales["image_encoder.blocks.1.mlp.lin2"].max()))
     assert model(images).isfinite().all()
     ops.check_status()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_every_layer_of_a_converted_encoder(cuda_device, fmt):
+    """Each layer on what the encoder gives it (input, residual, activation, output type), against its definition."""
+    model = sam_encoder.build_encoder("vit_b", seed=1, img_size=64, embed_dim=64, depth=2, num_heads=4, window_size=2, global_attn_indexes=(1,),
+                                      out_chans=32, device=cuda_device)
+    replace_linear_with_target_and_quantize(model, FP4Linear, 4, [], weight_quant=fmt, act_quant=fmt)
+    seen, held = [], {}
+
+    def before(layer, args, kw):
+        held[layer] = (args[0].clone(), {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in kw.items()})
+
+    for layer in model.modules():
+        if isinstance(layer, FP4Linear):
+            layer.register_forward_pre_hook(before, with_kwargs=True)
+            layer.register_forward_hook(lambda m, args, y: seen.append((m, *held[m], y.clone())))
+    model(torch.rand(2, 3, 64, 64, generator=torch.Generator().manual_seed(0)).half().to(cuda_device))
+    assert len(seen) == 8 and sum(kw.get("residual") is not None for _, _, kw, _ in seen) >= 2 and any(kw.get("activation") == "gelu" for _, _, kw, _ in seen)
+    for layer, x, kw, y in seen:
+        r = kw.get("residual")
+        want, bound = _reference(x.reshape(-1, layer.in_features), layer, None if r is None else r.reshape(-1, layer.out_features), kw.get("activation") == "gelu")
+        half = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}[y.dtype]
+        # the epilogue takes its bias in the output type: an fp16 bias under a bf16 output is off by half a step of it, up to 1.13
+        # times that behind the GELU (its slope)
+        if layer.bias.dtype != y.dtype:
+            bound = bound + 1.13 * half * layer.bias.double().abs()
+        # the alpha / bias step and the residual's addition: half a step of fp32 each
+        assert ((y.reshape(want.shape).double() - want).abs() <= bound + (half + 2.0 ** -22) * (want.abs() + bound) + 2.0 ** -25).all()
+    ops.check_status()
