@@ -14,9 +14,9 @@
 // scales straight into the shared-memory layout that the MMA reads, which saves a launch and the trip through memory.
 // Every N tile repeats that work, so it is for at most 32 rows.
 //
-// Measured (calls in a captured graph): 8 x 3840 x 1280 4.9 us, 1 x 5120 x 1280 with the quantization 5.5, 196 x 2304 x 768
-// 5.1: the latency of one pass (loads 1.1 us, stores 0.4, the rest launch and set-up); 1 x 40000 x 5120 from memory 30 us,
-// 4.2 TB/s.
+// Measured (20 calls in a captured graph, behind a flush of L2, on up to six weights in turn): 8 x 3840 x 1280 5.3 us, 1 x 5120 x
+// 1280 with the quantization 5.9, 196 x 2304 x 768 5.3: the latency of one pass (loads 1.1 us, stores 0.4, the rest launch and
+// set-up); 1 x 40000 x 5120 from memory 28 us, 4.1 TB/s.
 #include "fp4_gemm.cuh"
 #include <float.h>
 
@@ -442,9 +442,11 @@ int active_clusters(int split) {
     return known[dev][split] = 2 * n;
 }
 
-// Split K while SMs are idle, but leave a CTA four blocks of 256 columns at least: joining two halves costs about as much as
-// two more blocks (one token, 1280 -> 3840: 6.2 us whole, 6.6 us in two; 5120 -> 1280: 16.4 and 8.2 in five).  All clusters
-// are on the device at once: one token, 10240 -> 5120 takes 11.6 us in six and 20 in seven, 30 of whose 40 clusters fit.
+// Split K while SMs are idle, but leave a CTA four blocks of 256 columns at least: of five blocks two CTAs gain nothing (us, whole /
+// in two: 1 x 3840 x 1280 4.9 / 4.9, 8 x 3840 x 1280 5.3 / 5.6, 64 x 1280 x 2048 6.6 / 7.0), of twenty five gain much (1 x 1280 x
+// 5120 10.6 / 5.8 in five).  The border is not the best everywhere: shares of two blocks take 1 x 1280 x 2560 from 6.0 in two
+// to 4.9 in five.  All clusters are on the device at once: 1 x 5120 x 10240 takes 10.7 us in six and 13.4 in seven, 30 of whose 40
+// clusters fit.
 int split_of(const Fp4Call& c, int T) {
     const int64_t tiles = (c.N + BW - 1) / BW * ((c.M + MAX_T - 1) / MAX_T), k_blocks = (c.K + KPAD - 1) / KPAD;
     const int64_t room = (T <= 32 ? 2 : 1) * (int64_t)sm_count() / tiles;
@@ -561,9 +563,11 @@ int check_call(Fp4Call& c, int64_t M, int64_t N, int64_t K, int fmt, const uint8
 // the product of a checked call whose activation is set
 int run_gemm(Fp4Call& c) {
     // The small kernel while all of its CTAs are on the device at once (two an SM), and for a single tile of rows, of
-    // which the pair kernel would compute two.  us, small / pair: 2048 x 2304 x 768 (288 CTAs) 8.6 / 10.3, 512 x 5120 x
-    // 1280 (160) 9.1 / 10.3, 1000 x 5120 x 1280 (320) 14.3 / 12.3, 200 x 20000 x 768 (314) 11.8 / 10.3, 2048 x 5120 x 5120
-    // (640) 40.8 / 33.8, 100 x 20000 x 5120 (157) 16.6 / 23.9
+    // which the pair kernel would compute two.  us, small / pair: 2048 x 2304 x 768 (288 CTAs) 7.1 / 8.6, 512 x 5120 x
+    // 1280 (160) 7.7 / 8.1, 1000 x 5120 x 1280 (320) 11.6 / 10.1, 200 x 20000 x 768 (314) 9.7 / 8.6, 2048 x 5120 x 5120
+    // (640) 35.8 / 31.6, 100 x 20000 x 5120 (157) 14.4 / 22.4, 300 x 1280 x 5120 (30) 10.1 / 13.6.  The rule does not ask for K:
+    // 2048 x 2304 x 2560 10.4 / 10.8, but at K = 5120 the small kernel's 128 x 128 tiles lose some (2048 x 2304 15.4 / 14.6, 1500 x
+    // 2560 15.2 / 14.4, 1000 x 2560 14.6 / 13.9).
     if (c.M <= MAX_T || (c.M + MAX_T - 1) / MAX_T * ((c.N + BW - 1) / BW) <= 2 * sm_count()) return gemm_fp4_small(c, nullptr, 0, 1.0f);
     const int esz = c.out_dtype == SAMQ_F32 ? 4 : 2;
     int rc = SAMQ_OK;
@@ -576,8 +580,8 @@ int run_gemm(Fp4Call& c) {
 
 // Whether the layer quantizes its activation in the product's kernel.  Every CTA quantizes all rows of its share of K: where
 // that is much, and there is a workspace, the quantizer runs first.  us, one kernel / two: 32 rows, 1280 -> 5120 (a share of 5
-// blocks) 8.1 / 7.6, but the second launch costs the host 3 us; 32, 5120 -> 10240 (7) 17.5 / 13.8; 8, 10240 -> 10240 (14)
-// 17.4 / 18.2, 16 20.9 / 18.2; 8, 5120 -> 20000 (20) 19.0 / 17.3; 1, 10240 -> 20000 (40) 32.5 / 26.3.
+// blocks) 8.2 / 7.0, but the second launch costs the host 3 us; 32, 5120 -> 10240 (7) 17.3 / 13.7; 8, 10240 -> 10240 (14)
+// 17.1 / 18.4, 16 20.7 / 18.2; 8, 5120 -> 20000 (20) 18.5 / 17.4; 1, 10240 -> 20000 (40) 32.3 / 26.8; 32, 5120 -> 20000 33.1 / 17.0.
 bool one_kernel(const Fp4Call& c, int dtype, bool has_workspace) {
     if (c.M > FUSED_MAX_ROWS || dtype != c.out_dtype) return false;
     const int64_t k_blocks = (c.K + KPAD - 1) / KPAD;

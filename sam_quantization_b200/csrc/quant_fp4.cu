@@ -4,8 +4,8 @@
 //   nvfp4 : s = e4m3(max|x| / (6 g)) * g   per 16 columns, g a power of two
 //
 // Bound: HBM (a row of K 16-bit values is 2K bytes in and K/2 + K/16 or K/32 out, plus 2K for the values).  Measured with the
-// values: 32768 x 5120 bf16 mxfp4 114 us, 6.7 TB/s; nvfp4 125, where the instructions of twice the scales count (9 an
-// element); 32768 x 1280 / 1278 / 1279 fp16 nvfp4 35 / 50 / 58 us (see STAGED).
+// values: 32768 x 5120 bf16 mxfp4 114 us, 6.7 TB/s (above the rate of a copy, 6.55: the last writes are still in L2 at the end);
+// nvfp4 127-129, where the instructions of twice the scales count (9 an element); 32768 x 1280 / 1278 / 1279 fp16 nvfp4 35 / 50 / 58 us (see STAGED).
 #include "fp4.cuh"
 
 namespace samq {

@@ -457,7 +457,8 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, 
     Returns a dict with ``q`` int8 [..., K] (unless ``codes=False``) and ``scale`` fp32 [...], what ``gemm_i8`` takes,
     ``fq`` (with ``fake_quant``) the values ``q * scale`` in the tensor dtype and, with a ``residual``, ``residual``:
     the sum ``x + residual`` in the tensor dtype, in a new tensor or in ``residual_out`` (which may be ``residual`` or
-    ``x`` itself).  The normed value is quantized from fp32, without a rounding to the tensor dtype in between."""
+    ``x`` itself).  The normed value is quantized from fp32, without a rounding to the tensor dtype in between.  A ``weight``
+    of another dtype is converted to that of ``x`` (an fp32 weight is rounded to it), by a kernel in every call."""
     if not x.is_cuda:
         _require_cuda(x, "x")
     dtype, dev, shape = x.dtype, x.device, x.shape
@@ -611,7 +612,8 @@ def _linear_args(N: int, M: int, bias, residual, out_dtype, dev):
 def gemm_fp4(a: Fp4Tensor, w: Fp4Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
              activation: int = ACT_NONE, out_dtype: torch.dtype = torch.float16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``act(a @ w.T + bias) + residual`` -> [a.rows, w.rows] of ``out_dtype`` from two 4-bit operands of one format, on
-    the tensor cores' block-scaled kinds (``samq_gemm_fp4``)."""
+    the tensor cores' block-scaled kinds (``samq_gemm_fp4``).  A ``bias`` of another dtype is converted to ``out_dtype``, by a
+    kernel in every call."""
     ac, wc = a.codes, w.codes
     dev = ac.device
     if not ac.is_cuda:
@@ -637,7 +639,7 @@ def linear_fp4(x: torch.Tensor, w: Fp4Tensor, bias: Optional[torch.Tensor] = Non
 
     ``x_global_scale`` (nvfp4) is the power of two under which ``x`` is quantized: magnitudes beyond 2688 times it saturate,
     blocks below about 2^-6 times it lose resolution.  The default serves activations around 1; ``fp4_global_scale`` gives
-    the scale for a calibrated largest magnitude."""
+    the scale for a calibrated largest magnitude.  ``bias`` as in ``gemm_fp4``."""
     if x.shape[-1] != w.K:
         raise ValueError(f"x must be [..., {w.K}]")
     if not x.is_cuda:
