@@ -23,6 +23,7 @@ class FP4Linear(nn.Module):
 
     # callers that know this module may fuse the following GELU / residual add into the product
     supports_fused_epilogue = True
+    act_global_scale = output_global_scale = 1.0          # of pickled modules that are older than these
 
     def __init__(self, in_features, out_features, bias=True, weight_quant="nvfp4", quantize_output=False):
         super().__init__()

@@ -2,6 +2,7 @@
 (argument checks answer before any device work)."""
 import math
 import os
+import pickle
 import re
 
 import numpy as np
@@ -178,3 +179,11 @@ def test_scales_whose_product_leaves_fp32_are_refused(name, change):
                                       (2688.0 * 2.0 ** 63, 2.0 ** 63), (1e308, 2.0 ** 64)])
 def test_global_scale_at_its_ends(absmax, g):
     assert ops.fp4_global_scale(absmax) == g
+
+
+def test_pickled_layers_without_activation_scales_have_ones():
+    layer = FP4Linear(32, 16, True, "nvfp4")
+    for name in ("act_global_scale", "output_global_scale"):
+        del layer.__dict__[name]
+    again = pickle.loads(pickle.dumps(layer))
+    assert again.act_global_scale == again.output_global_scale == 1.0
