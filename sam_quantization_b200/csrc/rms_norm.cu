@@ -8,7 +8,7 @@
 // One pass: a row stays in registers between the two reductions (sum of squares, largest magnitude).  Bound: HBM,
 // 2 + 2 + 2 + 1 bytes an element of a 16-bit type (x, residual, h, q), 2 more for the dequantized values.  A row is kept
 // in its own type (60 registers instead of 110 of fp32: 66.3 -> 61.5 us).  Measured, 32768 x 1280 fp16 with residual and
-// values: 61.5 us, 6.1 TB/s; without either 28.6; 1278 columns (4-byte accesses) 74, 1279 80; bfloat16 within 5 % of these.
+// values: 61.5 us, 6.1 TB/s; without either 28.6; 1278 columns (4-byte accesses) 74, 1279 80; bfloat16 within 6 % of these.
 #include "common.cuh"
 #include <float.h>
 #include <type_traits>
